@@ -209,6 +209,68 @@ int ssd_tree_attention(const void* q, int64_t ldq, int64_t T, int64_t n_heads, i
                        const uint64_t* spec_mask, int64_t mask_words, int64_t kv_bound, void* out, int64_t ldo,
                        int dtype, void* workspace, int64_t workspace_bytes, uint32_t* status, void* stream);
 
+/* ------------------------------------------------------- 8-bit KV cache
+ * One layer of a key/value cache held in 8 bits: half the bytes of a bf16
+ * cache, for contexts and batches bound by them. No counterpart in the
+ * reference: an addition of this library. A row (one slot of one KV head) is
+ * head_dim e4m3 codes and one scale byte, the biased exponent e + 127 of a
+ * power of two: the smallest e with amax <= 448 * 2^e over the row's finite
+ * elements, limited to -40 .. 119. Element i stands for code[i] * 2^e, which
+ * bf16 and fp32 hold exactly. +-Inf is held as +-448 * 2^e, NaN as NaN.
+ * k, v: [n_kv_heads, max_slots, head_dim] codes, head stride `head_stride`
+ * bytes (a multiple of 16, base 16-byte aligned); k_scale, v_scale:
+ * [n_kv_heads, max_slots] bytes, head stride `scale_head_stride`. head_dim: a
+ * multiple of 16 up to 128. */
+typedef struct SsdKvQ8 {
+  void* k;
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int64_t head_stride;
+  int64_t scale_head_stride;
+  int64_t max_slots;
+  int64_t n_kv_heads;
+  int64_t head_dim;
+} SsdKvQ8;
+
+/* Rotary embedding and quantised cache write of T projected rows: q_out[t] =
+ * R(positions[t]) q[t] (dtype; q_out may be q; q NULL: cache write only), and
+ * the rows R(positions[t]) k[t] and v[t] of every KV head into cache slot
+ * slots[t]. R turns the first rot_dim elements of a head (even, 0 .. head_dim;
+ * 0: no rotation) by the fp32 tables rope_cos / rope_sin [max_pos, rot_dim/2],
+ * which carry any frequency scaling: pairs (i, i + rot_dim/2), or (2i, 2i+1)
+ * if `interleaved`. q / k / v: row strides in elements, heads contiguous. The
+ * slots of one call are distinct. A slot outside the cache is not written and
+ * a position outside the tables is taken as 0; either sets status bit 2. */
+int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t T,
+                         int64_t n_heads, const float* rope_cos, const float* rope_sin, int64_t max_pos,
+                         int64_t rot_dim, int interleaved, const int32_t* positions, const int32_t* slots,
+                         const SsdKvQ8* cache, void* q_out, int64_t ldqo, int dtype, uint32_t* status, void* stream);
+
+/* Rows of the cache as values: k_out[i] / v_out[i] (dtype, n_kv_heads *
+ * head_dim wide, row strides ldk / ldv; either may be NULL) = slot slots[i],
+ * or slot first + i if slots is NULL. A slot outside the cache gives zeros
+ * and sets status bit 2. */
+int ssd_kv_read_q8(const SsdKvQ8* cache, const int32_t* slots, int64_t first, int64_t n, void* k_out, int64_t ldk,
+                   void* v_out, int64_t ldv, int dtype, uint32_t* status, void* stream);
+
+/* ssd_tree_attention over the 8-bit cache: same rows, masks, slot ranges
+ * (prefix_start and prefix_len per row, mask bits from spec_base, kv_bound)
+ * and outputs (a row that sees nothing: zeros). dtype: of q and out. */
+int ssd_tree_attention_q8(const void* q, int64_t ldq, int64_t T, int64_t n_heads, const SsdKvQ8* cache,
+                          const int32_t* prefix_len, const int32_t* prefix_start, const int32_t* spec_base,
+                          const uint64_t* spec_mask, int64_t mask_words, int64_t kv_bound, void* out, int64_t ldo,
+                          int dtype, void* workspace, int64_t workspace_bytes, uint32_t* status, void* stream);
+
+/* ssd_kv_compact for the 8-bit cache: codes [n_layers, 2, n_kv_heads,
+ * max_slots, head_dim] and scale bytes [n_layers, 2, n_kv_heads, max_slots]
+ * with the given strides (bytes), moved together. */
+int ssd_kv_compact_q8(void* codes, uint8_t* scales, int64_t n_layers, int64_t layer_stride, int64_t kv_stride,
+                      int64_t head_stride, int64_t scale_layer_stride, int64_t scale_kv_stride,
+                      int64_t scale_head_stride, int64_t n_kv_heads, int64_t head_dim, int64_t max_slots,
+                      const int32_t* start, const int32_t* keep_slots, const int32_t* n_keep, int64_t max_keep,
+                      uint32_t* status, void* stream);
+
 /* Verify head: full-vocab lm_head fused with a per-row argmax (first index
  * of the maximum, as torch.argmax). Also writes the top-2 gap per row.
  * Replaces lm_head + argmax (subnetwork_draft.py:349, ssd/engine/verify.py:47,

@@ -44,6 +44,12 @@ class SsdLinearArgs(C.Structure):
                 ("k_cache", P), ("v_cache", P), ("cache_head_stride", I64), ("max_slots", I64)]
 
 
+class SsdKvQ8(C.Structure):
+    """include/ssd_b200.h SsdKvQ8: one layer of the 8-bit key/value cache."""
+    _fields_ = [("k", P), ("v", P), ("k_scale", P), ("v_scale", P), ("head_stride", I64), ("scale_head_stride", I64),
+                ("max_slots", I64), ("n_kv_heads", I64), ("head_dim", I64)]
+
+
 EPI_QKV = 16
 CHAIN_MAX = 6
 
@@ -71,6 +77,10 @@ SIGNATURES: dict[str, tuple] = {
                            P, I64, P, P, P]),
     "ssd_tree_attention": (I32, [P, I64, I64, I64, I64, I64, P, P, I64, I64, P, P, P, P, I64, I64, P, I64, I32, P,
                                  I64, P, P]),
+    "ssd_rope_kv_write_q8": (I32, [P, I64, P, I64, P, I64, I64, I64, P, P, I64, I64, I32, P, P, P, P, I64, I32, P, P]),
+    "ssd_kv_read_q8": (I32, [P, P, I64, I64, P, I64, P, I64, I32, P, P]),
+    "ssd_tree_attention_q8": (I32, [P, I64, I64, I64, P, P, P, P, P, I64, I64, P, I64, I32, P, I64, P, P]),
+    "ssd_kv_compact_q8": (I32, [P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, P, P, P, I64, P, P]),
     "ssd_linear_chain": (I32, [C.c_int32, P, I64, I32, P, I64, P, P]),
     "ssd_head_argmax": (I32, [P, I64, I64, I64, P, I64, P, P, P, I32, P, I64, P, P, P]),
     "ssd_head_topk": (I32, [P, I64, I64, I64, P, I64, P, I64, P, P, I32, P, I64, P, P, P]),

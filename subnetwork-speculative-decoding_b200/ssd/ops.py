@@ -250,6 +250,170 @@ def tree_attention(q, k_cache, v_cache, n_heads, n_kv, head_dim, prefix_len, out
            kv_bound, _p(out), out.stride(0), dtype_code(q.dtype), ws.ptr, ws.nbytes, _p(ws.status), _stream())
 
 
+# ------------------------------------------------------------- 8-bit KV cache
+class KVLayerQ8:
+    """One layer of an 8-bit key/value cache (SsdKvQ8): codes k, v
+    [n_kv, max_slots, head_dim] float8_e4m3fn and scale bytes k_scale, v_scale
+    [n_kv, max_slots] uint8 (views with any head stride; slots and elements
+    contiguous). Element i of a row stands for code[i] * 2^(scale - 127)."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_kv", "max_slots", "head_dim", "device", "_c", "_ref")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        n_kv, slots, hd = k.shape
+        if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+            raise ValueError("KVLayerQ8: codes must be float8_e4m3fn")
+        if k_scale.dtype != torch.uint8 or v_scale.dtype != torch.uint8:
+            raise ValueError("KVLayerQ8: scale bytes must be uint8")
+        if v.shape != k.shape or k_scale.shape != (n_kv, slots) or v_scale.shape != (n_kv, slots):
+            raise ValueError("KVLayerQ8: k, v [n_kv, max_slots, head_dim] and scales [n_kv, max_slots] do not match")
+        if (k.stride(1), k.stride(2)) != (hd, 1) or v.stride() != k.stride():
+            raise ValueError("KVLayerQ8: k and v need contiguous slots and equal strides")
+        if k_scale.stride(1) != 1 or v_scale.stride() != k_scale.stride():
+            raise ValueError("KVLayerQ8: k_scale and v_scale need contiguous slots and equal strides")
+        if not k.is_cuda or not (k.device == v.device == k_scale.device == v_scale.device):
+            raise ValueError("KVLayerQ8: the cache must live on one CUDA device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_kv, self.max_slots, self.head_dim, self.device = n_kv, slots, hd, k.device
+        # the stride of a single head is never used; give the C side one that cannot overlap
+        hs = k.stride(0) if n_kv > 1 else slots * hd
+        ss = k_scale.stride(0) if n_kv > 1 else slots
+        self._c = L.SsdKvQ8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), hs, ss, slots, n_kv, hd)
+        self._ref = C.byref(self._c)
+
+
+def _q8_ptr(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, dev, numel: int) -> Optional[int]:
+    """Pointer of a contiguous index / table argument of an 8-bit cache op."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.numel() < numel:
+        raise ValueError(f"{name}: expected >= {numel} contiguous {dtype} values on {dev}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _q8_rows(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, dev, rows: int, width: int) -> tuple:
+    """(pointer, row stride) of a [rows, width] activation argument."""
+    if t is None:
+        return None, 0
+    if t.dim() != 2 or t.dtype != dtype or t.device != dev or t.shape[0] < rows or t.shape[1] != width or \
+            (width > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: expected [>= {rows}, {width}] {dtype} rows on {dev}, got {tuple(t.shape)} {t.dtype} "
+                         f"on {t.device} with strides {t.stride()}")
+    return t.data_ptr(), t.stride(0)
+
+
+def _q8_call(name: str, dev, *args) -> None:
+    """Launch on the tensors' device and that device's current stream."""
+    if dev.index == torch.cuda.current_device():
+        L.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            L.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _q8_status(ws: Optional[Workspace], dev) -> Optional[int]:
+    if ws is None:
+        return None
+    if ws.status.device != dev:
+        raise ValueError(f"the workspace lives on {ws.status.device}, the cache on {dev}")
+    return ws.status.data_ptr()
+
+
+def rope_kv_write_q8(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, n_heads: int, n_kv: int,
+                     head_dim: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                     positions: Optional[torch.Tensor], slots: torch.Tensor, layer: KVLayerQ8,
+                     q_out: Optional[torch.Tensor], ws: Optional[Workspace] = None, *, T: Optional[int] = None,
+                     rot_dim: Optional[int] = None, interleaved: bool = False) -> None:
+    """q_out <- rotated q; rotated k and v, quantised, into cache slots
+    slots[t] (ssd_rope_kv_write_q8). q [T, n_heads * head_dim], k / v
+    [T, n_kv * head_dim], bf16 or fp32 rows of any stride; cos / sin
+    [max_pos, rot_dim / 2] fp32 (None: no rotation). rot_dim: how many elements
+    of a head turn (default: twice the tables' width); interleaved: pairs
+    (2i, 2i + 1) instead of (i, i + rot_dim / 2). q None: cache write only;
+    q_out may be q. The slots of one call must be distinct. Bad slots and
+    positions are reported by ws.check_status()."""
+    T = k.shape[0] if T is None else T
+    dev, dt = layer.device, k.dtype
+    if n_kv != layer.n_kv or head_dim != layer.head_dim:
+        raise ValueError(f"rope_kv_write_q8: cache of {layer.n_kv} heads x {layer.head_dim}, got {n_kv} x {head_dim}")
+    if rot_dim is None:
+        rot_dim = 0 if cos is None else 2 * cos.shape[1]
+    max_pos = 0
+    if rot_dim:
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] != rot_dim:
+            raise ValueError(f"rope_kv_write_q8: rot_dim {rot_dim} needs cos / sin tables [max_pos, {rot_dim // 2}]")
+        max_pos = cos.shape[0]
+    if q is not None and q_out is None:
+        raise ValueError("rope_kv_write_q8: q needs q_out")
+    pq, ldq = _q8_rows("q", q, dt, dev, T, n_heads * head_dim)
+    pk, ldk = _q8_rows("k", k, dt, dev, T, n_kv * head_dim)
+    pv, ldv = _q8_rows("v", v, dt, dev, T, n_kv * head_dim)
+    po, ldo = _q8_rows("q_out", q_out if q is not None else None, dt, dev, T, n_heads * head_dim)
+    f32, i32 = torch.float32, torch.int32
+    _q8_call("ssd_rope_kv_write_q8", dev, pq, ldq, pk, ldk, pv, ldv, T, n_heads,
+             _q8_ptr("cos", cos, f32, dev, 0) if rot_dim else None, _q8_ptr("sin", sin, f32, dev, 0) if rot_dim else None,
+             max_pos, rot_dim, 1 if interleaved else 0,
+             _q8_ptr("positions", positions, i32, dev, T) if rot_dim else None, _q8_ptr("slots", slots, i32, dev, T),
+             layer._ref, po, ldo, dtype_code(dt), _q8_status(ws, dev))
+
+
+def kv_read_q8(layer: KVLayerQ8, slots: Optional[torch.Tensor], k_out: Optional[torch.Tensor],
+               v_out: Optional[torch.Tensor], ws: Optional[Workspace] = None, *, first: int = 0,
+               n: Optional[int] = None) -> None:
+    """k_out / v_out [n, n_kv * head_dim] (bf16 or fp32; either None) <- the
+    values of slots[i], or of slot first + i if slots is None (ssd_kv_read_q8)."""
+    out = k_out if k_out is not None else v_out
+    if out is None:
+        raise ValueError("kv_read_q8: k_out or v_out is needed")
+    if n is None:
+        n = slots.numel() if slots is not None else out.shape[0]
+    dev, dt, width = layer.device, out.dtype, layer.n_kv * layer.head_dim
+    pk, ldk = _q8_rows("k_out", k_out, dt, dev, n, width)
+    pv, ldv = _q8_rows("v_out", v_out, dt, dev, n, width)
+    _q8_call("ssd_kv_read_q8", dev, layer._ref, _q8_ptr("slots", slots, torch.int32, dev, n), first, n, pk, ldk, pv, ldv,
+             dtype_code(dt), _q8_status(ws, dev))
+
+
+def tree_attention_q8(q: torch.Tensor, layer: KVLayerQ8, n_heads: int, n_kv: int, head_dim: int,
+                      prefix_len: torch.Tensor, out: torch.Tensor, ws: Workspace, *,
+                      spec_base: Optional[torch.Tensor] = None, spec_mask: Optional[torch.Tensor] = None,
+                      kv_bound: int = 0, T: Optional[int] = None,
+                      prefix_start: Optional[torch.Tensor] = None) -> None:
+    """tree_attention over an 8-bit cache layer (ssd_tree_attention_q8): row t
+    attends slots [prefix_start[t] (0 if None), prefix_len[t]) plus its mask
+    bits from spec_base[0]; a row that sees nothing gives zeros."""
+    T = q.shape[0] if T is None else T
+    dev, dt = layer.device, q.dtype
+    if n_kv != layer.n_kv or head_dim != layer.head_dim:
+        raise ValueError(f"tree_attention_q8: cache of {layer.n_kv} heads x {layer.head_dim}, got {n_kv} x {head_dim}")
+    pq, ldq = _q8_rows("q", q, dt, dev, T, n_heads * head_dim)
+    po, ldo = _q8_rows("out", out, dt, dev, T, n_heads * head_dim)
+    mw = spec_mask.shape[-1] if spec_mask is not None else 0
+    i32 = torch.int32
+    _q8_call("ssd_tree_attention_q8", dev, pq, ldq, T, n_heads, layer._ref,
+             _q8_ptr("prefix_len", prefix_len, i32, dev, T), _q8_ptr("prefix_start", prefix_start, i32, dev, T),
+             _q8_ptr("spec_base", spec_base, i32, dev, 1), _q8_ptr("spec_mask", spec_mask, torch.int64, dev, T * mw), mw,
+             kv_bound, po, ldo, dtype_code(dt), ws.ptr, ws.nbytes, _q8_status(ws, dev))
+
+
+def kv_compact_q8(codes: torch.Tensor, scales: torch.Tensor, start, keep_slots, n_keep, max_keep: int,
+                  ws: Optional[Workspace] = None) -> None:
+    """kv_compact for an 8-bit cache: codes [L, 2, n_kv, max_slots, head_dim]
+    float8_e4m3fn, scales [L, 2, n_kv, max_slots] uint8 (ssd_kv_compact_q8)."""
+    Ln, two, n_kv, slots, hd = codes.shape
+    dev, i32 = codes.device, torch.int32
+    if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8 or scales.shape != (Ln, two, n_kv, slots):
+        raise ValueError("kv_compact_q8: codes float8_e4m3fn [L, 2, n_kv, max_slots, head_dim], scales uint8 "
+                         "[L, 2, n_kv, max_slots]")
+    if two != 2 or not codes.is_cuda or scales.device != dev or codes.stride()[3:] != (hd, 1) or scales.stride(3) != 1:
+        raise ValueError("kv_compact_q8: K and V on one CUDA device with contiguous slots")
+    _q8_call("ssd_kv_compact_q8", dev, codes.data_ptr(), scales.data_ptr(), Ln, codes.stride(0), codes.stride(1),
+             codes.stride(2), scales.stride(0), scales.stride(1), scales.stride(2), n_kv, hd, slots,
+             _q8_ptr("start", start, i32, dev, 1), _q8_ptr("keep_slots", keep_slots, i32, dev, 1),
+             _q8_ptr("n_keep", n_keep, i32, dev, 1), max_keep, _q8_status(ws, dev))
+
+
 def head_argmax(x, w, out_idx, ws: Workspace, out_max=None, out_gap=None, T: Optional[int] = None,
                 in_norm: Optional[RowNorm] = None) -> None:
     T = x.shape[0] if T is None else T
