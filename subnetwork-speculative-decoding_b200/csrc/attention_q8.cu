@@ -306,6 +306,852 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
   return go(attn_q8_simt_kernel<bf16>, set_bf16);
 }
 
+// ------------------------------------------------------------ tensor cores
+// bf16 queries, head_dim 64 or 128, in the transposed form: keys are the
+// M = 128 rows of the tensor-core tiles, query rows their N columns, so that
+// a block of 128 keys costs what its N = 16 .. 160 query rows need and no
+// padding of few query rows to 128 (decode has 4 .. 132).
+//   S^T [128 keys x N]  = K8 [128 x hd] Q^T          (K8: codes as stored)
+//   O^T [hd x N]       += V8^T [hd x 128] P'^T       (V8: codes as stored)
+// The cache's codes feed the tensor cores untouched (kind::f8f6f4); what they
+// multiply is split into two e4m3 terms: a bf16 query element has 8
+// significant bits, q = (hi + lo) 2^eq with hi its nearest e4m3 and lo the
+// exact rest, and P' = hi + lo keeps 7 .. 8 bits (hi truncated, lo rounded).
+// Scales never touch the operands: a softmax thread owns one key (= TMEM
+// lane), so 2^ek is a factor of its scores and 2^ev an addend in its exponent,
+//   t = s log2 e + ev,  P' = 2^(t - M + kBias),  l += P' 2^-ev,
+// with M a per-row reference (power-of-two scale of O and l). M is the true
+// maximum of t over the row's first visible block and moves only when some t
+// exceeds it by kGrow (then O and l are rescaled), so the usual block needs no
+// reduction over keys, only one vote. P' <= 2^(kBias + kGrow) = 256 < 448; its
+// second term rounds at 2^-10, i.e. 2^-15 of the weight at the reference, and
+// l sums the unrounded P' in fp32 per thread until the end.
+//
+// A CTA = one KV head x up to 160 query rows (whole tokens) x one slice of the
+// key blocks that some row sees (a bitmap in shared memory: slot ranges of
+// other sequences in between are not read). Warps 0-3 take the first half of
+// the columns, 4-7 the second; warps 8 / 9 stream K / V blocks by TMA; lane 0
+// of warp 10 issues the MMAs, S^T(b + 1) and O(b) as each is ready; warp 11
+// zeroes V rows that no query row sees (0 * NaN) before they are used.
+constexpr int kQ8Keys = 128;
+constexpr int kQ8MaxRows = 160;       // query rows per CTA: TMEM holds 2 S^T + 1 O^T
+constexpr int kQ8Threads = 384;
+constexpr int kQ8MaxStages = 6;
+constexpr int kQ8MapWords = 256;      // bitmap of key blocks (units of 2^unit_shift blocks)
+constexpr float kQ8Bias = 5.f;
+constexpr float kQ8Grow = 3.f;
+constexpr float kQ8Unset = 1e30f;     // reference of a row that saw no key yet: every t exceeds it
+constexpr uint32_t kQ8ColO = 320;     // TMEM columns: S^T buffers at 0 and 160, O^T at 320
+
+struct AttnQ8Maps {
+  CUtensorMap k, v;  // [n_kv][max_slots][hd] bytes, box {hd, 128, 1}
+};
+
+struct AttnQ8Meta {
+  float rowc[kQ8MaxRows];                      // 2^eq scale log2 e per query row
+  float bias_ref[kQ8MaxRows];                  // kBias - M
+  float wmax[8][16];                           // growth path: per-warp column maxima
+  float alpha[2][16];                          // growth path: the chunk's factors of O and l
+  int len[kQ8MaxRows], start[kQ8MaxRows];      // per token
+  uint32_t vis[2][kQ8MaxRows][4];              // per block buffer and token: which of the block's keys it sees
+  uint32_t map[kQ8MapWords];
+  int max_start, min_len;                      // a block inside [max_start, min_len) is visible to every row
+  int first, count;                            // this CTA's units of the bitmap
+  int abort;
+  uint32_t tmem;
+  uint64_t k_full[kQ8MaxStages], k_empty[kQ8MaxStages], v_full[kQ8MaxStages], v_clean[kQ8MaxStages],
+      v_empty[kQ8MaxStages];
+  uint64_t s_full[2], s_free[2], p_full[2], p_free[2], vis_full[2], o_full;
+};
+
+__host__ __device__ constexpr int q8_p_bytes(int n) { return (n + 31) / 32 * 4096; }  // one term of one buffer
+__host__ __device__ constexpr int q8_fixed_smem(int hd, int n) {
+  return 1024 + 2 * n * hd + 4 * q8_p_bytes(n) + (int)sizeof(AttnQ8Meta);
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T, e4m3 in, fp32 accumulate.
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Shared-memory matrix descriptor; swizzle: 2 = 128 B, 4 = 64 B, 6 = 32 B.
+__device__ __forceinline__ uint64_t sdesc_q8(uint32_t saddr, uint32_t lbo, uint32_t sbo, uint32_t swizzle) {
+  uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(swizzle) << 61;
+  return d;
+}
+// e4m3 A/B, fp32 D, M x N; mn: both operands MN-major.
+__host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool mn) {
+  return (1u << 4) | (mn ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+__device__ __forceinline__ float q8_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two fp32 lanes per instruction.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Which of the slots kb .. kb + 63 a token sees: its range [start, len) plus
+// the mask bits (bit i = slot sb + i) below kv_end.
+__device__ __forceinline__ uint64_t q8_low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
+__device__ __forceinline__ uint64_t q8_seen_bits(int kb, int start, int len, const uint64_t* mask, int words, int sb,
+                                                 int kv_end) {
+  const uint64_t range = len > start ? q8_low_bits(len - kb) & ~q8_low_bits(start - kb) : 0ull;
+  const int64_t off = (int64_t)kb - sb;  // mask bit of slot kb
+  if (off <= -64 || off >= words * 64) return range;
+  const int w = off >= 0 ? (int)(off >> 6) : -1, sh = (int)(off - (int64_t)w * 64);  // 0 .. 63
+  const uint64_t lo = w >= 0 ? mask[w] : 0ull, up = w + 1 < words ? mask[w + 1] : 0ull;
+  const uint64_t spec = sh == 0 ? lo : (lo >> sh) | (up << (64 - sh));
+  return range | (spec & q8_low_bits(kv_end - kb));
+}
+
+// Walks the key blocks of this CTA's slice in ascending order.
+struct Q8Blocks {
+  const uint32_t* map;
+  uint32_t bits;
+  int word, shift, sub, unit;
+  __device__ Q8Blocks(const AttnQ8Meta& m, int unit_shift) : map(m.map), shift(unit_shift), sub(0), unit(0) {
+    word = m.first >> 5;
+    bits = m.count ? m.map[word] & (~0u << (m.first & 31)) : 0u;
+  }
+  __device__ __forceinline__ int next() {  // first slot of the next block
+    if (sub == 0) {
+      while (bits == 0u) bits = map[++word];
+      unit = word * 32 + __ffs(bits) - 1;
+      bits &= bits - 1;
+    }
+    const int block = (unit << shift) + sub;
+    sub = sub + 1 < (1 << shift) ? sub + 1 : 0;
+    return block * kQ8Keys;
+  }
+};
+
+template <int HD, int CH>
+__global__ void __launch_bounds__(kQ8Threads, 1)
+    attn_q8_tc_kernel(const __grid_constant__ AttnQ8Maps maps, const AttnQ8Args a, const int n_chunks,
+                      const int tok_per_group, const int stages, const int unit_shift) {
+  constexpr int TILE = kQ8Keys * HD;              // bytes of a K or V block
+  constexpr uint32_t SW = HD == 128 ? 2u : 4u;    // 128-byte or 64-byte swizzle: one atom row per cache row
+  constexpr uint32_t SBO = 8 * HD;                // 8 rows of HD bytes
+  extern __shared__ uint8_t q8_smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(q8_smem_raw) + 1023) & ~uintptr_t(1023));
+  const int N = 16 * n_chunks;
+  const int p_bytes = q8_p_bytes(N), atoms = (N + 31) / 32;
+  uint8_t* k_ring = sm;
+  uint8_t* v_ring = k_ring + stages * TILE;
+  uint8_t* p_buf = v_ring + stages * TILE;        // [2 buffers][hi, lo][keys / 8][atoms][8 keys x 32 rows]
+  uint8_t* q_hi = p_buf + 4 * p_bytes;            // [N][HD]
+  uint8_t* q_lo = q_hi + N * HD;
+  AttnQ8Meta& m = *reinterpret_cast<AttnQ8Meta*>(q_lo + N * HD);
+  volatile int* abort_flag = &m.abort;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x % a.n_kv, group = a.tiles - 1 - blockIdx.x / a.n_kv;  // longest causal rows first
+  const int split = blockIdx.y;
+  const int t0 = group * tok_per_group;
+  const int ntok = min(tok_per_group, a.T - t0);
+  const int nrows = ntok * a.G;
+  const bool two = n_chunks > CH;                 // the second warpgroup has columns
+
+  if (threadIdx.x == 0) {
+    m.max_start = 0;
+    m.min_len = INT32_MAX;
+    m.abort = 0;
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&m.k_full[i], 1);
+      mbar_init(&m.k_empty[i], 1);
+      mbar_init(&m.v_full[i], 1);
+      mbar_init(&m.v_clean[i], 1);
+      mbar_init(&m.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&m.s_full[i], 1);
+      mbar_init(&m.s_free[i], two ? 8 : 4);
+      mbar_init(&m.p_full[i], two ? 8 : 4);
+      mbar_init(&m.p_free[i], 1);
+      mbar_init(&m.vis_full[i], 1);
+    }
+    mbar_init(&m.o_full, 1);
+    fence_mbar_init();
+  }
+  for (int i = threadIdx.x; i < kQ8MapWords; i += kQ8Threads) m.map[i] = 0u;
+  if (warp == 10) {
+    tmem_alloc(&m.tmem, 512);
+    tmem_relinquish();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = m.tmem;
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- tokens: slot ranges and masks, the bitmap of blocks that some row sees
+  const int sb = a.mask ? a.spec_base[0] : 0;
+  for (int i = threadIdx.x; i < ntok; i += kQ8Threads) {
+    const int t = t0 + i;
+    const int start = max(a.prefix_start ? a.prefix_start[t] : 0, 0);
+    const int len = min(a.prefix_len[t], a.kv_end);
+    m.start[i] = start;
+    m.len[i] = len;
+    atomicMax(&m.max_start, start);
+    atomicMin(&m.min_len, len);
+    auto mark = [&](int lo, int hi) {  // slots lo .. hi
+      const int u0 = (lo / kQ8Keys) >> unit_shift, u1 = (hi / kQ8Keys) >> unit_shift;
+      for (int w = u0 >> 5; w <= u1 >> 5; ++w) {
+        uint32_t bits = ~0u;
+        if (w == u0 >> 5) bits &= ~0u << (u0 & 31);
+        if (w == u1 >> 5) bits &= ~0u >> (31 - (u1 & 31));
+        if ((m.map[w] & bits) != bits) atomicOr(&m.map[w], bits);
+      }
+    };
+    if (len > start) mark(start, len - 1);
+    for (int w = 0; w < a.mask_words; ++w) {
+      const uint64_t bits = a.mask[(int64_t)t * a.mask_words + w];
+      if (!bits) continue;
+      const int64_t lo = (int64_t)sb + w * 64 + __ffsll(bits) - 1, hi = (int64_t)sb + w * 64 + 63 - __clzll(bits);
+      if (hi < 0 || lo >= a.kv_end) continue;
+      mark((int)max(lo, (int64_t)0), (int)min(hi, (int64_t)a.kv_end - 1));
+    }
+  }
+  // ---- queries: two e4m3 terms per element, K-major rows of HD bytes. A row
+  // is LPR lanes x 8 elements; a lane loads the rows of a batch before it
+  // converts the first.
+  {
+    constexpr int LPR = HD / 8, RPP = kQ8Threads / LPR, BATCH = 4;
+    const bf16* qb = static_cast<const bf16*>(a.q);
+    const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0;
+    const int l8 = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
+    for (int rb = 0; rb < N; rb += RPP * BATCH) {
+      uint32_t raw[BATCH][4];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int r = rb + u * RPP + r0;
+        raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
+        if (r < nrows) {
+          const bf16* src = qb + (int64_t)(t0 + r / a.G) * a.ldq + (int64_t)(h * a.G + r % a.G) * HD + l8 * 8;
+          if (wide) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            raw[u][0] = v.x, raw[u][1] = v.y, raw[u][2] = v.z, raw[u][3] = v.w;
+          } else {
+            const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[u][e] = s16[2 * e] | (static_cast<uint32_t>(s16[2 * e + 1]) << 16);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int r = rb + u * RPP + r0;
+        float x[8], amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = __uint_as_float(raw[u][e] << 16);
+          x[2 * e + 1] = __uint_as_float(raw[u][e] & 0xffff0000u);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // Inf and NaN become the row's amax: they compare above every finite value
+          const float v = fabsf(x[e]);
+          amax = v <= 3.402823466e38f ? fmaxf(amax, v) : INFINITY;
+        }
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const bool fine = amax <= 3.402823466e38f;
+        const int byte = q8_scale_byte(fine ? amax : 0.f);
+        const float inv = q8_inv_scale(byte);
+        uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
+          const uint32_t c = q8_pack2(y0, y1);
+          const float2 back = q8_unpack2(c);
+          hi[e >> 2] |= c << (8 * (e & 3));
+          lo[e >> 2] |= q8_pack2(y0 - back.x, y1 - back.y) << (8 * (e & 3));
+        }
+        if (r < N) {
+          const int sw = HD == 128 ? (r & 7) : ((r >> 1) & 3);  // swizzled place of the lane's 8 bytes
+          const int at = r * HD + (((l8 >> 1) ^ sw) << 4) + (l8 & 1) * 8;
+          *reinterpret_cast<uint2*>(q_hi + at) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(q_lo + at) = make_uint2(lo[0], lo[1]);
+          if (l8 == 0) {
+            m.rowc[r] = fine ? q8_scale(byte) * (a.scale * 1.4426950408889634f) : __int_as_float(0x7fffffff);
+            m.bias_ref[r] = r < nrows ? kQ8Unset : -kQ8Unset;  // columns past the rows: P' = 0
+          }
+        }
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  __syncthreads();
+  // ---- this CTA's slice of the marked units
+  if (warp == 0) {
+    constexpr int PER = kQ8MapWords / 32;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += __popc(m.map[lane * PER + i]);
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += up;
+    }
+    const int total = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
+    const int u0 = (int)((int64_t)total * split / a.n_splits), u1 = (int)((int64_t)total * (split + 1) / a.n_splits);
+    if (lane == 0) m.count = u1 - u0;
+    if (u1 > u0 && u0 >= before && u0 < before + mine) {
+      int skip = u0 - before;
+      for (int i = 0; i < PER; ++i) {
+        uint32_t bits = m.map[lane * PER + i];
+        const int n = __popc(bits);
+        if (skip >= n) {
+          skip -= n;
+          continue;
+        }
+        for (; skip > 0; --skip) bits &= bits - 1;
+        m.first = (lane * PER + i) * 32 + __ffs(bits) - 1;
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  const int nblocks = m.count << unit_shift;
+  const int max_start = m.max_start, min_len = m.min_len;
+  const uint32_t p_s = smem_u32(p_buf);
+  auto give_up = [&] {
+    report_error(a.status, kErrWaitTimeout);
+    *abort_flag = 1;
+  };
+
+  float l[16 * CH];
+#pragma unroll
+  for (int i = 0; i < 16 * CH; ++i) l[i] = 0.f;
+  const int wg = warp >> 2, quarter = warp & 3;   // (softmax warps 0 .. 7)
+  const int my_chunks = wg == 0 ? CH : n_chunks - CH;
+  const int col_base = wg == 0 ? 0 : 16 * CH;
+  const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+
+  if (warp == 8 || warp == 9) {
+    if (lane == 0) {
+      const bool is_v = warp == 9;
+      uint64_t* full = is_v ? m.v_full : m.k_full;
+      uint64_t* empty = is_v ? m.v_empty : m.k_empty;
+      uint8_t* ring = is_v ? v_ring : k_ring;
+      const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+      const uint64_t pol = l2_policy_evict_first();
+      Q8Blocks it(m, unit_shift);
+      int st = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int b = 0; b < nblocks; ++b) {
+        if ((b >= stages && !mbar_wait(&empty[st], phase ^ 1u)) || *abort_flag) {
+          give_up();
+          break;
+        }
+        mbar_arrive_expect_tx(&full[st], TILE);
+        tma_load_3d(ring + st * TILE, map, &full[st], 0, it.next(), h, pol);
+        ++issued;
+        if (++st == stages) st = 0, phase ^= 1u;
+      }
+      if (*abort_flag)  // copies in flight land before the CTA leaves
+        for (int b = max(issued - stages, 0); b < issued; ++b) (void)mbar_wait(&full[b % stages], (b / stages) & 1);
+    }
+  } else if (warp == 10) {
+    if (lane == 0 && nblocks > 0) {
+      const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true);
+      const uint32_t kr = smem_u32(k_ring), vr = smem_u32(v_ring), qh = smem_u32(q_hi), ql = smem_u32(q_lo);
+      int nS = 0, nP = 0, sS = 0, sP = 0;
+      uint32_t phS = 0, phP = 0, idle = 0;
+      while (nP < nblocks) {
+        bool prog = false;
+        if (nS < nblocks && mbar_test(&m.k_full[sS], phS) &&
+            (nS < 2 || mbar_test(&m.s_free[nS & 1], ((nS >> 1) - 1) & 1))) {
+          tc_fence_after();
+          const uint32_t kb = kr + sS * TILE, d = tmem + (nS & 1) * kQ8MaxRows;
+#pragma unroll
+          for (int ks = 0; ks < HD / 32; ++ks)
+            umma_f8(d, sdesc_q8(kb + ks * 32, 16, SBO, SW), sdesc_q8(qh + ks * 32, 16, SBO, SW), id_s, ks > 0);
+#pragma unroll
+          for (int ks = 0; ks < HD / 32; ++ks)
+            umma_f8(d, sdesc_q8(kb + ks * 32, 16, SBO, SW), sdesc_q8(ql + ks * 32, 16, SBO, SW), id_s, 1u);
+          umma_commit(&m.s_full[nS & 1]);
+          umma_commit(&m.k_empty[sS]);
+          ++nS;
+          if (++sS == stages) sS = 0, phS ^= 1u;
+          prog = true;
+        }
+        if (nP < nS && mbar_test(&m.p_full[nP & 1], (nP >> 1) & 1) && mbar_test(&m.v_clean[sP], phP)) {
+          tc_fence_after();
+          // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
+          // M = 128 repeats the first (lanes 64 .. 127 are not read). P': MN-major, atoms of 32 rows x 8 keys.
+          const uint32_t vb = vr + sP * TILE, pb = p_s + (nP & 1) * 2 * p_bytes;
+          const uint32_t psbo = atoms * 256;
+#pragma unroll
+          for (int term = 0; term < 2; ++term)
+#pragma unroll
+            for (int kk = 0; kk < kQ8Keys / 32; ++kk)
+              umma_f8(tmem + kQ8ColO, sdesc_q8(vb + kk * 32 * HD, 0, SBO, SW),
+                      sdesc_q8(pb + term * p_bytes + kk * 4 * psbo, 256, psbo, 6u), id_o,
+                      (nP > 0 || term > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&m.p_free[nP & 1]);
+          umma_commit(&m.v_empty[sP]);
+          ++nP;
+          if (++sP == stages) sP = 0, phP ^= 1u;
+          prog = true;
+        }
+        idle = prog ? 0u : idle + 1u;
+        if (idle > kWaitLimit || *abort_flag) {
+          give_up();
+          break;
+        }
+      }
+    }
+    if (lane == 0) umma_commit(&m.o_full);
+  } else if (warp == 11) {
+    // Blocks that not every row sees whole: the keys that each token sees, for
+    // the softmax warps, and zeros in the V rows that none does.
+    Q8Blocks it(m, unit_shift);
+    int st = 0;
+    uint32_t phase = 0;
+    for (int b = 0; b < nblocks; ++b) {
+      const int kb = it.next();
+      const bool part = kb < max_start || kb + kQ8Keys > min_len;
+      bool bad = b >= 2 && !mbar_wait(&m.s_free[b & 1], ((b >> 1) - 1) & 1);  // vis[b & 1] was read for b - 2
+      uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
+      if (part) {
+        seen[0] = seen[1] = seen[2] = seen[3] = 0u;
+        for (int i = lane; i < ntok; i += 32) {
+          const uint64_t* mask = a.mask + (int64_t)(t0 + i) * a.mask_words;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint64_t v = q8_seen_bits(kb + 64 * half, m.start[i], m.len[i], mask, a.mask_words, sb, a.kv_end);
+            m.vis[b & 1][i][2 * half] = static_cast<uint32_t>(v);
+            m.vis[b & 1][i][2 * half + 1] = static_cast<uint32_t>(v >> 32);
+            seen[2 * half] |= static_cast<uint32_t>(v);
+            seen[2 * half + 1] |= static_cast<uint32_t>(v >> 32);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.vis_full[b & 1]);
+      bad = bad || !mbar_wait(&m.v_full[st], phase);
+      if (__any_sync(0xffffffffu, bad) || *abort_flag) {
+        if (lane == 0) give_up();
+        break;
+      }
+      if (part) {
+        bool wrote = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!((__reduce_or_sync(0xffffffffu, seen[i]) >> lane) & 1u)) {
+            uint4* row = reinterpret_cast<uint4*>(v_ring + st * TILE + (i * 32 + lane) * HD);
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) row[c] = make_uint4(0, 0, 0, 0);
+            wrote = true;
+          }
+        }
+        if (wrote) fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(&m.v_clean[st]);
+      if (++st == stages) st = 0, phase ^= 1u;
+    }
+  } else if (my_chunks > 0) {
+    // ---- softmax warps: thread = key
+    const int key = quarter * 32 + lane;
+    const int bar = 1 + wg;
+    const uint8_t* ksc = a.ks + (int64_t)h * a.scale_head_stride;
+    const uint8_t* vsc = a.vs + (int64_t)h * a.scale_head_stride;
+    const uint32_t p_at = (key >> 3) * atoms * 256 + (key & 7) * 32;
+    const uint32_t p_flip = (key >> 2) & 1;
+    Q8Blocks it(m, unit_shift);
+    int kb = 0, kbyte = 0, vbyte = 0;
+    auto fetch = [&] {
+      kb = it.next();
+      const bool in = kb + key < a.kv_end;
+      kbyte = in ? ksc[kb + key] : 0;
+      vbyte = in ? vsc[kb + key] : 0;
+    };
+    if (nblocks > 0) fetch();
+    bool bad = false;
+    for (int b = 0; b < nblocks; ++b) {
+      const bool full_block = kb >= max_start && kb + kQ8Keys <= min_len;
+      const float ck = q8_scale(kbyte);
+      const int vb = max(vbyte, kQ8MinScale);
+      const float ev = static_cast<float>(vb - 127);
+      const float inv_v = q8_inv_scale(vb);
+      const uint64_t ck2 = f2_pack(ck, ck), ev2 = f2_pack(ev, ev), iv2 = f2_pack(inv_v, inv_v);
+      if (b + 1 < nblocks) fetch();
+      // After a timeout the loop runs on without waiting: the warpgroup's barriers stay matched.
+      if (!bad && (*abort_flag || !mbar_wait(&m.s_full[b & 1], (b >> 1) & 1))) {
+        bad = true;
+        give_up();
+      }
+      if (!bad && (*abort_flag || !mbar_wait(&m.vis_full[b & 1], (b >> 1) & 1))) {
+        bad = true;
+        give_up();
+      }
+      tc_fence_after();
+      const uint32_t ts = tmem + (b & 1) * kQ8MaxRows + lane_base + col_base;
+      const uint32_t pb = p_s + (b & 1) * 2 * p_bytes + p_at;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (c < my_chunks) {
+          const int col = col_base + c * 16;
+          uint32_t vis = 0xffffu;
+          if (!full_block) {
+            vis = 0u;
+            const int tl = min((col + 15) / a.G, ntok - 1);
+            for (int t = col / a.G; t <= tl; ++t)
+              if ((m.vis[b & 1][t][quarter] >> lane) & 1u) {
+                const int lo = max(t * a.G - col, 0), hi = min((t + 1) * a.G - col, 16);
+                vis |= ((1u << hi) - 1u) & ~((1u << lo) - 1u);
+              }
+          }
+          float x[16];
+          tmem_ld16(ts + c * 16, x);
+          uint64_t w[8];
+          const ulonglong2* rc = reinterpret_cast<const ulonglong2*>(m.rowc + col);
+          const ulonglong2* rf = reinterpret_cast<const ulonglong2*>(m.bias_ref + col);
+          float top = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const ulonglong2 r = rc[j], f = rf[j];
+            w[2 * j] = f2_add(f2_fma(f2_mul(f2_pack(x[4 * j], x[4 * j + 1]), r.x), ck2, ev2), f.x);
+            w[2 * j + 1] = f2_add(f2_fma(f2_mul(f2_pack(x[4 * j + 2], x[4 * j + 3]), r.y), ck2, ev2), f.y);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f2_unpack(w[j], x[2 * j], x[2 * j + 1]);
+          if (!full_block) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = (vis >> j) & 1u ? x[j] : -INFINITY;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
+          if (named_bar_or(bar, 128, top > kQ8Bias + kQ8Grow)) {
+            // Some row's reference moves: column maxima of t over the block's 128 keys (halving the columns
+            // a lane holds at every step), then O, l and x of the chunk to the new references.
+            float t[16], v[16];
+            tmem_ld16(ts + c * 16, t);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              t[j] = fmaf(t[j] * m.rowc[col + j], ck, ev);
+              if (!((vis >> j) & 1u)) t[j] = -INFINITY;
+              v[j] = t[j];
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) {
+#pragma unroll
+              for (int j = 0; j < o; ++j) {
+                const bool up = lane & o;
+                const float give = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
+                v[j] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
+              }
+            }
+            v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
+            if (lane < 16) m.wmax[warp][lane] = v[0];
+            __syncwarp();
+            named_bar_sync(bar, 128);
+            if (threadIdx.x % 128 < 16) {
+              const int j = threadIdx.x % 128;
+              const float mx = fmaxf(fmaxf(m.wmax[wg * 4][j], m.wmax[wg * 4 + 1][j]),
+                                     fmaxf(m.wmax[wg * 4 + 2][j], m.wmax[wg * 4 + 3][j]));
+              const float old = m.bias_ref[col + j];
+              const bool move = mx + old > kQ8Bias + kQ8Grow;
+              const float now = move ? kQ8Bias - mx : old;
+              m.alpha[wg][j] = !move ? 1.f : old == kQ8Unset ? 0.f : exp2f(now - old);
+              m.bias_ref[col + j] = now;
+            }
+            __syncwarp();
+            named_bar_sync(bar, 128);
+            float alpha[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              alpha[j] = m.alpha[wg][j];
+              x[j] = t[j] + m.bias_ref[col + j];
+              l[c * 16 + j] *= alpha[j];
+            }
+            if (b > 0) {
+              if (!bad && !mbar_wait(&m.p_free[(b - 1) & 1], ((b - 1) >> 1) & 1)) {
+                bad = true;
+                give_up();
+              }
+              tc_fence_after();
+              float o[16];
+              tmem_ld16(tmem + kQ8ColO + lane_base + col, o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = alpha[j] == 0.f ? 0.f : o[j] * alpha[j];
+              tmem_st16(tmem + kQ8ColO + lane_base + col, o);
+              tmem_wait_st();
+            }
+          }
+          if (c == my_chunks - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&m.s_free[b & 1]);
+          }
+          if (c == 0 && b >= 2 && !bad && !mbar_wait(&m.p_free[b & 1], ((b >> 1) - 1) & 1)) {
+            bad = true;
+            give_up();
+          }
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] = q8_ex2(x[j]);
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            uint64_t acc = f2_pack(l[c * 16 + j], l[c * 16 + j + 1]);
+            acc = f2_fma(f2_pack(x[j], x[j + 1]), iv2, acc);
+            f2_unpack(acc, l[c * 16 + j], l[c * 16 + j + 1]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float t4[4], r4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              t4[e] = __uint_as_float(__float_as_uint(x[4 * j + e]) & 0xfff00000u);  // 4 significant bits
+              r4[e] = x[4 * j + e] - t4[e];
+            }
+            hi[j] = q8_pack4(t4[0], t4[1], t4[2], t4[3]);
+            lo[j] = q8_pack4(r4[0], r4[1], r4[2], r4[3]);
+          }
+          const uint32_t at = pb + (col >> 5) * 256 + ((((col >> 4) & 1u) ^ p_flip) << 4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]),
+                       "r"(hi[3])
+                       : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + p_bytes), "r"(lo[0]), "r"(lo[1]),
+                       "r"(lo[2]), "r"(lo[3])
+                       : "memory");
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.p_full[b & 1]);
+    }
+  }
+  // ---- results: l summed over the 128 keys' threads, O^T read back (lane = head dim)
+  __syncwarp();
+  float* s_l = reinterpret_cast<float*>(p_buf);  // [4][N]: the P buffers are free once every MMA retired
+  bool done = true;
+  if (warp < 8 && my_chunks > 0) {
+    done = mbar_wait(&m.o_full, 0);
+    if (!done && lane == 0) give_up();
+    tc_fence_after();
+  }
+  __syncthreads();
+  if (warp < 8 && my_chunks > 0) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (c < my_chunks) {
+        // 16 columns over 32 lanes: halve the columns a lane holds at every step
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = l[c * 16 + j];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+#pragma unroll
+          for (int j = 0; j < o; ++j) {
+            const bool up = lane & o;
+            const float give = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
+            v[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+        }
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
+        if (lane < 16) s_l[quarter * N + col_base + c * 16 + lane] = v[0];
+      }
+    }
+    named_bar_sync(1 + wg, 128);
+    const int d = quarter * 32 + lane;
+    const int64_t rec0 = ((int64_t)blockIdx.x * a.n_splits + split) * kQ8MaxRows;
+    float* o_part = a.part;
+    float* ml_part = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (c < my_chunks) {
+        const int col = col_base + c * 16;
+        float o[16];
+        if (nblocks > 0) {
+          tmem_ld16(tmem + kQ8ColO + lane_base + col, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int r = col + j;
+          if (r < nrows && d < HD) {
+            const float sum = (s_l[r] + s_l[N + r]) + (s_l[2 * N + r] + s_l[3 * N + r]);
+            if (a.n_splits == 1) {
+              const float inv = sum == 0.f ? 0.f : 1.f / sum;
+              static_cast<bf16*>(a.out)[(int64_t)(t0 + r / a.G) * a.ldo + (int64_t)(h * a.G + r % a.G) * HD + d] =
+                  f2bf(sum == 0.f ? 0.f : o[j] * inv);
+            } else {
+              if (sum != 0.f) o_part[(rec0 + r) * HD + d] = o[j];
+              if (d == 0) *reinterpret_cast<float2*>(ml_part + (rec0 + r) * 2) = make_float2(kQ8Bias - m.bias_ref[r], sum);
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 10) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the key slices' records {O 2^(..M), M, l} of one query row: one warp a
+// row, weights 2^(M_s - max M), in slice order. Slices that saw nothing have
+// l = 0 and no O.
+template <int HD>
+__global__ void __launch_bounds__(256) attn_q8_join_kernel(const AttnQ8Args a, const int tok_per_group) {
+  constexpr int DPL = HD / 32;
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x % a.n_kv, group = a.tiles - 1 - blockIdx.x / a.n_kv;
+  const int t0 = group * tok_per_group;
+  const int nrows = min(tok_per_group, a.T - t0) * a.G;
+  const int r = blockIdx.y * 8 + warp;
+  if (r >= nrows) return;
+  const float* o_part = a.part;
+  const float* ml_part = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD;
+  const int64_t rec0 = (int64_t)blockIdx.x * a.n_splits * kQ8MaxRows + r;
+  float top = -INFINITY;
+  for (int s = lane; s < a.n_splits; s += 32) {
+    const float2 ml = *reinterpret_cast<const float2*>(ml_part + (rec0 + (int64_t)s * kQ8MaxRows) * 2);
+    if (ml.y != 0.f) top = fmaxf(top, ml.x);
+  }
+  top = warp_max(top);
+  float sum = 0.f, acc[DPL];
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
+  for (int s0 = 0; s0 < a.n_splits; s0 += 32) {
+    float w = 0.f, ls = 0.f;
+    if (s0 + lane < a.n_splits) {
+      const float2 ml = *reinterpret_cast<const float2*>(ml_part + (rec0 + (int64_t)(s0 + lane) * kQ8MaxRows) * 2);
+      ls = ml.y;
+      w = ls != 0.f ? exp2f(ml.x - top) : 0.f;
+    }
+    sum += warp_sum(ls * w);
+    const uint32_t live = __ballot_sync(0xffffffffu, ls != 0.f);
+    const int n = min(32, a.n_splits - s0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      if ((live >> s) & 1u) {
+        const float* o = o_part + (rec0 + (int64_t)(s0 + s) * kQ8MaxRows) * HD + lane * DPL;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) acc[i] = fmaf(ws, o[i], acc[i]);
+      }
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  bf16* dst = static_cast<bf16*>(a.out) + (int64_t)(t0 + r / a.G) * a.ldo + (int64_t)(h * a.G + r % a.G) * HD + lane * DPL;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) dst[i] = f2bf(acc[i] * inv);
+}
+
+static int q8_tensor_map(const void* base, const SsdKvQ8& c, CUtensorMap* out) {
+  TensorMapEncodeFn encode = tensor_map_encoder();
+  if (!encode) return fail(SSD_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.max_slots, (cuuint64_t)c.n_kv_heads};
+  cuuint64_t strides[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.head_stride};
+  cuuint32_t box[3] = {(cuuint32_t)c.head_dim, (cuuint32_t)kQ8Keys, 1u};
+  cuuint32_t estr[3] = {1u, 1u, 1u};
+  const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SSD_ERR_CUDA, "ssd_tree_attention_q8: tensor map (%d)", (int)r);
+  return SSD_OK;
+}
+
+template <int HD>
+static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64_t workspace_bytes,
+                     cudaStream_t stream) {
+  // Query rows in as few groups of whole tokens as fit 160 columns, evenly.
+  int tpg = kQ8MaxRows / a.G;
+  a.tiles = (a.T + tpg - 1) / tpg;
+  tpg = (a.T + a.tiles - 1) / a.tiles;
+  a.tiles = (a.T + tpg - 1) / tpg;
+  const int chunks = (tpg * a.G + 15) / 16, ch = (chunks + 1) / 2;
+  const int64_t blocks = (int64_t)a.n_kv * a.tiles;
+  if (blocks > INT32_MAX) return fail(SSD_ERR_UNSUPPORTED, "ssd_tree_attention_q8: too many row groups");
+  const int key_blocks = (a.kv_end + kQ8Keys - 1) / kQ8Keys;
+  int shift = 0;
+  while ((key_blocks >> shift) >= kQ8MapWords * 32) ++shift;
+  // One CTA per SM; slices of at least two key blocks.
+  int64_t splits = device_sms() / blocks;
+  const int64_t by_len = (key_blocks + 1) / 2;
+  if (splits > by_len) splits = by_len;
+  if (splits < 1) splits = 1;
+  a.n_splits = (int)splits;
+  if (splits > 1) {
+    const int64_t need = kCounterBytes + blocks * splits * kQ8MaxRows * (HD + 2) * 4;
+    if (!workspace || need > workspace_bytes)
+      return fail(SSD_ERR_WORKSPACE, "ssd_tree_attention_q8: workspace too small (need %lld)", (long long)need);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+  }
+  AttnQ8Maps maps;
+  if (const int rc = q8_tensor_map(cache.k, cache, &maps.k)) return rc;
+  if (const int rc = q8_tensor_map(cache.v, cache, &maps.v)) return rc;
+  const int fixed = q8_fixed_smem(HD, chunks * 16);
+  int stages = (232448 - fixed) / (2 * kQ8Keys * HD);
+  if (stages > kQ8MaxStages) stages = kQ8MaxStages;
+  const size_t smem = (size_t)fixed + (size_t)stages * 2 * kQ8Keys * HD;
+  void (*const kerns[5])(const AttnQ8Maps, const AttnQ8Args, int, int, int, int) = {
+      attn_q8_tc_kernel<HD, 1>, attn_q8_tc_kernel<HD, 2>, attn_q8_tc_kernel<HD, 3>, attn_q8_tc_kernel<HD, 4>,
+      attn_q8_tc_kernel<HD, 5>};
+  static bool set = false;
+  if (!set) {
+    for (auto k : kerns) allow_max_dynamic_smem(k);
+    set = true;
+  }
+  int rc = launch_kernel("attn_q8_tc_kernel", kerns[ch - 1], dim3((unsigned)blocks, (unsigned)splits),
+                         dim3(kQ8Threads), smem, stream, 1u, 1u, maps, a, chunks, tpg, stages, shift);
+  if (rc || splits == 1) return rc;
+  return launch_kernel("attn_q8_join_kernel", attn_q8_join_kernel<HD>,
+                       dim3((unsigned)blocks, (unsigned)((tpg * a.G + 7) / 8)), dim3(256), 0, stream, 1u, 1u, a, tpg);
+}
+
 }  // namespace ssd
 
 using namespace ssd;
@@ -349,5 +1195,10 @@ extern "C" int ssd_tree_attention_q8(const void* q, int64_t ldq, int64_t T, int6
   a.ldo = ldo;
   a.status = status;
   a.scale = 1.0f / sqrtf((float)hd);
-  return launch_simt(a, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == SSD_BF16 && a.G <= kQ8MaxRows) {
+    if (hd == 128) return launch_tc<128>(a, *cache, workspace, workspace_bytes, s);
+    if (hd == 64) return launch_tc<64>(a, *cache, workspace, workspace_bytes, s);
+  }
+  return launch_simt(a, dtype, workspace, workspace_bytes, s);
 }
