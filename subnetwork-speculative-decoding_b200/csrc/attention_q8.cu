@@ -309,7 +309,7 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 // ------------------------------------------------------------ tensor cores
 // bf16 queries, head_dim 64 or 128, in the transposed form: keys are the
 // M = 128 rows of the tensor-core tiles, query rows their N columns, so that
-// a block of 128 keys costs what its N = 16 .. 160 query rows need and no
+// a block of 128 keys costs what its N = 16 .. 144 query rows need and no
 // padding of few query rows to 128 (decode has 4 .. 132).
 //   S^T [128 keys x N]  = K8 [128 x hd] Q^T          (K8: codes as stored)
 //   O^T [hd x N]       += V8^T [hd x 128] P'^T       (V8: codes as stored)
@@ -327,21 +327,21 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 // second term rounds at 2^-10, i.e. 2^-15 of the weight at the reference, and
 // l sums the unrounded P' in fp32 per thread until the end.
 //
-// A CTA = one KV head x up to 160 query rows (whole tokens) x one slice of the
+// A CTA = one KV head x up to 144 query rows (whole tokens) x one slice of the
 // key blocks that some row sees (a bitmap in shared memory: slot ranges of
 // other sequences in between are not read). Warps 0-3 take the first half of
 // the columns, 4-7 the second; warps 8 / 9 stream K / V blocks by TMA; lane 0
 // of warp 10 issues the MMAs, S^T(b + 1) and O(b) as each is ready; warp 11
 // zeroes V rows that no query row sees (0 * NaN) before they are used.
 constexpr int kQ8Keys = 128;
-constexpr int kQ8MaxRows = 160;       // query rows per CTA: TMEM holds 2 S^T + 1 O^T
+constexpr int kQ8MaxRows = 144;       // query rows per CTA: three ring stages fit next to their Q and P'
 constexpr int kQ8Threads = 384;
 constexpr int kQ8MaxStages = 6;
 constexpr int kQ8MapWords = 256;      // bitmap of key blocks (units of 2^unit_shift blocks)
 constexpr float kQ8Bias = 5.f;
 constexpr float kQ8Grow = 3.f;
 constexpr float kQ8Unset = 1e30f;     // reference of a row that saw no key yet: every t exceeds it
-constexpr uint32_t kQ8ColO = 320;     // TMEM columns: S^T buffers at 0 and 160, O^T at 320
+constexpr uint32_t kQ8ColO = 2 * kQ8MaxRows;  // TMEM columns: two S^T buffers, then O^T
 
 struct AttnQ8Maps {
   CUtensorMap k, v;  // [n_kv][max_slots][hd] bytes, box {hd, 128, 1}
@@ -350,8 +350,8 @@ struct AttnQ8Maps {
 struct AttnQ8Meta {
   float rowc[kQ8MaxRows];                      // 2^eq scale log2 e per query row
   float bias_ref[kQ8MaxRows];                  // kBias - M
-  float wmax[8][16];                           // growth path: per-warp column maxima
-  float alpha[2][16];                          // growth path: the chunk's factors of O and l
+  float wmax[4][kQ8MaxRows];                   // growth path: column maxima of a warp's 32 keys
+  float alpha[kQ8MaxRows];                     // growth path: factors of O and l
   int len[kQ8MaxRows], start[kQ8MaxRows];      // per token
   uint32_t vis[2][kQ8MaxRows][4];              // per block buffer and token: which of the block's keys it sees
   uint32_t map[kQ8MapWords];
@@ -361,7 +361,7 @@ struct AttnQ8Meta {
   uint32_t tmem;
   uint64_t k_full[kQ8MaxStages], k_empty[kQ8MaxStages], v_full[kQ8MaxStages], v_clean[kQ8MaxStages],
       v_empty[kQ8MaxStages];
-  uint64_t s_full[2], s_free[2], p_full[2], p_free[2], vis_full[2], o_full;
+  uint64_t s_full[2], s_free[2], p_full[2], p_free[2], vis_full[2], q_ready, o_full;
 };
 
 __host__ __device__ constexpr int q8_p_bytes(int n) { return (n + 31) / 32 * 4096; }  // one term of one buffer
@@ -458,6 +458,214 @@ struct Q8Blocks {
   }
 };
 
+// The CTA's query rows as two e4m3 terms per element, K-major rows of HD bytes
+// (by the eight softmax warps). A row is LPR lanes x 8 elements; a lane loads
+// the rows of a batch before it converts the first.
+template <int HD>
+__device__ __forceinline__ void q8_queries(const AttnQ8Args& a, AttnQ8Meta& m, uint8_t* q_hi, uint8_t* q_lo, int N,
+                                           int nrows, int t0, int h) {
+  constexpr int LPR = HD / 8, RPP = 256 / LPR, BATCH = 4;
+  const bf16* qb = static_cast<const bf16*>(a.q);
+  const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0;
+  const int l8 = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
+  for (int rb = 0; rb < N; rb += RPP * BATCH) {
+    uint32_t raw[BATCH][4];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int r = rb + u * RPP + r0;
+      raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
+      if (r < nrows) {
+        const bf16* src = qb + (int64_t)(t0 + r / a.G) * a.ldq + (int64_t)(h * a.G + r % a.G) * HD + l8 * 8;
+        if (wide) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src);
+          raw[u][0] = v.x, raw[u][1] = v.y, raw[u][2] = v.z, raw[u][3] = v.w;
+        } else {
+          const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raw[u][e] = s16[2 * e] | (static_cast<uint32_t>(s16[2 * e + 1]) << 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int r = rb + u * RPP + r0;
+      float x[8], amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(raw[u][e] << 16);
+        x[2 * e + 1] = __uint_as_float(raw[u][e] & 0xffff0000u);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // Inf and NaN become the row's amax: they compare above every finite value
+        const float v = fabsf(x[e]);
+        amax = v <= 3.402823466e38f ? fmaxf(amax, v) : INFINITY;
+      }
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      const bool fine = amax <= 3.402823466e38f;
+      const int byte = q8_scale_byte(fine ? amax : 0.f);
+      const float inv = q8_inv_scale(byte);
+      uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
+        const uint32_t c = q8_pack2(y0, y1);
+        const float2 back = q8_unpack2(c);
+        hi[e >> 2] |= c << (8 * (e & 3));
+        lo[e >> 2] |= q8_pack2(y0 - back.x, y1 - back.y) << (8 * (e & 3));
+      }
+      if (r < N) {
+        const int sw = HD == 128 ? (r & 7) : ((r >> 1) & 3);  // swizzled place of the lane's 8 bytes
+        const int at = r * HD + (((l8 >> 1) ^ sw) << 4) + (l8 & 1) * 8;
+        *reinterpret_cast<uint2*>(q_hi + at) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(q_lo + at) = make_uint2(lo[0], lo[1]);
+        if (l8 == 0) {
+          m.rowc[r] = fine ? q8_scale(byte) * (a.scale * 1.4426950408889634f) : __int_as_float(0x7fffffff);
+          m.bias_ref[r] = r < nrows ? kQ8Unset : -kQ8Unset;  // columns past the rows: P' = 0
+        }
+      }
+    }
+  }
+}
+
+// Visibility of the 16 columns from `col` for the thread's key (bit j = column
+// col + j), from the block's per-token key masks.
+__device__ __forceinline__ uint32_t q8_chunk_vis(const AttnQ8Meta& m, int buf, int col, int G, int ntok, int quarter,
+                                                 int lane) {
+  uint32_t vis = 0u;
+  const int last = min((col + 15) / G, ntok - 1);
+  for (int t = col / G; t <= last; ++t)
+    if ((m.vis[buf][t][quarter] >> lane) & 1u) {
+      const int lo = max(t * G - col, 0), hi = min((t + 1) * G - col, 16);
+      vis |= ((1u << hi) - 1u) & ~((1u << lo) - 1u);
+    }
+  return vis;
+}
+
+// One halving step of a reduction of 16 columns over 32 lanes: afterwards
+// lane i < 16 (and i + 16) holds column i's maximum (or sum) in v[0].
+template <bool MAX>
+__device__ __forceinline__ float q8_columns_reduce(float* v, int lane) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+#pragma unroll
+    for (int j = 0; j < o; ++j) {
+      const bool up = lane & o;
+      const float give = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
+      const float got = __shfl_xor_sync(0xffffffffu, give, o);
+      v[j] = MAX ? fmaxf(keep, got) : keep + got;
+    }
+  }
+  const float got = __shfl_xor_sync(0xffffffffu, v[0], 16);
+  return MAX ? fmaxf(v[0], got) : v[0] + got;
+}
+
+// Some of the warpgroup's references move: column maxima of t over the
+// block's 128 keys, new references and factors into shared memory, O's columns
+// rescaled. `pv_done` has completed `parity` once the previous block's P V has
+// retired (NULL: first block). Returns false on a timeout. All 128 threads of
+// the warpgroup call it; out of line, as most blocks do not need it.
+__device__ __noinline__ bool q8_move_references(AttnQ8Meta& m, uint32_t ts, uint32_t to, int col_base, int chunks,
+                                                int wg, float ck, float ev, bool part, int buf, int G, int ntok,
+                                                uint64_t* pv_done, uint32_t parity) {
+  const int tid = threadIdx.x & 127, quarter = tid >> 5, lane = tid & 31;
+  for (int c = 0; c < chunks; ++c) {
+    const int col = col_base + c * 16;
+    const uint32_t vis = part ? q8_chunk_vis(m, buf, col, G, ntok, quarter, lane) : 0xffffu;
+    float t[16];
+    tmem_ld16(ts + c * 16, t);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      t[j] = fmaf(t[j] * m.rowc[col + j], ck, ev);
+      if (!((vis >> j) & 1u)) t[j] = -INFINITY;
+    }
+    const float top = q8_columns_reduce<true>(t, lane);
+    if (lane < 16) m.wmax[quarter][col + lane] = top;
+  }
+  __syncwarp();
+  named_bar_sync(1 + wg, 128);
+  if (tid < 16 * chunks) {
+    const int r = col_base + tid;
+    const float mx = fmaxf(fmaxf(m.wmax[0][r], m.wmax[1][r]), fmaxf(m.wmax[2][r], m.wmax[3][r]));
+    const float old = m.bias_ref[r];
+    const bool move = mx + old > kQ8Bias + kQ8Grow;
+    const float now = move ? kQ8Bias - mx : old;
+    m.alpha[r] = !move ? 1.f : old == kQ8Unset ? 0.f : exp2f(now - old);
+    m.bias_ref[r] = now;
+  }
+  __syncwarp();
+  named_bar_sync(1 + wg, 128);
+  if (!pv_done) return true;
+  bool ok = true, waited = false;
+  for (int c = 0; c < chunks; ++c) {
+    float f[16];
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(&m.alpha[col_base + c * 16 + j]);
+      f[j] = v.x, f[j + 1] = v.y, f[j + 2] = v.z, f[j + 3] = v.w;
+      any = any || v.x != 1.f || v.y != 1.f || v.z != 1.f || v.w != 1.f;
+    }
+    if (!any) continue;  // uniform
+    if (!waited) {
+      ok = mbar_wait(pv_done, parity);
+      tc_fence_after();
+      waited = true;
+    }
+    float o[16];
+    tmem_ld16(to + c * 16, o);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = f[j] == 0.f ? 0.f : o[j] * f[j];
+    tmem_st16(to + c * 16, o);
+  }
+  if (waited) tmem_wait_st();
+  return ok;
+}
+
+// TMEM load without its wait; the wait takes the registers along so that
+// nothing reads them before it.
+__device__ __forceinline__ void q8_tmem_ld16(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void q8_tmem_wait16(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
+
+// x[j] = exponent of P' for 16 columns, from their scores (x: raw products).
+// Returns the largest.
+__device__ __forceinline__ float q8_exponents(const AttnQ8Meta& m, int col, float* x, uint64_t ck2, uint64_t ev2,
+                                              bool part, uint32_t vis) {
+  const ulonglong2* rc = reinterpret_cast<const ulonglong2*>(m.rowc + col);
+  const ulonglong2* rf = reinterpret_cast<const ulonglong2*>(m.bias_ref + col);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const ulonglong2 r = rc[j], f = rf[j];
+    f2_unpack(f2_add(f2_fma(f2_mul(f2_pack(x[4 * j], x[4 * j + 1]), r.x), ck2, ev2), f.x), x[4 * j], x[4 * j + 1]);
+    f2_unpack(f2_add(f2_fma(f2_mul(f2_pack(x[4 * j + 2], x[4 * j + 3]), r.y), ck2, ev2), f.y), x[4 * j + 2],
+              x[4 * j + 3]);
+  }
+  if (part) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = (vis >> j) & 1u ? x[j] : -INFINITY;
+  }
+  float t0 = fmaxf(x[0], x[1]), t1 = fmaxf(x[2], x[3]);
+#pragma unroll
+  for (int j = 4; j < 16; j += 4) {
+    t0 = fmaxf(t0, fmaxf(x[j], x[j + 1]));
+    t1 = fmaxf(t1, fmaxf(x[j + 2], x[j + 3]));
+  }
+  return fmaxf(t0, t1);
+}
+
 template <int HD, int CH>
 __global__ void __launch_bounds__(kQ8Threads, 1)
     attn_q8_tc_kernel(const __grid_constant__ AttnQ8Maps maps, const AttnQ8Args a, const int n_chunks,
@@ -465,6 +673,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
   constexpr int TILE = kQ8Keys * HD;              // bytes of a K or V block
   constexpr uint32_t SW = HD == 128 ? 2u : 4u;    // 128-byte or 64-byte swizzle: one atom row per cache row
   constexpr uint32_t SBO = 8 * HD;                // 8 rows of HD bytes
+  constexpr int KEEP = CH <= 3 ? CH : 1;          // chunks whose exponents fit the registers next to l
   extern __shared__ uint8_t q8_smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(q8_smem_raw) + 1023) & ~uintptr_t(1023));
   const int N = 16 * n_chunks;
@@ -503,6 +712,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       mbar_init(&m.p_free[i], 1);
       mbar_init(&m.vis_full[i], 1);
     }
+    mbar_init(&m.q_ready, 8);
     mbar_init(&m.o_full, 1);
     fence_mbar_init();
   }
@@ -550,74 +760,6 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       mark((int)max(lo, (int64_t)0), (int)min(hi, (int64_t)a.kv_end - 1));
     }
   }
-  // ---- queries: two e4m3 terms per element, K-major rows of HD bytes. A row
-  // is LPR lanes x 8 elements; a lane loads the rows of a batch before it
-  // converts the first.
-  {
-    constexpr int LPR = HD / 8, RPP = kQ8Threads / LPR, BATCH = 4;
-    const bf16* qb = static_cast<const bf16*>(a.q);
-    const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0;
-    const int l8 = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
-    for (int rb = 0; rb < N; rb += RPP * BATCH) {
-      uint32_t raw[BATCH][4];
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        const int r = rb + u * RPP + r0;
-        raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
-        if (r < nrows) {
-          const bf16* src = qb + (int64_t)(t0 + r / a.G) * a.ldq + (int64_t)(h * a.G + r % a.G) * HD + l8 * 8;
-          if (wide) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            raw[u][0] = v.x, raw[u][1] = v.y, raw[u][2] = v.z, raw[u][3] = v.w;
-          } else {
-            const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) raw[u][e] = s16[2 * e] | (static_cast<uint32_t>(s16[2 * e + 1]) << 16);
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        const int r = rb + u * RPP + r0;
-        float x[8], amax = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] = __uint_as_float(raw[u][e] << 16);
-          x[2 * e + 1] = __uint_as_float(raw[u][e] & 0xffff0000u);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {  // Inf and NaN become the row's amax: they compare above every finite value
-          const float v = fabsf(x[e]);
-          amax = v <= 3.402823466e38f ? fmaxf(amax, v) : INFINITY;
-        }
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const bool fine = amax <= 3.402823466e38f;
-        const int byte = q8_scale_byte(fine ? amax : 0.f);
-        const float inv = q8_inv_scale(byte);
-        uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
-          const uint32_t c = q8_pack2(y0, y1);
-          const float2 back = q8_unpack2(c);
-          hi[e >> 2] |= c << (8 * (e & 3));
-          lo[e >> 2] |= q8_pack2(y0 - back.x, y1 - back.y) << (8 * (e & 3));
-        }
-        if (r < N) {
-          const int sw = HD == 128 ? (r & 7) : ((r >> 1) & 3);  // swizzled place of the lane's 8 bytes
-          const int at = r * HD + (((l8 >> 1) ^ sw) << 4) + (l8 & 1) * 8;
-          *reinterpret_cast<uint2*>(q_hi + at) = make_uint2(hi[0], hi[1]);
-          *reinterpret_cast<uint2*>(q_lo + at) = make_uint2(lo[0], lo[1]);
-          if (l8 == 0) {
-            m.rowc[r] = fine ? q8_scale(byte) * (a.scale * 1.4426950408889634f) : __int_as_float(0x7fffffff);
-            m.bias_ref[r] = r < nrows ? kQ8Unset : -kQ8Unset;  // columns past the rows: P' = 0
-          }
-        }
-      }
-    }
-  }
-  fence_proxy_async_smem();
   __syncthreads();
   // ---- this CTA's slice of the marked units
   if (warp == 0) {
@@ -697,7 +839,9 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       const uint32_t kr = smem_u32(k_ring), vr = smem_u32(v_ring), qh = smem_u32(q_hi), ql = smem_u32(q_lo);
       int nS = 0, nP = 0, sS = 0, sP = 0;
       uint32_t phS = 0, phP = 0, idle = 0;
-      while (nP < nblocks) {
+      const bool ready = mbar_wait(&m.q_ready, 0);
+      if (!ready) give_up();
+      while (ready && nP < nblocks) {
         bool prog = false;
         if (nS < nblocks && mbar_test(&m.k_full[sS], phS) &&
             (nS < 2 || mbar_test(&m.s_free[nS & 1], ((nS >> 1) - 1) & 1))) {
@@ -791,10 +935,9 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       if (lane == 0) mbar_arrive(&m.v_clean[st]);
       if (++st == stages) st = 0, phase ^= 1u;
     }
-  } else if (my_chunks > 0) {
-    // ---- softmax warps: thread = key
+  } else {
+    // ---- softmax warps: the queries, then thread = key
     const int key = quarter * 32 + lane;
-    const int bar = 1 + wg;
     const uint8_t* ksc = a.ks + (int64_t)h * a.scale_head_stride;
     const uint8_t* vsc = a.vs + (int64_t)h * a.scale_head_stride;
     const uint32_t p_at = (key >> 3) * atoms * 256 + (key & 7) * 32;
@@ -807,10 +950,15 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       kbyte = in ? ksc[kb + key] : 0;
       vbyte = in ? vsc[kb + key] : 0;
     };
-    if (nblocks > 0) fetch();
+    if (nblocks > 0 && my_chunks > 0) fetch();
+    q8_queries<HD>(a, m, q_hi, q_lo, N, nrows, t0, h);
+    fence_proxy_async_smem();
+    named_bar_sync(3, 256);  // the references are read by other warps than wrote them
+    if (lane == 0) mbar_arrive(&m.q_ready);
     bool bad = false;
-    for (int b = 0; b < nblocks; ++b) {
-      const bool full_block = kb >= max_start && kb + kQ8Keys <= min_len;
+    for (int b = 0; b < (my_chunks > 0 ? nblocks : 0); ++b) {
+      const int buf = b & 1;
+      const bool part = kb < max_start || kb + kQ8Keys > min_len;
       const float ck = q8_scale(kbyte);
       const int vb = max(vbyte, kQ8MinScale);
       const float ev = static_cast<float>(vb - 127);
@@ -818,133 +966,84 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       const uint64_t ck2 = f2_pack(ck, ck), ev2 = f2_pack(ev, ev), iv2 = f2_pack(inv_v, inv_v);
       if (b + 1 < nblocks) fetch();
       // After a timeout the loop runs on without waiting: the warpgroup's barriers stay matched.
-      if (!bad && (*abort_flag || !mbar_wait(&m.s_full[b & 1], (b >> 1) & 1))) {
+      if (!bad && (*abort_flag || !mbar_wait(&m.s_full[buf], (b >> 1) & 1))) {
         bad = true;
         give_up();
       }
-      if (!bad && (*abort_flag || !mbar_wait(&m.vis_full[b & 1], (b >> 1) & 1))) {
+      // (every block: the barrier's parity tells one phase from the next, not from the one after)
+      if (!bad && !mbar_wait(&m.vis_full[buf], (b >> 1) & 1)) {
         bad = true;
         give_up();
       }
       tc_fence_after();
-      const uint32_t ts = tmem + (b & 1) * kQ8MaxRows + lane_base + col_base;
-      const uint32_t pb = p_s + (b & 1) * 2 * p_bytes + p_at;
+      const uint32_t ts = tmem + buf * kQ8MaxRows + lane_base + col_base;
+      const uint32_t pb = p_s + buf * 2 * p_bytes + p_at;
+      const uint64_t minus1 = f2_pack(-1.f, -1.f);
+      // Scores to exponents; with up to KEEP chunks they stay in registers
+      // for the weights below, with more they are computed again there.
+      float x[16 * KEEP];
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          if (c < my_chunks) {
+            float* xc = x + 16 * (CH <= KEEP ? c : 0);
+            const uint32_t vis = part ? q8_chunk_vis(m, buf, col_base + c * 16, a.G, ntok, quarter, lane) : 0xffffu;
+            q8_tmem_ld16(ts + c * 16, xc);
+            q8_tmem_wait16(xc);
+            top = fmaxf(top, q8_exponents(m, col_base + c * 16, xc, ck2, ev2, part, vis));
+          }
+        }
+        if (!named_bar_or(1 + wg, 128, top > kQ8Bias + kQ8Grow)) break;
+        if (!q8_move_references(m, ts, tmem + kQ8ColO + lane_base + col_base, col_base, my_chunks, wg, ck, ev, part, buf,
+                                a.G, ntok, b > 0 && !bad ? &m.p_free[buf ^ 1] : nullptr, ((b - 1) >> 1) & 1)) {
+          bad = true;
+          give_up();
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          if (c < my_chunks) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) l[c * 16 + j] *= m.alpha[col_base + c * 16 + j];
+          }
+        }
+      }
+      if (CH <= KEEP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.s_free[buf]);
+      }
+      if (b >= 2 && !bad && !mbar_wait(&m.p_free[buf], ((b >> 1) - 1) & 1)) {  // P V of block b - 2 read this buffer
+        bad = true;
+        give_up();
+      }
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
           const int col = col_base + c * 16;
-          uint32_t vis = 0xffffu;
-          if (!full_block) {
-            vis = 0u;
-            const int tl = min((col + 15) / a.G, ntok - 1);
-            for (int t = col / a.G; t <= tl; ++t)
-              if ((m.vis[b & 1][t][quarter] >> lane) & 1u) {
-                const int lo = max(t * a.G - col, 0), hi = min((t + 1) * a.G - col, 16);
-                vis |= ((1u << hi) - 1u) & ~((1u << lo) - 1u);
-              }
-          }
-          float x[16];
-          tmem_ld16(ts + c * 16, x);
-          uint64_t w[8];
-          const ulonglong2* rc = reinterpret_cast<const ulonglong2*>(m.rowc + col);
-          const ulonglong2* rf = reinterpret_cast<const ulonglong2*>(m.bias_ref + col);
-          float top = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const ulonglong2 r = rc[j], f = rf[j];
-            w[2 * j] = f2_add(f2_fma(f2_mul(f2_pack(x[4 * j], x[4 * j + 1]), r.x), ck2, ev2), f.x);
-            w[2 * j + 1] = f2_add(f2_fma(f2_mul(f2_pack(x[4 * j + 2], x[4 * j + 3]), r.y), ck2, ev2), f.y);
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f2_unpack(w[j], x[2 * j], x[2 * j + 1]);
-          if (!full_block) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = (vis >> j) & 1u ? x[j] : -INFINITY;
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
-          if (named_bar_or(bar, 128, top > kQ8Bias + kQ8Grow)) {
-            // Some row's reference moves: column maxima of t over the block's 128 keys (halving the columns
-            // a lane holds at every step), then O, l and x of the chunk to the new references.
-            float t[16], v[16];
-            tmem_ld16(ts + c * 16, t);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              t[j] = fmaf(t[j] * m.rowc[col + j], ck, ev);
-              if (!((vis >> j) & 1u)) t[j] = -INFINITY;
-              v[j] = t[j];
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) {
-#pragma unroll
-              for (int j = 0; j < o; ++j) {
-                const bool up = lane & o;
-                const float give = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
-                v[j] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
-              }
-            }
-            v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
-            if (lane < 16) m.wmax[warp][lane] = v[0];
-            __syncwarp();
-            named_bar_sync(bar, 128);
-            if (threadIdx.x % 128 < 16) {
-              const int j = threadIdx.x % 128;
-              const float mx = fmaxf(fmaxf(m.wmax[wg * 4][j], m.wmax[wg * 4 + 1][j]),
-                                     fmaxf(m.wmax[wg * 4 + 2][j], m.wmax[wg * 4 + 3][j]));
-              const float old = m.bias_ref[col + j];
-              const bool move = mx + old > kQ8Bias + kQ8Grow;
-              const float now = move ? kQ8Bias - mx : old;
-              m.alpha[wg][j] = !move ? 1.f : old == kQ8Unset ? 0.f : exp2f(now - old);
-              m.bias_ref[col + j] = now;
-            }
-            __syncwarp();
-            named_bar_sync(bar, 128);
-            float alpha[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              alpha[j] = m.alpha[wg][j];
-              x[j] = t[j] + m.bias_ref[col + j];
-              l[c * 16 + j] *= alpha[j];
-            }
-            if (b > 0) {
-              if (!bad && !mbar_wait(&m.p_free[(b - 1) & 1], ((b - 1) >> 1) & 1)) {
-                bad = true;
-                give_up();
-              }
-              tc_fence_after();
-              float o[16];
-              tmem_ld16(tmem + kQ8ColO + lane_base + col, o);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = alpha[j] == 0.f ? 0.f : o[j] * alpha[j];
-              tmem_st16(tmem + kQ8ColO + lane_base + col, o);
-              tmem_wait_st();
-            }
-          }
-          if (c == my_chunks - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&m.s_free[b & 1]);
-          }
-          if (c == 0 && b >= 2 && !bad && !mbar_wait(&m.p_free[b & 1], ((b >> 1) - 1) & 1)) {
-            bad = true;
-            give_up();
+          float* xc = x + 16 * (CH <= KEEP ? c : 0);
+          if (CH > KEEP) {
+            const uint32_t vis = part ? q8_chunk_vis(m, buf, col, a.G, ntok, quarter, lane) : 0xffffu;
+            q8_tmem_ld16(ts + c * 16, xc);
+            q8_tmem_wait16(xc);
+            (void)q8_exponents(m, col, xc, ck2, ev2, part, vis);
           }
           uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) x[j] = q8_ex2(x[j]);
-#pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            uint64_t acc = f2_pack(l[c * 16 + j], l[c * 16 + j + 1]);
-            acc = f2_fma(f2_pack(x[j], x[j + 1]), iv2, acc);
-            f2_unpack(acc, l[c * 16 + j], l[c * 16 + j + 1]);
-          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float t4[4], r4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              t4[e] = __uint_as_float(__float_as_uint(x[4 * j + e]) & 0xfff00000u);  // 4 significant bits
-              r4[e] = x[4 * j + e] - t4[e];
+              xc[4 * j + e] = q8_ex2(xc[4 * j + e]);
+              t4[e] = __uint_as_float(__float_as_uint(xc[4 * j + e]) & 0xfff00000u);  // 4 significant bits
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const uint64_t p2 = f2_pack(xc[4 * j + e], xc[4 * j + e + 1]);
+              f2_unpack(f2_fma(f2_pack(t4[e], t4[e + 1]), minus1, p2), r4[e], r4[e + 1]);
+              f2_unpack(f2_fma(p2, iv2, f2_pack(l[c * 16 + 4 * j + e], l[c * 16 + 4 * j + e + 1])),
+                        l[c * 16 + 4 * j + e], l[c * 16 + 4 * j + e + 1]);
             }
             hi[j] = q8_pack4(t4[0], t4[1], t4[2], t4[3]);
             lo[j] = q8_pack4(r4[0], r4[1], r4[2], r4[3]);
@@ -961,72 +1060,68 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&m.p_full[b & 1]);
+      if (lane == 0) {
+        if (CH > KEEP) mbar_arrive(&m.s_free[buf]);
+        mbar_arrive(&m.p_full[buf]);
+      }
     }
   }
   // ---- results: l summed over the 128 keys' threads, O^T read back (lane = head dim)
   __syncwarp();
   float* s_l = reinterpret_cast<float*>(p_buf);  // [4][N]: the P buffers are free once every MMA retired
-  bool done = true;
   if (warp < 8 && my_chunks > 0) {
-    done = mbar_wait(&m.o_full, 0);
-    if (!done && lane == 0) give_up();
+    if (!mbar_wait(&m.o_full, 0) && lane == 0) give_up();
     tc_fence_after();
-  }
-  __syncthreads();
-  if (warp < 8 && my_chunks > 0) {
+    named_bar_sync(3, two ? 256 : 128);  // (a timed-out warp may still have been writing P)
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if (c < my_chunks) {
-        // 16 columns over 32 lanes: halve the columns a lane holds at every step
-        float v[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = l[c * 16 + j];
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) {
-#pragma unroll
-          for (int j = 0; j < o; ++j) {
-            const bool up = lane & o;
-            const float give = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
-            v[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-          }
-        }
-        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
-        if (lane < 16) s_l[quarter * N + col_base + c * 16 + lane] = v[0];
+        const float sum = q8_columns_reduce<false>(l + c * 16, lane);
+        if (lane < 16) s_l[quarter * N + col_base + c * 16 + lane] = sum;
       }
     }
+    __syncwarp();
+    named_bar_sync(1 + wg, 128);
+    // thread i of the warpgroup: row col_base + i's sum, as the factor of its output or the record {M, l}
+    const int64_t rec0 = ((int64_t)blockIdx.x * a.n_splits + split) * kQ8MaxRows;
+    const int i = threadIdx.x & 127;
+    if (i < 16 * my_chunks) {
+      const int r = col_base + i;
+      const float sum = (s_l[r] + s_l[N + r]) + (s_l[2 * N + r] + s_l[3 * N + r]);
+      m.alpha[r] = sum == 0.f ? 0.f : 1.f / sum;
+      if (a.n_splits > 1 && r < nrows) {
+        float* ml = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD + (rec0 + r) * 2;
+        *reinterpret_cast<float2*>(ml) = make_float2(kQ8Bias - m.bias_ref[r], sum);
+      }
+    }
+    __syncwarp();
     named_bar_sync(1 + wg, 128);
     const int d = quarter * 32 + lane;
-    const int64_t rec0 = ((int64_t)blockIdx.x * a.n_splits + split) * kQ8MaxRows;
-    float* o_part = a.part;
-    float* ml_part = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      if (c < my_chunks) {
+    if (quarter * 32 < HD && nblocks > 0) {
+#pragma unroll 1
+      for (int c = 0; c < my_chunks; ++c) {
         const int col = col_base + c * 16;
         float o[16];
-        if (nblocks > 0) {
-          tmem_ld16(tmem + kQ8ColO + lane_base + col, o);
+        tmem_ld16(tmem + kQ8ColO + lane_base + col, o);
+        if (a.n_splits > 1) {
+          float* dst = a.part + (rec0 + col) * HD + d;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (col + j < nrows) dst[j * HD] = o[j];
         } else {
+          int tok = col / a.G, g = col - tok * a.G;
+          bf16* base = static_cast<bf16*>(a.out) + (int64_t)h * a.G * HD + d;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int r = col + j;
-          if (r < nrows && d < HD) {
-            const float sum = (s_l[r] + s_l[N + r]) + (s_l[2 * N + r] + s_l[3 * N + r]);
-            if (a.n_splits == 1) {
-              const float inv = sum == 0.f ? 0.f : 1.f / sum;
-              static_cast<bf16*>(a.out)[(int64_t)(t0 + r / a.G) * a.ldo + (int64_t)(h * a.G + r % a.G) * HD + d] =
-                  f2bf(sum == 0.f ? 0.f : o[j] * inv);
-            } else {
-              if (sum != 0.f) o_part[(rec0 + r) * HD + d] = o[j];
-              if (d == 0) *reinterpret_cast<float2*>(ml_part + (rec0 + r) * 2) = make_float2(kQ8Bias - m.bias_ref[r], sum);
-            }
+          for (int j = 0; j < 16; ++j) {
+            const float f = m.alpha[col + j];
+            if (col + j < nrows) base[(int64_t)(t0 + tok) * a.ldo + g * HD] = f2bf(f == 0.f ? 0.f : o[j] * f);
+            if (++g == a.G) g = 0, ++tok;
           }
         }
       }
+    } else if (quarter * 32 < HD && a.n_splits == 1) {
+      for (int r = col_base; r < min(col_base + 16 * my_chunks, nrows); ++r)
+        static_cast<bf16*>(a.out)[(int64_t)(t0 + r / a.G) * a.ldo + (int64_t)(h * a.G + r % a.G) * HD + d] = f2bf(0.f);
     }
   }
   tc_fence_before();
@@ -1107,7 +1202,7 @@ static int q8_tensor_map(const void* base, const SsdKvQ8& c, CUtensorMap* out) {
 template <int HD>
 static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64_t workspace_bytes,
                      cudaStream_t stream) {
-  // Query rows in as few groups of whole tokens as fit 160 columns, evenly.
+  // Query rows in as few groups of whole tokens as fit the columns, evenly.
   int tpg = kQ8MaxRows / a.G;
   a.tiles = (a.T + tpg - 1) / tpg;
   tpg = (a.T + a.tiles - 1) / a.tiles;
