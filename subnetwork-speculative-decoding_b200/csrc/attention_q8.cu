@@ -323,25 +323,30 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 // with M a per-row reference (power-of-two scale of O and l). M is the true
 // maximum of t over the row's first visible block and moves only when some t
 // exceeds it by kGrow (then O and l are rescaled), so the usual block needs no
-// reduction over keys, only one vote. P' <= 2^(kBias + kGrow) = 256 < 448; its
-// second term rounds at 2^-10, i.e. 2^-15 of the weight at the reference, and
+// reduction over keys, only one vote. P' <= 2^(kBias + kGrow) < 448; its
+// second term rounds at 2^-10, i.e. 2^-13 of the weight at the reference, and
 // l sums the unrounded P' in fp32 per thread until the end.
 //
 // A CTA = one KV head x up to 144 query rows (whole tokens) x one slice of the
 // key blocks that some row sees (a bitmap in shared memory: slot ranges of
-// other sequences in between are not read). Warps 0-3 take the first half of
-// the columns, 4-7 the second; warps 8 / 9 stream K / V blocks by TMA; lane 0
-// of warp 10 issues the MMAs, S^T(b + 1) and O(b) as each is ready; warp 11
-// zeroes V rows that no query row sees (0 * NaN) before they are used.
+// other sequences in between are not read). Warps 0-7 prepare the queries and
+// then run the softmax; 8 / 9 stream K / V blocks by TMA; 10 issues the MMAs,
+// S^T(b + 1) and O(b) as each is ready; 11 works out the visibility of blocks
+// that not every row sees whole and zeroes V rows that none does (0 * NaN).
+// The softmax's two warpgroups either take the key blocks in turn, with a
+// reference, l and O of their own (ALT: up to 80 columns, what their
+// registers hold of l), or half of the columns each.
 constexpr int kQ8Keys = 128;
 constexpr int kQ8MaxRows = 144;       // query rows per CTA: three ring stages fit next to their Q and P'
+constexpr int kQ8AltRows = 80;        // up to here the warpgroups take blocks in turn
+constexpr int kQ8RowState = 160;      // rows of per-row state: 144, or 2 x 80
 constexpr int kQ8Threads = 384;
 constexpr int kQ8MaxStages = 6;
 constexpr int kQ8MapWords = 256;      // bitmap of key blocks (units of 2^unit_shift blocks)
-constexpr float kQ8Bias = 5.f;
-constexpr float kQ8Grow = 3.f;
+constexpr float kQ8Bias = 3.f;
+constexpr float kQ8Grow = 5.75f;
 constexpr float kQ8Unset = 1e30f;     // reference of a row that saw no key yet: every t exceeds it
-constexpr uint32_t kQ8ColO = 2 * kQ8MaxRows;  // TMEM columns: two S^T buffers, then O^T
+constexpr uint32_t kQ8ColO = 2 * kQ8MaxRows;  // TMEM columns: two S^T buffers, then O^T (ALT: two of kQ8AltRows)
 
 struct AttnQ8Maps {
   CUtensorMap k, v;  // [n_kv][max_slots][hd] bytes, box {hd, 128, 1}
@@ -349,9 +354,9 @@ struct AttnQ8Maps {
 
 struct AttnQ8Meta {
   float rowc[kQ8MaxRows];                      // 2^eq scale log2 e per query row
-  float bias_ref[kQ8MaxRows];                  // kBias - M
-  float wmax[4][kQ8MaxRows];                   // growth path: column maxima of a warp's 32 keys
-  float alpha[kQ8MaxRows];                     // growth path: factors of O and l
+  float bias_ref[kQ8RowState];                 // kBias - M (ALT: per warpgroup, 16 CH rows apart)
+  float alpha[kQ8RowState];                    // reference moves: factors of O and l
+  float wmax[4][kQ8RowState];                  // reference moves: column maxima of a warp's 32 keys
   int len[kQ8MaxRows], start[kQ8MaxRows];      // per token
   uint32_t vis[2][kQ8MaxRows][4];              // per block buffer and token: which of the block's keys it sees
   uint32_t map[kQ8MapWords];
@@ -361,7 +366,7 @@ struct AttnQ8Meta {
   uint32_t tmem;
   uint64_t k_full[kQ8MaxStages], k_empty[kQ8MaxStages], v_full[kQ8MaxStages], v_clean[kQ8MaxStages],
       v_empty[kQ8MaxStages];
-  uint64_t s_full[2], s_free[2], p_full[2], p_free[2], vis_full[2], q_ready, o_full;
+  uint64_t s_full[2], s_free[2], p_full[2], p_free[2], vis_full[2], meta_ready, q_ready, o_full;
 };
 
 __host__ __device__ constexpr int q8_p_bytes(int n) { return (n + 31) / 32 * 4096; }  // one term of one buffer
@@ -379,19 +384,33 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Shared-memory matrix descriptor; swizzle: 2 = 128 B, 4 = 64 B, 6 = 32 B.
-__device__ __forceinline__ uint64_t sdesc_q8(uint32_t saddr, uint32_t lbo, uint32_t sbo, uint32_t swizzle) {
-  uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
-  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(swizzle) << 61;
+// Shared-memory matrix descriptor in two words: address and leading offset in
+// the low one (an operand's later parts add (bytes >> 4) there), stride offset,
+// version and swizzle (2 = 128 B, 4 = 64 B, 6 = 32 B) in the high one.
+__device__ __forceinline__ uint32_t q8_desc_lo(uint32_t saddr, uint32_t lbo) {
+  return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);
+}
+__device__ __forceinline__ uint32_t q8_desc_hi(uint32_t sbo, uint32_t swizzle) {
+  return (sbo >> 4) | (1u << 14) | (swizzle << 29);
+}
+__device__ __forceinline__ uint64_t q8_desc(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
   return d;
 }
 // e4m3 A/B, fp32 D, M x N; mn: both operands MN-major.
 __host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool mn) {
   return (1u << 4) | (mn ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(r));
+  return r != 0;
 }
 __device__ __forceinline__ float q8_ex2(float x) {
   float y;
@@ -442,9 +461,10 @@ struct Q8Blocks {
   const uint32_t* map;
   uint32_t bits;
   int word, shift, sub, unit;
-  __device__ Q8Blocks(const AttnQ8Meta& m, int unit_shift) : map(m.map), shift(unit_shift), sub(0), unit(0) {
-    word = m.first >> 5;
-    bits = m.count ? m.map[word] & (~0u << (m.first & 31)) : 0u;
+  __device__ Q8Blocks(const uint32_t* m, int first, int count, int unit_shift)
+      : map(m), shift(unit_shift), sub(0), unit(0) {
+    word = first >> 5;
+    bits = count ? map[word] & (~0u << (first & 31)) : 0u;
   }
   __device__ __forceinline__ int next() {  // first slot of the next block
     if (sub == 0) {
@@ -458,71 +478,140 @@ struct Q8Blocks {
   }
 };
 
+// The CTA's tokens (by warps 8 .. 11): slot ranges, and the bitmap of key
+// blocks that some row sees.
+__device__ __forceinline__ void q8_tokens(const AttnQ8Args& a, AttnQ8Meta& m, int t0, int ntok, int sb,
+                                          int unit_shift) {
+  auto mark = [&](int lo, int hi) {  // slots lo .. hi
+    const int u0 = (lo / kQ8Keys) >> unit_shift, u1 = (hi / kQ8Keys) >> unit_shift;
+    for (int w = u0 >> 5; w <= u1 >> 5; ++w) {
+      uint32_t bits = ~0u;
+      if (w == u0 >> 5) bits &= ~0u << (u0 & 31);
+      if (w == u1 >> 5) bits &= ~0u >> (31 - (u1 & 31));
+      if ((m.map[w] & bits) != bits) atomicOr(&m.map[w], bits);
+    }
+  };
+  for (int i = threadIdx.x - 256; i < ntok; i += 128) {
+    const int t = t0 + i;
+    const int start = max(a.prefix_start ? a.prefix_start[t] : 0, 0);
+    const int len = min(a.prefix_len[t], a.kv_end);
+    m.start[i] = start;
+    m.len[i] = len;
+    atomicMax(&m.max_start, start);
+    atomicMin(&m.min_len, len);
+    if (len > start) mark(start, len - 1);
+    for (int w = 0; w < a.mask_words; ++w) {
+      const uint64_t bits = a.mask[(int64_t)t * a.mask_words + w];
+      if (!bits) continue;
+      const int64_t lo = (int64_t)sb + w * 64 + __ffsll(bits) - 1, hi = (int64_t)sb + w * 64 + 63 - __clzll(bits);
+      if (hi < 0 || lo >= a.kv_end) continue;
+      mark((int)max(lo, (int64_t)0), (int)min(hi, (int64_t)a.kv_end - 1));
+    }
+  }
+}
+// Slice `split` of the marked units, in equal shares: its first unit and how
+// many (computed alike by each warp that asks).
+__device__ __forceinline__ void q8_slice(const AttnQ8Meta& m, int split, int n_splits, int& first, int& count) {
+  constexpr int PER = kQ8MapWords / 32;
+  const int lane = threadIdx.x & 31;
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mine += __popc(m.map[lane * PER + i]);
+  int before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += up;
+  }
+  const int total = __shfl_sync(0xffffffffu, before, 31);
+  before -= mine;
+  const int u0 = (int)((int64_t)total * split / n_splits);
+  count = (int)((int64_t)total * (split + 1) / n_splits) - u0;
+  const bool here = count > 0 && u0 >= before && u0 < before + mine;
+  int at = 0;
+  if (here) {
+    int skip = u0 - before;
+    for (int i = 0; i < PER; ++i) {
+      uint32_t bits = m.map[lane * PER + i];
+      const int n = __popc(bits);
+      if (skip >= n) {
+        skip -= n;
+        continue;
+      }
+      for (; skip > 0; --skip) bits &= bits - 1;
+      at = (lane * PER + i) * 32 + __ffs(bits) - 1;
+      break;
+    }
+  }
+  const uint32_t who = __ballot_sync(0xffffffffu, here);
+  first = who ? __shfl_sync(0xffffffffu, at, __ffs(who) - 1) : 0;
+}
+
 // The CTA's query rows as two e4m3 terms per element, K-major rows of HD bytes
 // (by the eight softmax warps). A row is LPR lanes x 8 elements; a lane loads
-// the rows of a batch before it converts the first.
-template <int HD>
+// all its rows before it converts the first.
+template <int HD, int ROWS>
 __device__ __forceinline__ void q8_queries(const AttnQ8Args& a, AttnQ8Meta& m, uint8_t* q_hi, uint8_t* q_lo, int N,
-                                           int nrows, int t0, int h) {
-  constexpr int LPR = HD / 8, RPP = 256 / LPR, BATCH = 4;
+                                           int nrows, int t0, int h, int second_ref) {
+  constexpr int LPR = HD / 8, RPP = 256 / LPR, BATCH = (ROWS + RPP - 1) / RPP;
   const bf16* qb = static_cast<const bf16*>(a.q);
   const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0;
   const int l8 = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
-  for (int rb = 0; rb < N; rb += RPP * BATCH) {
-    uint32_t raw[BATCH][4];
+  uint32_t raw[BATCH][4];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int r = rb + u * RPP + r0;
-      raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
-      if (r < nrows) {
-        const bf16* src = qb + (int64_t)(t0 + r / a.G) * a.ldq + (int64_t)(h * a.G + r % a.G) * HD + l8 * 8;
-        if (wide) {
-          const uint4 v = *reinterpret_cast<const uint4*>(src);
-          raw[u][0] = v.x, raw[u][1] = v.y, raw[u][2] = v.z, raw[u][3] = v.w;
-        } else {
-          const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
+  for (int u = 0; u < BATCH; ++u) {
+    const int r = u * RPP + r0;
+    raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
+    if (r < nrows) {
+      const bf16* src = qb + (int64_t)(t0 + r / a.G) * a.ldq + (int64_t)(h * a.G + r % a.G) * HD + l8 * 8;
+      if (wide) {
+        const uint4 v = *reinterpret_cast<const uint4*>(src);
+        raw[u][0] = v.x, raw[u][1] = v.y, raw[u][2] = v.z, raw[u][3] = v.w;
+      } else {
+        const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) raw[u][e] = s16[2 * e] | (static_cast<uint32_t>(s16[2 * e + 1]) << 16);
-        }
+        for (int e = 0; e < 4; ++e) raw[u][e] = s16[2 * e] | (static_cast<uint32_t>(s16[2 * e + 1]) << 16);
       }
     }
+  }
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int r = rb + u * RPP + r0;
-      float x[8], amax = 0.f;
+  for (int u = 0; u < BATCH; ++u) {
+    const int r = u * RPP + r0;
+    if (u * RPP >= N) break;  // uniform
+    float x[8], amax = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = __uint_as_float(raw[u][e] << 16);
-        x[2 * e + 1] = __uint_as_float(raw[u][e] & 0xffff0000u);
-      }
+    for (int e = 0; e < 4; ++e) {
+      x[2 * e] = __uint_as_float(raw[u][e] << 16);
+      x[2 * e + 1] = __uint_as_float(raw[u][e] & 0xffff0000u);
+    }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {  // Inf and NaN become the row's amax: they compare above every finite value
-        const float v = fabsf(x[e]);
-        amax = v <= 3.402823466e38f ? fmaxf(amax, v) : INFINITY;
-      }
+    for (int e = 0; e < 8; ++e) {  // Inf and NaN become the row's amax: they compare above every finite value
+      const float v = fabsf(x[e]);
+      amax = v <= 3.402823466e38f ? fmaxf(amax, v) : INFINITY;
+    }
 #pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      const bool fine = amax <= 3.402823466e38f;
-      const int byte = q8_scale_byte(fine ? amax : 0.f);
-      const float inv = q8_inv_scale(byte);
-      uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+    for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const bool fine = amax <= 3.402823466e38f;
+    const int byte = q8_scale_byte(fine ? amax : 0.f);
+    const float inv = q8_inv_scale(byte);
+    uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
-        const uint32_t c = q8_pack2(y0, y1);
-        const float2 back = q8_unpack2(c);
-        hi[e >> 2] |= c << (8 * (e & 3));
-        lo[e >> 2] |= q8_pack2(y0 - back.x, y1 - back.y) << (8 * (e & 3));
-      }
-      if (r < N) {
-        const int sw = HD == 128 ? (r & 7) : ((r >> 1) & 3);  // swizzled place of the lane's 8 bytes
-        const int at = r * HD + (((l8 >> 1) ^ sw) << 4) + (l8 & 1) * 8;
-        *reinterpret_cast<uint2*>(q_hi + at) = make_uint2(hi[0], hi[1]);
-        *reinterpret_cast<uint2*>(q_lo + at) = make_uint2(lo[0], lo[1]);
-        if (l8 == 0) {
-          m.rowc[r] = fine ? q8_scale(byte) * (a.scale * 1.4426950408889634f) : __int_as_float(0x7fffffff);
-          m.bias_ref[r] = r < nrows ? kQ8Unset : -kQ8Unset;  // columns past the rows: P' = 0
-        }
+    for (int e = 0; e < 8; e += 2) {
+      const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
+      const uint32_t c = q8_pack2(y0, y1);
+      const float2 back = q8_unpack2(c);
+      hi[e >> 2] |= c << (8 * (e & 3));
+      lo[e >> 2] |= q8_pack2(y0 - back.x, y1 - back.y) << (8 * (e & 3));
+    }
+    if (r < N) {
+      const int sw = HD == 128 ? (r & 7) : ((r >> 1) & 3);  // swizzled place of the lane's 8 bytes
+      const int at = r * HD + (((l8 >> 1) ^ sw) << 4) + (l8 & 1) * 8;
+      *reinterpret_cast<uint2*>(q_hi + at) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(q_lo + at) = make_uint2(lo[0], lo[1]);
+      if (l8 == 0) {
+        m.rowc[r] = fine ? q8_scale(byte) * (a.scale * 1.4426950408889634f) : __int_as_float(0x7fffffff);
+        m.bias_ref[r] = r < nrows ? kQ8Unset : -kQ8Unset;  // columns past the rows: P' = 0
+        if (second_ref) m.bias_ref[second_ref + r] = r < nrows ? kQ8Unset : -kQ8Unset;
       }
     }
   }
@@ -542,8 +631,8 @@ __device__ __forceinline__ uint32_t q8_chunk_vis(const AttnQ8Meta& m, int buf, i
   return vis;
 }
 
-// One halving step of a reduction of 16 columns over 32 lanes: afterwards
-// lane i < 16 (and i + 16) holds column i's maximum (or sum) in v[0].
+// Maximum (or sum) of 16 columns over 32 lanes, halving the columns a lane
+// holds at every step: lane i (and i + 16) returns column i & 15's.
 template <bool MAX>
 __device__ __forceinline__ float q8_columns_reduce(float* v, int lane) {
 #pragma unroll
@@ -562,30 +651,31 @@ __device__ __forceinline__ float q8_columns_reduce(float* v, int lane) {
 
 // Some of the warpgroup's references move: column maxima of t over the
 // block's 128 keys, new references and factors into shared memory, O's columns
-// rescaled. `pv_done` has completed `parity` once the previous block's P V has
-// retired (NULL: first block). Returns false on a timeout. All 128 threads of
-// the warpgroup call it; out of line, as most blocks do not need it.
-__device__ __noinline__ bool q8_move_references(AttnQ8Meta& m, uint32_t ts, uint32_t to, int col_base, int chunks,
+// rescaled. The warpgroup's columns start at `col` of the query rows and at
+// `ref` of the per-row state, `ts` / `to` of S^T and O^T in TMEM. `pv_done`
+// completes `parity` when the last P V into this O has retired (NULL: there is
+// none yet). Returns false on a timeout. All 128 threads call it; out of line,
+// as most blocks do not need it.
+__device__ __noinline__ bool q8_move_references(AttnQ8Meta& m, uint32_t ts, uint32_t to, int col, int ref, int chunks,
                                                 int wg, float ck, float ev, bool part, int buf, int G, int ntok,
                                                 uint64_t* pv_done, uint32_t parity) {
   const int tid = threadIdx.x & 127, quarter = tid >> 5, lane = tid & 31;
   for (int c = 0; c < chunks; ++c) {
-    const int col = col_base + c * 16;
-    const uint32_t vis = part ? q8_chunk_vis(m, buf, col, G, ntok, quarter, lane) : 0xffffu;
+    const uint32_t vis = part ? q8_chunk_vis(m, buf, col + c * 16, G, ntok, quarter, lane) : 0xffffu;
     float t[16];
     tmem_ld16(ts + c * 16, t);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      t[j] = fmaf(t[j] * m.rowc[col + j], ck, ev);
+      t[j] = fmaf(t[j] * m.rowc[col + c * 16 + j], ck, ev);
       if (!((vis >> j) & 1u)) t[j] = -INFINITY;
     }
     const float top = q8_columns_reduce<true>(t, lane);
-    if (lane < 16) m.wmax[quarter][col + lane] = top;
+    if (lane < 16) m.wmax[quarter][ref + c * 16 + lane] = top;
   }
   __syncwarp();
   named_bar_sync(1 + wg, 128);
   if (tid < 16 * chunks) {
-    const int r = col_base + tid;
+    const int r = ref + tid;
     const float mx = fmaxf(fmaxf(m.wmax[0][r], m.wmax[1][r]), fmaxf(m.wmax[2][r], m.wmax[3][r]));
     const float old = m.bias_ref[r];
     const bool move = mx + old > kQ8Bias + kQ8Grow;
@@ -602,7 +692,7 @@ __device__ __noinline__ bool q8_move_references(AttnQ8Meta& m, uint32_t ts, uint
     bool any = false;
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(&m.alpha[col_base + c * 16 + j]);
+      const float4 v = *reinterpret_cast<const float4*>(&m.alpha[ref + c * 16 + j]);
       f[j] = v.x, f[j + 1] = v.y, f[j + 2] = v.z, f[j + 3] = v.w;
       any = any || v.x != 1.f || v.y != 1.f || v.z != 1.f || v.w != 1.f;
     }
@@ -642,10 +732,10 @@ __device__ __forceinline__ void q8_tmem_wait16(float* v) {
 
 // x[j] = exponent of P' for 16 columns, from their scores (x: raw products).
 // Returns the largest.
-__device__ __forceinline__ float q8_exponents(const AttnQ8Meta& m, int col, float* x, uint64_t ck2, uint64_t ev2,
-                                              bool part, uint32_t vis) {
-  const ulonglong2* rc = reinterpret_cast<const ulonglong2*>(m.rowc + col);
-  const ulonglong2* rf = reinterpret_cast<const ulonglong2*>(m.bias_ref + col);
+__device__ __forceinline__ float q8_exponents(const float* rowc, const float* bias_ref, float* x, uint64_t ck2,
+                                              uint64_t ev2, bool part, uint32_t vis) {
+  const ulonglong2* rc = reinterpret_cast<const ulonglong2*>(rowc);
+  const ulonglong2* rf = reinterpret_cast<const ulonglong2*>(bias_ref);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const ulonglong2 r = rc[j], f = rf[j];
@@ -666,7 +756,7 @@ __device__ __forceinline__ float q8_exponents(const AttnQ8Meta& m, int col, floa
   return fmaxf(t0, t1);
 }
 
-template <int HD, int CH>
+template <int HD, int CH, bool ALT>
 __global__ void __launch_bounds__(kQ8Threads, 1)
     attn_q8_tc_kernel(const __grid_constant__ AttnQ8Maps maps, const AttnQ8Args a, const int n_chunks,
                       const int tok_per_group, const int stages, const int unit_shift) {
@@ -692,7 +782,8 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
   const int t0 = group * tok_per_group;
   const int ntok = min(tok_per_group, a.T - t0);
   const int nrows = ntok * a.G;
-  const bool two = n_chunks > CH;                 // the second warpgroup has columns
+  const bool two = ALT || n_chunks > CH;          // both warpgroups have columns
+  const uint32_t per_buffer = !ALT && two ? 8 : 4;  // softmax warps that work on one block
 
   if (threadIdx.x == 0) {
     m.max_start = 0;
@@ -707,11 +798,12 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&m.s_full[i], 1);
-      mbar_init(&m.s_free[i], two ? 8 : 4);
-      mbar_init(&m.p_full[i], two ? 8 : 4);
+      mbar_init(&m.s_free[i], per_buffer);
+      mbar_init(&m.p_full[i], per_buffer);
       mbar_init(&m.p_free[i], 1);
       mbar_init(&m.vis_full[i], 1);
     }
+    mbar_init(&m.meta_ready, 1);
     mbar_init(&m.q_ready, 8);
     mbar_init(&m.o_full, 1);
     fence_mbar_init();
@@ -731,232 +823,207 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
   const uint32_t tmem = m.tmem;
   pdl_wait();
   pdl_trigger();
-
-  // ---- tokens: slot ranges and masks, the bitmap of blocks that some row sees
-  const int sb = a.mask ? a.spec_base[0] : 0;
-  for (int i = threadIdx.x; i < ntok; i += kQ8Threads) {
-    const int t = t0 + i;
-    const int start = max(a.prefix_start ? a.prefix_start[t] : 0, 0);
-    const int len = min(a.prefix_len[t], a.kv_end);
-    m.start[i] = start;
-    m.len[i] = len;
-    atomicMax(&m.max_start, start);
-    atomicMin(&m.min_len, len);
-    auto mark = [&](int lo, int hi) {  // slots lo .. hi
-      const int u0 = (lo / kQ8Keys) >> unit_shift, u1 = (hi / kQ8Keys) >> unit_shift;
-      for (int w = u0 >> 5; w <= u1 >> 5; ++w) {
-        uint32_t bits = ~0u;
-        if (w == u0 >> 5) bits &= ~0u << (u0 & 31);
-        if (w == u1 >> 5) bits &= ~0u >> (31 - (u1 & 31));
-        if ((m.map[w] & bits) != bits) atomicOr(&m.map[w], bits);
-      }
-    };
-    if (len > start) mark(start, len - 1);
-    for (int w = 0; w < a.mask_words; ++w) {
-      const uint64_t bits = a.mask[(int64_t)t * a.mask_words + w];
-      if (!bits) continue;
-      const int64_t lo = (int64_t)sb + w * 64 + __ffsll(bits) - 1, hi = (int64_t)sb + w * 64 + 63 - __clzll(bits);
-      if (hi < 0 || lo >= a.kv_end) continue;
-      mark((int)max(lo, (int64_t)0), (int)min(hi, (int64_t)a.kv_end - 1));
-    }
-  }
-  __syncthreads();
-  // ---- this CTA's slice of the marked units
-  if (warp == 0) {
-    constexpr int PER = kQ8MapWords / 32;
-    int mine = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) mine += __popc(m.map[lane * PER + i]);
-    int before = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += up;
-    }
-    const int total = __shfl_sync(0xffffffffu, before, 31);
-    before -= mine;
-    const int u0 = (int)((int64_t)total * split / a.n_splits), u1 = (int)((int64_t)total * (split + 1) / a.n_splits);
-    if (lane == 0) m.count = u1 - u0;
-    if (u1 > u0 && u0 >= before && u0 < before + mine) {
-      int skip = u0 - before;
-      for (int i = 0; i < PER; ++i) {
-        uint32_t bits = m.map[lane * PER + i];
-        const int n = __popc(bits);
-        if (skip >= n) {
-          skip -= n;
-          continue;
-        }
-        for (; skip > 0; --skip) bits &= bits - 1;
-        m.first = (lane * PER + i) * 32 + __ffs(bits) - 1;
-        break;
-      }
-    }
-  }
-  __syncthreads();
-  const int nblocks = m.count << unit_shift;
-  const int max_start = m.max_start, min_len = m.min_len;
   const uint32_t p_s = smem_u32(p_buf);
   auto give_up = [&] {
     report_error(a.status, kErrWaitTimeout);
     *abort_flag = 1;
   };
 
-  float l[16 * CH];
+  if (warp >= 8) {
+    const int sb = a.mask ? a.spec_base[0] : 0;
+    q8_tokens(a, m, t0, ntok, sb, unit_shift);
+    __syncwarp();
+    named_bar_sync(4, 128);
+    int first, count;
+    q8_slice(m, split, a.n_splits, first, count);
+    const int nblocks = count << unit_shift;
+    const int max_start = m.max_start, min_len = m.min_len;
+    if (warp == 11 && lane == 0) {
+      m.first = first;
+      m.count = count;
+      mbar_arrive(&m.meta_ready);
+    }
+    Q8Blocks it(m.map, first, count, unit_shift);
+    if (warp == 8 || warp == 9) {
+      if (lane == 0) {
+        const bool is_v = warp == 9;
+        uint64_t* full = is_v ? m.v_full : m.k_full;
+        uint64_t* empty = is_v ? m.v_empty : m.k_empty;
+        uint8_t* ring = is_v ? v_ring : k_ring;
+        const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+        const uint64_t pol = l2_policy_evict_first();
+        int st = 0, issued = 0;
+        uint32_t phase = 0;
+        for (int b = 0; b < nblocks; ++b) {
+          if ((b >= stages && !mbar_wait(&empty[st], phase ^ 1u)) || *abort_flag) {
+            give_up();
+            break;
+          }
+          mbar_arrive_expect_tx(&full[st], TILE);
+          tma_load_3d(ring + st * TILE, map, &full[st], 0, it.next(), h, pol);
+          ++issued;
+          if (++st == stages) st = 0, phase ^= 1u;
+        }
+        if (*abort_flag)  // copies in flight land before the CTA leaves
+          for (int b = max(issued - stages, 0); b < issued; ++b) (void)mbar_wait(&full[b % stages], (b / stages) & 1);
+      }
+    } else if (warp == 10) {
+      // The whole warp runs the loop (its addresses stay uniform), one lane
+      // issues. Descriptors of later parts of an operand add to the low word.
+      const bool leader = elect_one();
+      if (nblocks > 0) {
+        const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true);
+        const uint32_t rows_hi = q8_desc_hi(SBO, SW), p_hi = q8_desc_hi(atoms * 256, 6u);
+        const uint32_t k_lo = q8_desc_lo(smem_u32(k_ring), 16), v_lo = q8_desc_lo(smem_u32(v_ring), 0);
+        const uint32_t qh_lo = q8_desc_lo(smem_u32(q_hi), 16), ql_lo = q8_desc_lo(smem_u32(q_lo), 16);
+        const uint32_t p_lo = q8_desc_lo(p_s, 256);
+        int nS = 0, nP = 0, sS = 0, sP = 0;
+        uint32_t phS = 0, phP = 0, idle = 0;
+        const bool ready = __all_sync(0xffffffffu, mbar_wait(&m.q_ready, 0));
+        if (!ready && lane == 0) give_up();
+        while (ready && nP < nblocks) {
+          bool prog = false;
+          bool go = nS < nblocks && mbar_test(&m.k_full[sS], phS) &&
+                    (nS < 2 || mbar_test(&m.s_free[nS & 1], ((nS >> 1) - 1) & 1));
+          if (__all_sync(0xffffffffu, go)) {
+            tc_fence_after();
+            if (leader) {
+              const uint32_t d = tmem + (nS & 1) * kQ8MaxRows, k = k_lo + sS * (TILE >> 4);
 #pragma unroll
-  for (int i = 0; i < 16 * CH; ++i) l[i] = 0.f;
-  const int wg = warp >> 2, quarter = warp & 3;   // (softmax warps 0 .. 7)
-  const int my_chunks = wg == 0 ? CH : n_chunks - CH;
-  const int col_base = wg == 0 ? 0 : 16 * CH;
-  const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-
-  if (warp == 8 || warp == 9) {
-    if (lane == 0) {
-      const bool is_v = warp == 9;
-      uint64_t* full = is_v ? m.v_full : m.k_full;
-      uint64_t* empty = is_v ? m.v_empty : m.k_empty;
-      uint8_t* ring = is_v ? v_ring : k_ring;
-      const CUtensorMap* map = is_v ? &maps.v : &maps.k;
-      const uint64_t pol = l2_policy_evict_first();
-      Q8Blocks it(m, unit_shift);
-      int st = 0, issued = 0;
+              for (int ks = 0; ks < HD / 32; ++ks)
+                umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(qh_lo + ks * 2, rows_hi), id_s, ks > 0);
+#pragma unroll
+              for (int ks = 0; ks < HD / 32; ++ks)
+                umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(ql_lo + ks * 2, rows_hi), id_s, 1u);
+              umma_commit(&m.s_full[nS & 1]);
+              umma_commit(&m.k_empty[sS]);
+            }
+            __syncwarp();
+            ++nS;
+            if (++sS == stages) sS = 0, phS ^= 1u;
+            prog = true;
+          }
+          go = nP < nS && mbar_test(&m.p_full[nP & 1], (nP >> 1) & 1) && mbar_test(&m.v_clean[sP], phP);
+          if (__all_sync(0xffffffffu, go)) {
+            tc_fence_after();
+            if (leader) {
+              // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
+              // M = 128 repeats the first (lanes 64 .. 127 are not read). P': MN-major, atoms of 32 rows x 8 keys.
+              const uint32_t d = tmem + kQ8ColO + (ALT ? (nP & 1) * kQ8AltRows : 0);
+              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + (nP & 1) * (2 * p_bytes >> 4);
+#pragma unroll
+              for (int term = 0; term < 2; ++term)
+#pragma unroll
+                for (int kk = 0; kk < kQ8Keys / 32; ++kk)
+                  umma_f8(d, q8_desc(v + kk * 2 * HD, rows_hi),
+                          q8_desc(pl + term * (p_bytes >> 4) + kk * (atoms * 64), p_hi), id_o,
+                          (nP >= (ALT ? 2 : 1) || term > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&m.p_free[nP & 1]);
+              umma_commit(&m.v_empty[sP]);
+            }
+            __syncwarp();
+            ++nP;
+            if (++sP == stages) sP = 0, phP ^= 1u;
+            prog = true;
+          }
+          idle = prog ? 0u : idle + 1u;
+          if (__any_sync(0xffffffffu, idle > kWaitLimit || *abort_flag)) {
+            if (lane == 0) give_up();
+            break;
+          }
+        }
+      }
+      if (leader) umma_commit(&m.o_full);
+    } else {
+      // Blocks that not every row sees whole: the keys that each token sees,
+      // for the softmax warps, and zeros in the V rows that none does.
+      int st = 0;
       uint32_t phase = 0;
       for (int b = 0; b < nblocks; ++b) {
-        if ((b >= stages && !mbar_wait(&empty[st], phase ^ 1u)) || *abort_flag) {
-          give_up();
+        const int kb = it.next();
+        const bool part = kb < max_start || kb + kQ8Keys > min_len;
+        bool bad = b >= 2 && !mbar_wait(&m.s_free[b & 1], ((b >> 1) - 1) & 1);  // vis[b & 1] was read for b - 2
+        uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
+        if (part) {
+          seen[0] = seen[1] = seen[2] = seen[3] = 0u;
+          for (int i = lane; i < ntok; i += 32) {
+            const uint64_t* mask = a.mask + (int64_t)(t0 + i) * a.mask_words;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint64_t v = q8_seen_bits(kb + 64 * half, m.start[i], m.len[i], mask, a.mask_words, sb, a.kv_end);
+              m.vis[b & 1][i][2 * half] = static_cast<uint32_t>(v);
+              m.vis[b & 1][i][2 * half + 1] = static_cast<uint32_t>(v >> 32);
+              seen[2 * half] |= static_cast<uint32_t>(v);
+              seen[2 * half + 1] |= static_cast<uint32_t>(v >> 32);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.vis_full[b & 1]);
+        bad = bad || !mbar_wait(&m.v_full[st], phase);
+        if (__any_sync(0xffffffffu, bad || *abort_flag)) {
+          if (lane == 0) give_up();
           break;
         }
-        mbar_arrive_expect_tx(&full[st], TILE);
-        tma_load_3d(ring + st * TILE, map, &full[st], 0, it.next(), h, pol);
-        ++issued;
+        if (part) {
+          bool wrote = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!((__reduce_or_sync(0xffffffffu, seen[i]) >> lane) & 1u)) {
+              uint4* row = reinterpret_cast<uint4*>(v_ring + st * TILE + (i * 32 + lane) * HD);
+#pragma unroll
+              for (int c = 0; c < HD / 16; ++c) row[c] = make_uint4(0, 0, 0, 0);
+              wrote = true;
+            }
+          }
+          if (wrote) fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&m.v_clean[st]);
         if (++st == stages) st = 0, phase ^= 1u;
       }
-      if (*abort_flag)  // copies in flight land before the CTA leaves
-        for (int b = max(issued - stages, 0); b < issued; ++b) (void)mbar_wait(&full[b % stages], (b / stages) & 1);
-    }
-  } else if (warp == 10) {
-    if (lane == 0 && nblocks > 0) {
-      const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true);
-      const uint32_t kr = smem_u32(k_ring), vr = smem_u32(v_ring), qh = smem_u32(q_hi), ql = smem_u32(q_lo);
-      int nS = 0, nP = 0, sS = 0, sP = 0;
-      uint32_t phS = 0, phP = 0, idle = 0;
-      const bool ready = mbar_wait(&m.q_ready, 0);
-      if (!ready) give_up();
-      while (ready && nP < nblocks) {
-        bool prog = false;
-        if (nS < nblocks && mbar_test(&m.k_full[sS], phS) &&
-            (nS < 2 || mbar_test(&m.s_free[nS & 1], ((nS >> 1) - 1) & 1))) {
-          tc_fence_after();
-          const uint32_t kb = kr + sS * TILE, d = tmem + (nS & 1) * kQ8MaxRows;
-#pragma unroll
-          for (int ks = 0; ks < HD / 32; ++ks)
-            umma_f8(d, sdesc_q8(kb + ks * 32, 16, SBO, SW), sdesc_q8(qh + ks * 32, 16, SBO, SW), id_s, ks > 0);
-#pragma unroll
-          for (int ks = 0; ks < HD / 32; ++ks)
-            umma_f8(d, sdesc_q8(kb + ks * 32, 16, SBO, SW), sdesc_q8(ql + ks * 32, 16, SBO, SW), id_s, 1u);
-          umma_commit(&m.s_full[nS & 1]);
-          umma_commit(&m.k_empty[sS]);
-          ++nS;
-          if (++sS == stages) sS = 0, phS ^= 1u;
-          prog = true;
-        }
-        if (nP < nS && mbar_test(&m.p_full[nP & 1], (nP >> 1) & 1) && mbar_test(&m.v_clean[sP], phP)) {
-          tc_fence_after();
-          // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
-          // M = 128 repeats the first (lanes 64 .. 127 are not read). P': MN-major, atoms of 32 rows x 8 keys.
-          const uint32_t vb = vr + sP * TILE, pb = p_s + (nP & 1) * 2 * p_bytes;
-          const uint32_t psbo = atoms * 256;
-#pragma unroll
-          for (int term = 0; term < 2; ++term)
-#pragma unroll
-            for (int kk = 0; kk < kQ8Keys / 32; ++kk)
-              umma_f8(tmem + kQ8ColO, sdesc_q8(vb + kk * 32 * HD, 0, SBO, SW),
-                      sdesc_q8(pb + term * p_bytes + kk * 4 * psbo, 256, psbo, 6u), id_o,
-                      (nP > 0 || term > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&m.p_free[nP & 1]);
-          umma_commit(&m.v_empty[sP]);
-          ++nP;
-          if (++sP == stages) sP = 0, phP ^= 1u;
-          prog = true;
-        }
-        idle = prog ? 0u : idle + 1u;
-        if (idle > kWaitLimit || *abort_flag) {
-          give_up();
-          break;
-        }
-      }
-    }
-    if (lane == 0) umma_commit(&m.o_full);
-  } else if (warp == 11) {
-    // Blocks that not every row sees whole: the keys that each token sees, for
-    // the softmax warps, and zeros in the V rows that none does.
-    Q8Blocks it(m, unit_shift);
-    int st = 0;
-    uint32_t phase = 0;
-    for (int b = 0; b < nblocks; ++b) {
-      const int kb = it.next();
-      const bool part = kb < max_start || kb + kQ8Keys > min_len;
-      bool bad = b >= 2 && !mbar_wait(&m.s_free[b & 1], ((b >> 1) - 1) & 1);  // vis[b & 1] was read for b - 2
-      uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
-      if (part) {
-        seen[0] = seen[1] = seen[2] = seen[3] = 0u;
-        for (int i = lane; i < ntok; i += 32) {
-          const uint64_t* mask = a.mask + (int64_t)(t0 + i) * a.mask_words;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint64_t v = q8_seen_bits(kb + 64 * half, m.start[i], m.len[i], mask, a.mask_words, sb, a.kv_end);
-            m.vis[b & 1][i][2 * half] = static_cast<uint32_t>(v);
-            m.vis[b & 1][i][2 * half + 1] = static_cast<uint32_t>(v >> 32);
-            seen[2 * half] |= static_cast<uint32_t>(v);
-            seen[2 * half + 1] |= static_cast<uint32_t>(v >> 32);
-          }
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.vis_full[b & 1]);
-      bad = bad || !mbar_wait(&m.v_full[st], phase);
-      if (__any_sync(0xffffffffu, bad) || *abort_flag) {
-        if (lane == 0) give_up();
-        break;
-      }
-      if (part) {
-        bool wrote = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (!((__reduce_or_sync(0xffffffffu, seen[i]) >> lane) & 1u)) {
-            uint4* row = reinterpret_cast<uint4*>(v_ring + st * TILE + (i * 32 + lane) * HD);
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c) row[c] = make_uint4(0, 0, 0, 0);
-            wrote = true;
-          }
-        }
-        if (wrote) fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (lane == 0) mbar_arrive(&m.v_clean[st]);
-      if (++st == stages) st = 0, phase ^= 1u;
     }
   } else {
     // ---- softmax warps: the queries, then thread = key
+    const int wg = warp >> 2, quarter = warp & 3;
+    const int my_chunks = ALT ? n_chunks : wg == 0 ? CH : n_chunks - CH;
+    const int col_base = ALT || wg == 0 ? 0 : 16 * CH;
+    const int ref_base = ALT ? wg * 16 * CH : col_base;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t to = tmem + kQ8ColO + (ALT ? wg * kQ8AltRows : 0) + lane_base + col_base;
     const int key = quarter * 32 + lane;
     const uint8_t* ksc = a.ks + (int64_t)h * a.scale_head_stride;
     const uint8_t* vsc = a.vs + (int64_t)h * a.scale_head_stride;
     const uint32_t p_at = (key >> 3) * atoms * 256 + (key & 7) * 32;
     const uint32_t p_flip = (key >> 2) & 1;
-    Q8Blocks it(m, unit_shift);
+    const uint64_t minus1 = f2_pack(-1.f, -1.f);
+    q8_queries<HD, ALT ? 16 * CH : 32 * CH>(a, m, q_hi, q_lo, N, nrows, t0, h, ALT ? 16 * CH : 0);
+    fence_proxy_async_smem();
+    __syncwarp();
+    named_bar_sync(3, 256);  // the references are read by other warps than wrote them
+    if (lane == 0) mbar_arrive(&m.q_ready);
+    bool bad = !mbar_wait(&m.meta_ready, 0);
+    if (bad) give_up();
+    const int count = bad ? 0 : m.count;
+    const int nblocks = count << unit_shift;
+    const int max_start = m.max_start, min_len = m.min_len;
+    Q8Blocks it(m.map, bad ? 0 : m.first, count, unit_shift);
+    constexpr int STEP = ALT ? 2 : 1;
+    const int b0 = ALT ? wg : 0;
     int kb = 0, kbyte = 0, vbyte = 0;
-    auto fetch = [&] {
+    auto fetch = [&](int b) {  // block b's slot and the key's scale bytes
+      if (b >= nblocks || my_chunks == 0) return;
+      if (ALT && b > 0) (void)it.next();  // the other warpgroup's
       kb = it.next();
       const bool in = kb + key < a.kv_end;
       kbyte = in ? ksc[kb + key] : 0;
       vbyte = in ? vsc[kb + key] : 0;
     };
-    if (nblocks > 0 && my_chunks > 0) fetch();
-    q8_queries<HD>(a, m, q_hi, q_lo, N, nrows, t0, h);
-    fence_proxy_async_smem();
-    named_bar_sync(3, 256);  // the references are read by other warps than wrote them
-    if (lane == 0) mbar_arrive(&m.q_ready);
-    bool bad = false;
-    for (int b = 0; b < (my_chunks > 0 ? nblocks : 0); ++b) {
+    fetch(b0);
+    float l[16 * CH];
+#pragma unroll
+    for (int i = 0; i < 16 * CH; ++i) l[i] = 0.f;
+    for (int b = b0; b < (my_chunks > 0 ? nblocks : 0); b += STEP) {
       const int buf = b & 1;
       const bool part = kb < max_start || kb + kQ8Keys > min_len;
       const float ck = q8_scale(kbyte);
@@ -964,7 +1031,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       const float ev = static_cast<float>(vb - 127);
       const float inv_v = q8_inv_scale(vb);
       const uint64_t ck2 = f2_pack(ck, ck), ev2 = f2_pack(ev, ev), iv2 = f2_pack(inv_v, inv_v);
-      if (b + 1 < nblocks) fetch();
+      fetch(b + STEP);
       // After a timeout the loop runs on without waiting: the warpgroup's barriers stay matched.
       if (!bad && (*abort_flag || !mbar_wait(&m.s_full[buf], (b >> 1) & 1))) {
         bad = true;
@@ -978,26 +1045,33 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       tc_fence_after();
       const uint32_t ts = tmem + buf * kQ8MaxRows + lane_base + col_base;
       const uint32_t pb = p_s + buf * 2 * p_bytes + p_at;
-      const uint64_t minus1 = f2_pack(-1.f, -1.f);
       // Scores to exponents; with up to KEEP chunks they stay in registers
       // for the weights below, with more they are computed again there.
       float x[16 * KEEP];
 #pragma unroll 1
       for (int pass = 0; pass < 2; ++pass) {
         float top = -INFINITY;
+        if (CH <= KEEP) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+            if (c < my_chunks) q8_tmem_ld16(ts + c * 16, x + 16 * (c % KEEP));
+        }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           if (c < my_chunks) {
-            float* xc = x + 16 * (CH <= KEEP ? c : 0);
+            float* xc = x + 16 * (c % KEEP);
             const uint32_t vis = part ? q8_chunk_vis(m, buf, col_base + c * 16, a.G, ntok, quarter, lane) : 0xffffu;
-            q8_tmem_ld16(ts + c * 16, xc);
+            if (CH > KEEP) q8_tmem_ld16(ts + c * 16, xc);
             q8_tmem_wait16(xc);
-            top = fmaxf(top, q8_exponents(m, col_base + c * 16, xc, ck2, ev2, part, vis));
+            top = fmaxf(top, q8_exponents(m.rowc + col_base + c * 16, m.bias_ref + ref_base + c * 16, xc, ck2, ev2, part,
+                                          vis));
           }
         }
         if (!named_bar_or(1 + wg, 128, top > kQ8Bias + kQ8Grow)) break;
-        if (!q8_move_references(m, ts, tmem + kQ8ColO + lane_base + col_base, col_base, my_chunks, wg, ck, ev, part, buf,
-                                a.G, ntok, b > 0 && !bad ? &m.p_free[buf ^ 1] : nullptr, ((b - 1) >> 1) & 1)) {
+        const bool first = b < (ALT ? 2 : 1) || bad;
+        if (!q8_move_references(m, ts, to, col_base, ref_base, my_chunks, wg, ck, ev, part, buf, a.G, ntok,
+                                first ? nullptr : &m.p_free[ALT ? buf : buf ^ 1],
+                                (ALT ? (b >> 1) - 1 : (b - 1) >> 1) & 1)) {
           bad = true;
           give_up();
         }
@@ -1005,7 +1079,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
         for (int c = 0; c < CH; ++c) {
           if (c < my_chunks) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) l[c * 16 + j] *= m.alpha[col_base + c * 16 + j];
+            for (int j = 0; j < 16; ++j) l[c * 16 + j] *= m.alpha[ref_base + c * 16 + j];
           }
         }
       }
@@ -1022,12 +1096,12 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
           const int col = col_base + c * 16;
-          float* xc = x + 16 * (CH <= KEEP ? c : 0);
+          float* xc = x + 16 * (c % KEEP);
           if (CH > KEEP) {
             const uint32_t vis = part ? q8_chunk_vis(m, buf, col, a.G, ntok, quarter, lane) : 0xffffu;
             q8_tmem_ld16(ts + c * 16, xc);
             q8_tmem_wait16(xc);
-            (void)q8_exponents(m, col, xc, ck2, ev2, part, vis);
+            (void)q8_exponents(m.rowc + col, m.bias_ref + ref_base + c * 16, xc, ck2, ev2, part, vis);
           }
           uint32_t hi[4], lo[4];
 #pragma unroll
@@ -1065,65 +1139,92 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
         mbar_arrive(&m.p_full[buf]);
       }
     }
-  }
-  // ---- results: l summed over the 128 keys' threads, O^T read back (lane = head dim)
-  __syncwarp();
-  float* s_l = reinterpret_cast<float*>(p_buf);  // [4][N]: the P buffers are free once every MMA retired
-  if (warp < 8 && my_chunks > 0) {
-    if (!mbar_wait(&m.o_full, 0) && lane == 0) give_up();
-    tc_fence_after();
-    named_bar_sync(3, two ? 256 : 128);  // (a timed-out warp may still have been writing P)
+    // ---- results: l summed over the 128 keys' threads, O^T read back (lane = head dim)
+    if (two || wg == 0) {
+      const int parties = two ? 256 : 128;
+      if (!mbar_wait(&m.o_full, 0)) give_up();
+      tc_fence_after();
+      __syncwarp();
+      named_bar_sync(3, parties);
+      float* s_l = reinterpret_cast<float*>(p_buf);  // [ALT: 2][4][N]: the P buffers are free once every MMA retired
+      float* s_f = s_l + 8 * N;                       // [2][N] factors of the O accumulators
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      if (c < my_chunks) {
-        const float sum = q8_columns_reduce<false>(l + c * 16, lane);
-        if (lane < 16) s_l[quarter * N + col_base + c * 16 + lane] = sum;
+      for (int c = 0; c < CH; ++c) {
+        if (c < my_chunks) {
+          const float sum = q8_columns_reduce<false>(l + c * 16, lane);
+          if (lane < 16) s_l[((ALT ? wg * 4 : 0) + quarter) * N + col_base + c * 16 + lane] = sum;
+        }
       }
-    }
-    __syncwarp();
-    named_bar_sync(1 + wg, 128);
-    // thread i of the warpgroup: row col_base + i's sum, as the factor of its output or the record {M, l}
-    const int64_t rec0 = ((int64_t)blockIdx.x * a.n_splits + split) * kQ8MaxRows;
-    const int i = threadIdx.x & 127;
-    if (i < 16 * my_chunks) {
-      const int r = col_base + i;
-      const float sum = (s_l[r] + s_l[N + r]) + (s_l[2 * N + r] + s_l[3 * N + r]);
-      m.alpha[r] = sum == 0.f ? 0.f : 1.f / sum;
-      if (a.n_splits > 1 && r < nrows) {
-        float* ml = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD + (rec0 + r) * 2;
-        *reinterpret_cast<float2*>(ml) = make_float2(kQ8Bias - m.bias_ref[r], sum);
-      }
-    }
-    __syncwarp();
-    named_bar_sync(1 + wg, 128);
-    const int d = quarter * 32 + lane;
-    if (quarter * 32 < HD && nblocks > 0) {
-#pragma unroll 1
-      for (int c = 0; c < my_chunks; ++c) {
-        const int col = col_base + c * 16;
-        float o[16];
-        tmem_ld16(tmem + kQ8ColO + lane_base + col, o);
+      __syncwarp();
+      named_bar_sync(3, parties);
+      // thread i: row i's factors, and the record {M, l} of a slice
+      const int64_t rec0 = ((int64_t)blockIdx.x * a.n_splits + split) * kQ8MaxRows;
+      const int i = threadIdx.x;
+      if (i < N) {
+        float sum = (s_l[i] + s_l[N + i]) + (s_l[2 * N + i] + s_l[3 * N + i]), f0 = 1.f, f1 = 0.f;
+        float ref = kQ8Bias - m.bias_ref[i];
+        if (ALT) {  // join the warpgroups' halves of the slice
+          const float* s1 = s_l + 4 * N;
+          const float other = (s1[i] + s1[N + i]) + (s1[2 * N + i] + s1[3 * N + i]);
+          const float ref1 = kQ8Bias - m.bias_ref[16 * CH + i];
+          const float top = other == 0.f ? ref : sum == 0.f ? ref1 : fmaxf(ref, ref1);
+          f0 = sum == 0.f ? 0.f : exp2f(ref - top);
+          f1 = other == 0.f ? 0.f : exp2f(ref1 - top);
+          sum = fmaf(f0, sum, f1 * other);
+          ref = top;
+        }
         if (a.n_splits > 1) {
-          float* dst = a.part + (rec0 + col) * HD + d;
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (col + j < nrows) dst[j * HD] = o[j];
+          if (i < nrows) {
+            float* ml = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD + (rec0 + i) * 2;
+            *reinterpret_cast<float2*>(ml) = make_float2(ref, sum);
+          }
         } else {
-          int tok = col / a.G, g = col - tok * a.G;
-          bf16* base = static_cast<bf16*>(a.out) + (int64_t)h * a.G * HD + d;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          f0 *= inv;
+          f1 *= inv;
+        }
+        s_f[i] = nblocks > 0 ? f0 : 0.f;  // (an O that no block wrote is not read)
+        s_f[N + i] = ALT && nblocks > 1 ? f1 : 0.f;
+      }
+      __syncwarp();
+      named_bar_sync(3, parties);
+      const int d = quarter * 32 + lane;
+      if (quarter * 32 < HD) {
+        const uint32_t o0 = tmem + kQ8ColO + lane_base;
+#pragma unroll 1
+        for (int c = ALT ? wg : col_base / 16; c < (ALT ? n_chunks : col_base / 16 + my_chunks); c += STEP) {
+          const int col = c * 16;
+          float o[16], u[16];
+          tmem_ld16(o0 + col, o);
+          if (ALT) tmem_ld16(o0 + kQ8AltRows + col, u);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float f = m.alpha[col + j];
-            if (col + j < nrows) base[(int64_t)(t0 + tok) * a.ldo + g * HD] = f2bf(f == 0.f ? 0.f : o[j] * f);
-            if (++g == a.G) g = 0, ++tok;
+            const float f0 = s_f[col + j];
+            o[j] = f0 == 0.f ? 0.f : f0 * o[j];
+            if (ALT) {
+              const float f1 = s_f[N + col + j];
+              o[j] = f1 == 0.f ? o[j] : fmaf(f1, u[j], o[j]);
+            }
+          }
+          if (a.n_splits > 1) {
+            float* dst = a.part + (rec0 + col) * HD + d;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (col + j < nrows) dst[j * HD] = o[j];
+          } else {
+            int tok = col / a.G, g = col - tok * a.G;
+            bf16* base = static_cast<bf16*>(a.out) + (int64_t)h * a.G * HD + d;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (col + j < nrows) base[(int64_t)(t0 + tok) * a.ldo + g * HD] = f2bf(o[j]);
+              if (++g == a.G) g = 0, ++tok;
+            }
           }
         }
       }
-    } else if (quarter * 32 < HD && a.n_splits == 1) {
-      for (int r = col_base; r < min(col_base + 16 * my_chunks, nrows); ++r)
-        static_cast<bf16*>(a.out)[(int64_t)(t0 + r / a.G) * a.ldo + (int64_t)(h * a.G + r % a.G) * HD + d] = f2bf(0.f);
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 10) {
@@ -1207,7 +1308,7 @@ static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64
   a.tiles = (a.T + tpg - 1) / tpg;
   tpg = (a.T + a.tiles - 1) / a.tiles;
   a.tiles = (a.T + tpg - 1) / tpg;
-  const int chunks = (tpg * a.G + 15) / 16, ch = (chunks + 1) / 2;
+  const int chunks = (tpg * a.G + 15) / 16;
   const int64_t blocks = (int64_t)a.n_kv * a.tiles;
   if (blocks > INT32_MAX) return fail(SSD_ERR_UNSUPPORTED, "ssd_tree_attention_q8: too many row groups");
   const int key_blocks = (a.kv_end + kQ8Keys - 1) / kQ8Keys;
@@ -1232,16 +1333,20 @@ static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64
   int stages = (232448 - fixed) / (2 * kQ8Keys * HD);
   if (stages > kQ8MaxStages) stages = kQ8MaxStages;
   const size_t smem = (size_t)fixed + (size_t)stages * 2 * kQ8Keys * HD;
-  void (*const kerns[5])(const AttnQ8Maps, const AttnQ8Args, int, int, int, int) = {
-      attn_q8_tc_kernel<HD, 1>, attn_q8_tc_kernel<HD, 2>, attn_q8_tc_kernel<HD, 3>, attn_q8_tc_kernel<HD, 4>,
-      attn_q8_tc_kernel<HD, 5>};
+  typedef void (*Kern)(const AttnQ8Maps, const AttnQ8Args, int, int, int, int);
+  const Kern alt[5] = {attn_q8_tc_kernel<HD, 1, true>, attn_q8_tc_kernel<HD, 2, true>, attn_q8_tc_kernel<HD, 3, true>,
+                       attn_q8_tc_kernel<HD, 4, true>, attn_q8_tc_kernel<HD, 5, true>};
+  const Kern half[3] = {attn_q8_tc_kernel<HD, 3, false>, attn_q8_tc_kernel<HD, 4, false>,
+                        attn_q8_tc_kernel<HD, 5, false>};
   static bool set = false;
   if (!set) {
-    for (auto k : kerns) allow_max_dynamic_smem(k);
+    for (Kern k : alt) allow_max_dynamic_smem(k);
+    for (Kern k : half) allow_max_dynamic_smem(k);
     set = true;
   }
-  int rc = launch_kernel("attn_q8_tc_kernel", kerns[ch - 1], dim3((unsigned)blocks, (unsigned)splits),
-                         dim3(kQ8Threads), smem, stream, 1u, 1u, maps, a, chunks, tpg, stages, shift);
+  const Kern kern = chunks * 16 <= kQ8AltRows ? alt[chunks - 1] : half[(chunks + 1) / 2 - 3];
+  int rc = launch_kernel("attn_q8_tc_kernel", kern, dim3((unsigned)blocks, (unsigned)splits), dim3(kQ8Threads), smem,
+                         stream, 1u, 1u, maps, a, chunks, tpg, stages, shift);
   if (rc || splits == 1) return rc;
   return launch_kernel("attn_q8_join_kernel", attn_q8_join_kernel<HD>,
                        dim3((unsigned)blocks, (unsigned)((tpg * a.G + 7) / 8)), dim3(256), 0, stream, 1u, 1u, a, tpg);
