@@ -320,12 +320,12 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 // Scales never touch the operands: a softmax thread owns one key (= TMEM
 // lane), so 2^ek is a factor of its scores and 2^ev an addend in its exponent,
 //   t = s log2 e + ev,  P' = 2^(t - M + kBias),  l += P' 2^-ev,
-// with M a per-row reference (power-of-two scale of O and l). M is the true
-// maximum of t over the row's first visible block and moves only when some t
-// exceeds it by kGrow (then O and l are rescaled), so the usual block needs no
-// reduction over keys, only one vote. P' <= 2^(kBias + kGrow) < 448; its
-// second term rounds at 2^-10, i.e. 2^-13 of the weight at the reference, and
-// l sums the unrounded P' in fp32 per thread until the end.
+// with M a whole number per row that scales O and l. A block's column maxima
+// (one warp reduction instruction per column and warp, joined in shared memory)
+// move M only when some t exceeds it by kGrow; then O and l shift by whole
+// powers of two. P' <= 2^(kBias + kGrow) < 448; its second term rounds at
+// 2^-10, i.e. 2^-13 of the weight at the reference, and l sums the unrounded
+// P' in fp32 per thread until the end.
 //
 // A CTA = one KV head x up to 144 query rows (whole tokens) x one slice of the
 // key blocks that some row sees (a bitmap in shared memory: slot ranges of
@@ -339,7 +339,6 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 constexpr int kQ8Keys = 128;
 constexpr int kQ8MaxRows = 144;       // query rows per CTA: three ring stages fit next to their Q and P'
 constexpr int kQ8AltRows = 80;        // up to here the warpgroups take blocks in turn
-constexpr int kQ8RowState = 160;      // rows of per-row state: 144, or 2 x 80
 constexpr int kQ8Threads = 384;
 constexpr int kQ8MaxStages = 6;
 constexpr int kQ8MapWords = 256;      // bitmap of key blocks (units of 2^unit_shift blocks)
@@ -354,9 +353,9 @@ struct AttnQ8Maps {
 
 struct AttnQ8Meta {
   float rowc[kQ8MaxRows];                      // 2^eq scale log2 e per query row
-  float bias_ref[kQ8RowState];                 // kBias - M (ALT: per warpgroup, 16 CH rows apart)
-  float alpha[kQ8RowState];                    // reference moves: factors of O and l
-  float wmax[4][kQ8RowState];                  // reference moves: column maxima of a warp's 32 keys
+  float bias_ref[8][kQ8AltRows];               // kBias - M of the columns of each softmax warp (four alike)
+  float wmax[2][4][kQ8AltRows];                // per warpgroup: column maxima of a warp's 32 keys
+  uint8_t shift[8][kQ8AltRows];                // per softmax warp: log2 of the last move of M (255: O and l restart)
   int len[kQ8MaxRows], start[kQ8MaxRows];      // per token
   uint32_t vis[2][kQ8MaxRows][4];              // per block buffer and token: which of the block's keys it sees
   uint32_t map[kQ8MapWords];
@@ -552,7 +551,7 @@ __device__ __forceinline__ void q8_slice(const AttnQ8Meta& m, int split, int n_s
 // all its rows before it converts the first.
 template <int HD, int ROWS>
 __device__ __forceinline__ void q8_queries(const AttnQ8Args& a, AttnQ8Meta& m, uint8_t* q_hi, uint8_t* q_lo, int N,
-                                           int nrows, int t0, int h, int second_ref) {
+                                           int nrows, int t0, int h) {
   constexpr int LPR = HD / 8, RPP = 256 / LPR, BATCH = (ROWS + RPP - 1) / RPP;
   const bf16* qb = static_cast<const bf16*>(a.q);
   const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0;
@@ -610,8 +609,6 @@ __device__ __forceinline__ void q8_queries(const AttnQ8Args& a, AttnQ8Meta& m, u
       *reinterpret_cast<uint2*>(q_lo + at) = make_uint2(lo[0], lo[1]);
       if (l8 == 0) {
         m.rowc[r] = fine ? q8_scale(byte) * (a.scale * 1.4426950408889634f) : __int_as_float(0x7fffffff);
-        m.bias_ref[r] = r < nrows ? kQ8Unset : -kQ8Unset;  // columns past the rows: P' = 0
-        if (second_ref) m.bias_ref[second_ref + r] = r < nrows ? kQ8Unset : -kQ8Unset;
       }
     }
   }
@@ -649,67 +646,10 @@ __device__ __forceinline__ float q8_columns_reduce(float* v, int lane) {
   return MAX ? fmaxf(v[0], got) : v[0] + got;
 }
 
-// Some of the warpgroup's references move: column maxima of t over the
-// block's 128 keys, new references and factors into shared memory, O's columns
-// rescaled. The warpgroup's columns start at `col` of the query rows and at
-// `ref` of the per-row state, `ts` / `to` of S^T and O^T in TMEM. `pv_done`
-// completes `parity` when the last P V into this O has retired (NULL: there is
-// none yet). Returns false on a timeout. All 128 threads call it; out of line,
-// as most blocks do not need it.
-__device__ __noinline__ bool q8_move_references(AttnQ8Meta& m, uint32_t ts, uint32_t to, int col, int ref, int chunks,
-                                                int wg, float ck, float ev, bool part, int buf, int G, int ntok,
-                                                uint64_t* pv_done, uint32_t parity) {
-  const int tid = threadIdx.x & 127, quarter = tid >> 5, lane = tid & 31;
-  for (int c = 0; c < chunks; ++c) {
-    const uint32_t vis = part ? q8_chunk_vis(m, buf, col + c * 16, G, ntok, quarter, lane) : 0xffffu;
-    float t[16];
-    tmem_ld16(ts + c * 16, t);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      t[j] = fmaf(t[j] * m.rowc[col + c * 16 + j], ck, ev);
-      if (!((vis >> j) & 1u)) t[j] = -INFINITY;
-    }
-    const float top = q8_columns_reduce<true>(t, lane);
-    if (lane < 16) m.wmax[quarter][ref + c * 16 + lane] = top;
-  }
-  __syncwarp();
-  named_bar_sync(1 + wg, 128);
-  if (tid < 16 * chunks) {
-    const int r = ref + tid;
-    const float mx = fmaxf(fmaxf(m.wmax[0][r], m.wmax[1][r]), fmaxf(m.wmax[2][r], m.wmax[3][r]));
-    const float old = m.bias_ref[r];
-    const bool move = mx + old > kQ8Bias + kQ8Grow;
-    const float now = move ? kQ8Bias - mx : old;
-    m.alpha[r] = !move ? 1.f : old == kQ8Unset ? 0.f : exp2f(now - old);
-    m.bias_ref[r] = now;
-  }
-  __syncwarp();
-  named_bar_sync(1 + wg, 128);
-  if (!pv_done) return true;
-  bool ok = true, waited = false;
-  for (int c = 0; c < chunks; ++c) {
-    float f[16];
-    bool any = false;
-#pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(&m.alpha[ref + c * 16 + j]);
-      f[j] = v.x, f[j + 1] = v.y, f[j + 2] = v.z, f[j + 3] = v.w;
-      any = any || v.x != 1.f || v.y != 1.f || v.z != 1.f || v.w != 1.f;
-    }
-    if (!any) continue;  // uniform
-    if (!waited) {
-      ok = mbar_wait(pv_done, parity);
-      tc_fence_after();
-      waited = true;
-    }
-    float o[16];
-    tmem_ld16(to + c * 16, o);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] = f[j] == 0.f ? 0.f : o[j] * f[j];
-    tmem_st16(to + c * 16, o);
-  }
-  if (waited) tmem_wait_st();
-  return ok;
+// The last move of M, as a factor of O and l.
+__device__ __forceinline__ float q8_shift_factor(uint32_t bytes, int i) {
+  const uint32_t k = (bytes >> (8 * i)) & 0xffu;
+  return k > 126u ? 0.f : __uint_as_float((127u - k) << 23);
 }
 
 // TMEM load without its wait; the wait takes the registers along so that
@@ -730,30 +670,25 @@ __device__ __forceinline__ void q8_tmem_wait16(float* v) {
                : "memory");
 }
 
-// x[j] = exponent of P' for 16 columns, from their scores (x: raw products).
-// Returns the largest.
-__device__ __forceinline__ float q8_exponents(const float* rowc, const float* bias_ref, float* x, uint64_t ck2,
-                                              uint64_t ev2, bool part, uint32_t vis) {
+// t of 16 columns from their raw products x, in place.
+__device__ __forceinline__ void q8_scores(const float* rowc, float* x, uint64_t ck2, uint64_t ev2, bool part,
+                                          uint32_t vis) {
   const ulonglong2* rc = reinterpret_cast<const ulonglong2*>(rowc);
-  const ulonglong2* rf = reinterpret_cast<const ulonglong2*>(bias_ref);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const ulonglong2 r = rc[j], f = rf[j];
-    f2_unpack(f2_add(f2_fma(f2_mul(f2_pack(x[4 * j], x[4 * j + 1]), r.x), ck2, ev2), f.x), x[4 * j], x[4 * j + 1]);
-    f2_unpack(f2_add(f2_fma(f2_mul(f2_pack(x[4 * j + 2], x[4 * j + 3]), r.y), ck2, ev2), f.y), x[4 * j + 2],
-              x[4 * j + 3]);
+    const ulonglong2 r = rc[j];
+    f2_unpack(f2_fma(f2_mul(f2_pack(x[4 * j], x[4 * j + 1]), r.x), ck2, ev2), x[4 * j], x[4 * j + 1]);
+    f2_unpack(f2_fma(f2_mul(f2_pack(x[4 * j + 2], x[4 * j + 3]), r.y), ck2, ev2), x[4 * j + 2], x[4 * j + 3]);
   }
   if (part) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) x[j] = (vis >> j) & 1u ? x[j] : -INFINITY;
   }
-  float t0 = fmaxf(x[0], x[1]), t1 = fmaxf(x[2], x[3]);
-#pragma unroll
-  for (int j = 4; j < 16; j += 4) {
-    t0 = fmaxf(t0, fmaxf(x[j], x[j + 1]));
-    t1 = fmaxf(t1, fmaxf(x[j + 2], x[j + 3]));
-  }
-  return fmaxf(t0, t1);
+}
+__device__ __forceinline__ float q8_warp_max(float v) {  // NaN gives way to numbers, as in fmaxf
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 template <int HD, int CH, bool ALT>
@@ -988,7 +923,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
     const int wg = warp >> 2, quarter = warp & 3;
     const int my_chunks = ALT ? n_chunks : wg == 0 ? CH : n_chunks - CH;
     const int col_base = ALT || wg == 0 ? 0 : 16 * CH;
-    const int ref_base = ALT ? wg * 16 * CH : col_base;
+    float* const my_ref = m.bias_ref[warp];
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t to = tmem + kQ8ColO + (ALT ? wg * kQ8AltRows : 0) + lane_base + col_base;
     const int key = quarter * 32 + lane;
@@ -997,10 +932,12 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
     const uint32_t p_at = (key >> 3) * atoms * 256 + (key & 7) * 32;
     const uint32_t p_flip = (key >> 2) & 1;
     const uint64_t minus1 = f2_pack(-1.f, -1.f);
-    q8_queries<HD, ALT ? 16 * CH : 32 * CH>(a, m, q_hi, q_lo, N, nrows, t0, h, ALT ? 16 * CH : 0);
+    q8_queries<HD, ALT ? 16 * CH : 32 * CH>(a, m, q_hi, q_lo, N, nrows, t0, h);
+    for (int i = lane; i < 16 * CH; i += 32)  // columns past the rows: P' = 0
+      my_ref[i] = col_base + i < nrows ? kQ8Unset : -kQ8Unset;
     fence_proxy_async_smem();
     __syncwarp();
-    named_bar_sync(3, 256);  // the references are read by other warps than wrote them
+    named_bar_sync(3, 256);  // the rows' scales are read by other warps than wrote them
     if (lane == 0) mbar_arrive(&m.q_ready);
     bool bad = !mbar_wait(&m.meta_ready, 0);
     if (bad) give_up();
@@ -1045,43 +982,86 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       tc_fence_after();
       const uint32_t ts = tmem + buf * kQ8MaxRows + lane_base + col_base;
       const uint32_t pb = p_s + buf * 2 * p_bytes + p_at;
-      // Scores to exponents; with up to KEEP chunks they stay in registers
-      // for the weights below, with more they are computed again there.
+      // t of every column and its maximum over the warp's keys. With up to KEEP
+      // chunks t stays in registers, with more it is computed again below.
       float x[16 * KEEP];
-#pragma unroll 1
-      for (int pass = 0; pass < 2; ++pass) {
-        float top = -INFINITY;
-        if (CH <= KEEP) {
+      if (CH <= KEEP) {
 #pragma unroll
-          for (int c = 0; c < CH; ++c)
-            if (c < my_chunks) q8_tmem_ld16(ts + c * 16, x + 16 * (c % KEEP));
-        }
+        for (int c = 0; c < CH; ++c)
+          if (c < my_chunks) q8_tmem_ld16(ts + c * 16, x + 16 * (c % KEEP));
+      }
+      // (halves: s_full(b) does not say that the other warps have read the last block's maxima)
+      if (!ALT) named_bar_sync(1 + wg, 128);
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          if (c < my_chunks) {
-            float* xc = x + 16 * (c % KEEP);
-            const uint32_t vis = part ? q8_chunk_vis(m, buf, col_base + c * 16, a.G, ntok, quarter, lane) : 0xffffu;
-            if (CH > KEEP) q8_tmem_ld16(ts + c * 16, xc);
-            q8_tmem_wait16(xc);
-            top = fmaxf(top, q8_exponents(m.rowc + col_base + c * 16, m.bias_ref + ref_base + c * 16, xc, ck2, ev2, part,
-                                          vis));
+      for (int c = 0; c < CH; ++c) {
+        if (c < my_chunks) {
+          float* xc = x + 16 * (c % KEEP);
+          const uint32_t vis = part ? q8_chunk_vis(m, buf, col_base + c * 16, a.G, ntok, quarter, lane) : 0xffffu;
+          if (CH > KEEP) q8_tmem_ld16(ts + c * 16, xc);
+          q8_tmem_wait16(xc);
+          q8_scores(m.rowc + col_base + c * 16, xc, ck2, ev2, part, vis);
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 top = make_float4(q8_warp_max(xc[j]), q8_warp_max(xc[j + 1]), q8_warp_max(xc[j + 2]),
+                                           q8_warp_max(xc[j + 3]));
+            if (lane == 0) *reinterpret_cast<float4*>(&m.wmax[wg][quarter][c * 16 + j]) = top;
           }
         }
-        if (!named_bar_or(1 + wg, 128, top > kQ8Bias + kQ8Grow)) break;
-        const bool first = b < (ALT ? 2 : 1) || bad;
-        if (!q8_move_references(m, ts, to, col_base, ref_base, my_chunks, wg, ck, ev, part, buf, a.G, ntok,
-                                first ? nullptr : &m.p_free[ALT ? buf : buf ^ 1],
-                                (ALT ? (b >> 1) - 1 : (b - 1) >> 1) & 1)) {
+      }
+      __syncwarp();
+      named_bar_sync(1 + wg, 128);
+      // lane i: columns i, i + 32, ... (each warp for itself, all alike)
+      float now[(16 * CH + 31) / 32];
+      uint32_t by[(16 * CH + 31) / 32];
+      bool moves = false;
+#pragma unroll
+      for (int k = 0; k < (16 * CH + 31) / 32; ++k) {
+        const int i = lane + 32 * k;
+        by[k] = 0u;
+        if (i < 16 * my_chunks) {
+          const float mx = fmaxf(fmaxf(m.wmax[wg][0][i], m.wmax[wg][1][i]), fmaxf(m.wmax[wg][2][i], m.wmax[wg][3][i]));
+          const float old = my_ref[i];
+          now[k] = kQ8Bias - ceilf(mx);
+          if (mx + old > kQ8Bias + kQ8Grow) by[k] = old == kQ8Unset ? 255u : static_cast<uint32_t>(fminf(old - now[k], 255.f));
+          moves = moves || by[k];
+        }
+      }
+      if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+        for (int k = 0; k < (16 * CH + 31) / 32; ++k) {
+          const int i = lane + 32 * k;
+          if (i < 16 * my_chunks) {
+            if (by[k]) my_ref[i] = now[k];
+            m.shift[warp][i] = static_cast<uint8_t>(by[k]);
+          }
+        }
+        __syncwarp();
+        const bool has_o = b >= (ALT ? 2 : 1);
+        // the last P V into this O: block b - 2 of this warpgroup, or block b - 1
+        if (has_o && !bad && !mbar_wait(&m.p_free[ALT ? buf : buf ^ 1], (ALT ? (b >> 1) - 1 : (b - 1) >> 1) & 1)) {
           bad = true;
           give_up();
         }
+        tc_fence_after();
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           if (c < my_chunks) {
+            const uint4 sh = *reinterpret_cast<const uint4*>(&m.shift[warp][c * 16]);
+            if (sh.x | sh.y | sh.z | sh.w) {
+              const uint32_t w[4] = {sh.x, sh.y, sh.z, sh.w};
+              float o[16];
+              if (has_o) tmem_ld16(to + c * 16, o);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) l[c * 16 + j] *= m.alpha[ref_base + c * 16 + j];
+              for (int j = 0; j < 16; ++j) {
+                const float f = q8_shift_factor(w[j >> 2], j & 3);
+                l[c * 16 + j] *= f;
+                o[j] = has_o && f != 0.f ? o[j] * f : 0.f;
+              }
+              if (has_o) tmem_st16(to + c * 16, o);
+            }
           }
         }
+        tmem_wait_st();
       }
       if (CH <= KEEP) {
         tc_fence_before();
@@ -1101,15 +1081,17 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
             const uint32_t vis = part ? q8_chunk_vis(m, buf, col, a.G, ntok, quarter, lane) : 0xffffu;
             q8_tmem_ld16(ts + c * 16, xc);
             q8_tmem_wait16(xc);
-            (void)q8_exponents(m.rowc + col, m.bias_ref + ref_base + c * 16, xc, ck2, ev2, part, vis);
+            q8_scores(m.rowc + col, xc, ck2, ev2, part, vis);
           }
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
+            const float4 ref = *reinterpret_cast<const float4*>(my_ref + c * 16 + 4 * j);
+            const float r[4] = {ref.x, ref.y, ref.z, ref.w};
             float t4[4], r4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              xc[4 * j + e] = q8_ex2(xc[4 * j + e]);
+              xc[4 * j + e] = q8_ex2(xc[4 * j + e] + r[e]);
               t4[e] = __uint_as_float(__float_as_uint(xc[4 * j + e]) & 0xfff00000u);  // 4 significant bits
             }
 #pragma unroll
@@ -1162,11 +1144,12 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       const int i = threadIdx.x;
       if (i < N) {
         float sum = (s_l[i] + s_l[N + i]) + (s_l[2 * N + i] + s_l[3 * N + i]), f0 = 1.f, f1 = 0.f;
-        float ref = kQ8Bias - m.bias_ref[i];
+        const float* refs = ALT || i < 16 * CH ? m.bias_ref[0] + i : m.bias_ref[4] + (i - 16 * CH);
+        float ref = kQ8Bias - *refs;
         if (ALT) {  // join the warpgroups' halves of the slice
           const float* s1 = s_l + 4 * N;
           const float other = (s1[i] + s1[N + i]) + (s1[2 * N + i] + s1[3 * N + i]);
-          const float ref1 = kQ8Bias - m.bias_ref[16 * CH + i];
+          const float ref1 = kQ8Bias - m.bias_ref[4][i];
           const float top = other == 0.f ? ref : sum == 0.f ? ref1 : fmaxf(ref, ref1);
           f0 = sum == 0.f ? 0.f : exp2f(ref - top);
           f1 = other == 0.f ? 0.f : exp2f(ref1 - top);
