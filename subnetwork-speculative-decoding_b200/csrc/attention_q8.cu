@@ -329,23 +329,38 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 //
 // A CTA = one KV head x up to 144 query rows (whole tokens) x one slice of the
 // key blocks that some row sees (a bitmap in shared memory: slot ranges of
-// other sequences in between are not read). Warps 0-7 prepare the queries and
-// then run the softmax; 8 / 9 stream K / V blocks by TMA; 10 issues the MMAs,
-// S^T(b + 1) and O(b) as each is ready; 11 works out the visibility of blocks
-// that not every row sees whole and zeroes V rows that none does (0 * NaN).
-// The softmax's two warpgroups either take the key blocks in turn, with a
-// reference, l and O of their own (ALT: up to 80 columns, what their
-// registers hold of l), or half of the columns each.
+// other sequences in between are not read). Warps 0 / 1 stream K / V blocks by
+// TMA; 2 issues the MMAs, S^T(b + 1) and O(b) as each is ready; 3 fetches the
+// scale bytes, works out the visibility of blocks that not every row sees whole
+// and zeroes V rows that none does (0 * NaN). The other warps prepare the queries and then run the
+// softmax, as warpgroups of 128 threads = 128 keys. One warpgroup's block is a
+// long chain (two waits, TMEM loads, one barrier, 2^x, stores, a fence), so
+// several run side by side: CG of them share a block's columns, 16 CH each, and
+// A such sets take the blocks in turn, each with its own S^T and P' buffers,
+// references, l and O^T, joined at the end. What CH, CG and A are for N columns
+// follows from registers (l: 16 CH), TMEM (N (max(A, 2) + A) <= 512 columns)
+// and threads: see q8_shape.
 constexpr int kQ8Keys = 128;
 constexpr int kQ8MaxRows = 144;       // query rows per CTA: three ring stages fit next to their Q and P'
-constexpr int kQ8AltRows = 80;        // up to here the warpgroups take blocks in turn
-constexpr int kQ8Threads = 384;
 constexpr int kQ8MaxStages = 6;
-constexpr int kQ8MapWords = 256;      // bitmap of key blocks (units of 2^unit_shift blocks)
+constexpr int kQ8MapWords = 128;      // bitmap of key blocks (units of 2^unit_shift blocks)
+constexpr int kQ8Helpers = 128;       // threads of warps 0 .. 3
 constexpr float kQ8Bias = 3.f;
 constexpr float kQ8Grow = 5.75f;
 constexpr float kQ8Unset = 1e30f;     // reference of a row that saw no key yet: every t exceeds it
-constexpr uint32_t kQ8ColO = 2 * kQ8MaxRows;  // TMEM columns: two S^T buffers, then O^T (ALT: two of kQ8AltRows)
+constexpr int kQ8BarSoftmax = 8, kQ8BarHelpers = 9;  // named barriers (1 .. 5: the warpgroups')
+
+// Column chunks of 16 -> chunks per warpgroup, warpgroups that share a block,
+// sets of them that take blocks in turn.
+struct Q8Shape {
+  int ch, cg, sets;
+};
+static Q8Shape q8_shape(int chunks) {
+  if (chunks <= 2) return {chunks, 1, 4};
+  if (chunks <= 4) return {2, 2, 2};
+  if (chunks <= 8) return {2, (chunks + 1) / 2, 1};
+  return {3, 3, 1};
+}
 
 struct AttnQ8Maps {
   CUtensorMap k, v;  // [n_kv][max_slots][hd] bytes, box {hd, 128, 1}
@@ -353,24 +368,30 @@ struct AttnQ8Maps {
 
 struct AttnQ8Meta {
   float rowc[kQ8MaxRows];                      // 2^eq scale log2 e per query row
-  float bias_ref[8][kQ8AltRows];               // kBias - M of the columns of each softmax warp (four alike)
-  float wmax[2][4][kQ8AltRows];                // per warpgroup: column maxima of a warp's 32 keys
-  uint8_t shift[8][kQ8AltRows];                // per softmax warp: log2 of the last move of M (255: O and l restart)
   int len[kQ8MaxRows], start[kQ8MaxRows];      // per token
-  uint32_t vis[2][kQ8MaxRows][4];              // per block buffer and token: which of the block's keys it sees
   uint32_t map[kQ8MapWords];
   int max_start, min_len;                      // a block inside [max_start, min_len) is visible to every row
   int first, count;                            // this CTA's units of the bitmap
+  int ready;                                   // blocks whose scales and visibility are in place
+  int part[4];                                 // per block buffer: not every row sees the whole block
+  uint16_t scales[4][kQ8Keys];                 // per block buffer and key: K's scale byte, V's in the high half
   int abort;
-  uint32_t tmem;
+  uint32_t tmem, pad;
   uint64_t k_full[kQ8MaxStages], k_empty[kQ8MaxStages], v_full[kQ8MaxStages], v_clean[kQ8MaxStages],
       v_empty[kQ8MaxStages];
-  uint64_t s_full[2], s_free[2], p_full[2], p_free[2], vis_full[2], meta_ready, q_ready, o_full;
+  uint64_t s_full[4], s_free[4], p_full[4], p_free[4], meta_ready, q_ready, o_full, pad2;
 };
+static_assert(sizeof(AttnQ8Meta) % 16 == 0, "the arrays behind it are read 16 bytes at a time");
 
-__host__ __device__ constexpr int q8_p_bytes(int n) { return (n + 31) / 32 * 4096; }  // one term of one buffer
-__host__ __device__ constexpr int q8_fixed_smem(int hd, int n) {
-  return 1024 + 2 * n * hd + 4 * q8_p_bytes(n) + (int)sizeof(AttnQ8Meta);
+__host__ __device__ constexpr int q8_buffers(int sets) { return sets > 2 ? sets : 2; }  // of S^T and P'
+__host__ __device__ constexpr int q8_p_bytes(int n) { return (n + 31) / 32 * 4096; }    // one term of one buffer
+// Behind AttnQ8Meta: per softmax warp and column {kBias - M, the last move as
+// a bf16 factor}, per warpgroup {column maxima of each warp's 32 keys}, and per
+// block buffer and token the 128 bits of which of the block's keys it sees.
+static int q8_fixed_smem(int hd, int n, const Q8Shape& f) {
+  const int state = 4 * f.cg * f.sets * 16 * f.ch;
+  return 1024 + 2 * n * hd + q8_buffers(f.sets) * 2 * q8_p_bytes(n) + (int)sizeof(AttnQ8Meta) + state * 10 +
+         q8_buffers(f.sets) * n * 16;
 }
 
 // D[tmem] (+)= A[smem] * B[smem]^T, e4m3 in, fp32 accumulate.
@@ -477,7 +498,7 @@ struct Q8Blocks {
   }
 };
 
-// The CTA's tokens (by warps 8 .. 11): slot ranges, and the bitmap of key
+// The CTA's tokens (by warps 0 .. 3): slot ranges, and the bitmap of key
 // blocks that some row sees.
 __device__ __forceinline__ void q8_tokens(const AttnQ8Args& a, AttnQ8Meta& m, int t0, int ntok, int sb,
                                           int unit_shift) {
@@ -490,7 +511,7 @@ __device__ __forceinline__ void q8_tokens(const AttnQ8Args& a, AttnQ8Meta& m, in
       if ((m.map[w] & bits) != bits) atomicOr(&m.map[w], bits);
     }
   };
-  for (int i = threadIdx.x - 256; i < ntok; i += 128) {
+  for (int i = threadIdx.x; i < ntok; i += kQ8Helpers) {
     const int t = t0 + i;
     const int start = max(a.prefix_start ? a.prefix_start[t] : 0, 0);
     const int len = min(a.prefix_len[t], a.kv_end);
@@ -547,81 +568,84 @@ __device__ __forceinline__ void q8_slice(const AttnQ8Meta& m, int split, int n_s
 }
 
 // The CTA's query rows as two e4m3 terms per element, K-major rows of HD bytes
-// (by the eight softmax warps). A row is LPR lanes x 8 elements; a lane loads
-// all its rows before it converts the first.
-template <int HD, int ROWS>
+// (by the softmax warps). A row is LPR lanes x 8 elements; a lane loads a batch
+// of rows (all it has, in every shape) before it converts the first.
+template <int HD>
 __device__ __forceinline__ void q8_queries(const AttnQ8Args& a, AttnQ8Meta& m, uint8_t* q_hi, uint8_t* q_lo, int N,
                                            int nrows, int t0, int h) {
-  constexpr int LPR = HD / 8, RPP = 256 / LPR, BATCH = (ROWS + RPP - 1) / RPP;
+  constexpr int LPR = HD / 8, BATCH = 4;
+  const int rows_per_pass = (blockDim.x - kQ8Helpers) / LPR;
   const bf16* qb = static_cast<const bf16*>(a.q);
   const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0;
-  const int l8 = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
-  uint32_t raw[BATCH][4];
+  const int l8 = threadIdx.x % LPR, r0 = (threadIdx.x - kQ8Helpers) / LPR;
+  for (int rb = 0; rb < N; rb += rows_per_pass * BATCH) {
+    uint32_t raw[BATCH][4];
 #pragma unroll
-  for (int u = 0; u < BATCH; ++u) {
-    const int r = u * RPP + r0;
-    raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
-    if (r < nrows) {
-      const bf16* src = qb + (int64_t)(t0 + r / a.G) * a.ldq + (int64_t)(h * a.G + r % a.G) * HD + l8 * 8;
-      if (wide) {
-        const uint4 v = *reinterpret_cast<const uint4*>(src);
-        raw[u][0] = v.x, raw[u][1] = v.y, raw[u][2] = v.z, raw[u][3] = v.w;
-      } else {
-        const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
+    for (int u = 0; u < BATCH; ++u) {
+      const int r = rb + u * rows_per_pass + r0;
+      raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
+      if (r < nrows) {
+        const bf16* src = qb + (int64_t)(t0 + r / a.G) * a.ldq + (int64_t)(h * a.G + r % a.G) * HD + l8 * 8;
+        if (wide) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src);
+          raw[u][0] = v.x, raw[u][1] = v.y, raw[u][2] = v.z, raw[u][3] = v.w;
+        } else {
+          const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) raw[u][e] = s16[2 * e] | (static_cast<uint32_t>(s16[2 * e + 1]) << 16);
+          for (int e = 0; e < 4; ++e) raw[u][e] = s16[2 * e] | (static_cast<uint32_t>(s16[2 * e + 1]) << 16);
+        }
       }
     }
-  }
 #pragma unroll
-  for (int u = 0; u < BATCH; ++u) {
-    const int r = u * RPP + r0;
-    if (u * RPP >= N) break;  // uniform
-    float x[8], amax = 0.f;
+    for (int u = 0; u < BATCH; ++u) {
+      const int r = rb + u * rows_per_pass + r0;
+      if (rb + u * rows_per_pass >= N) break;  // uniform
+      float x[8], amax = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[2 * e] = __uint_as_float(raw[u][e] << 16);
-      x[2 * e + 1] = __uint_as_float(raw[u][e] & 0xffff0000u);
-    }
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(raw[u][e] << 16);
+        x[2 * e + 1] = __uint_as_float(raw[u][e] & 0xffff0000u);
+      }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {  // Inf and NaN become the row's amax: they compare above every finite value
-      const float v = fabsf(x[e]);
-      amax = v <= 3.402823466e38f ? fmaxf(amax, v) : INFINITY;
-    }
+      for (int e = 0; e < 8; ++e) {  // Inf and NaN become the row's amax: they compare above every finite value
+        const float v = fabsf(x[e]);
+        amax = v <= 3.402823466e38f ? fmaxf(amax, v) : INFINITY;
+      }
 #pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const bool fine = amax <= 3.402823466e38f;
-    const int byte = q8_scale_byte(fine ? amax : 0.f);
-    const float inv = q8_inv_scale(byte);
-    uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+      for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      const bool fine = amax <= 3.402823466e38f;
+      const int byte = q8_scale_byte(fine ? amax : 0.f);
+      const float inv = q8_inv_scale(byte);
+      uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
-      const uint32_t c = q8_pack2(y0, y1);
-      const float2 back = q8_unpack2(c);
-      hi[e >> 2] |= c << (8 * (e & 3));
-      lo[e >> 2] |= q8_pack2(y0 - back.x, y1 - back.y) << (8 * (e & 3));
-    }
-    if (r < N) {
-      const int sw = HD == 128 ? (r & 7) : ((r >> 1) & 3);  // swizzled place of the lane's 8 bytes
-      const int at = r * HD + (((l8 >> 1) ^ sw) << 4) + (l8 & 1) * 8;
-      *reinterpret_cast<uint2*>(q_hi + at) = make_uint2(hi[0], hi[1]);
-      *reinterpret_cast<uint2*>(q_lo + at) = make_uint2(lo[0], lo[1]);
-      if (l8 == 0) {
-        m.rowc[r] = fine ? q8_scale(byte) * (a.scale * 1.4426950408889634f) : __int_as_float(0x7fffffff);
+      for (int e = 0; e < 8; e += 2) {
+        const float y0 = x[e] * inv, y1 = x[e + 1] * inv;
+        const uint32_t c = q8_pack2(y0, y1);
+        const float2 back = q8_unpack2(c);
+        hi[e >> 2] |= c << (8 * (e & 3));
+        lo[e >> 2] |= q8_pack2(y0 - back.x, y1 - back.y) << (8 * (e & 3));
+      }
+      if (r < N) {
+        const int sw = HD == 128 ? (r & 7) : ((r >> 1) & 3);  // swizzled place of the lane's 8 bytes
+        const int at = r * HD + (((l8 >> 1) ^ sw) << 4) + (l8 & 1) * 8;
+        *reinterpret_cast<uint2*>(q_hi + at) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(q_lo + at) = make_uint2(lo[0], lo[1]);
+        if (l8 == 0) {
+          m.rowc[r] = fine ? q8_scale(byte) * (a.scale * 1.4426950408889634f) : __int_as_float(0x7fffffff);
+        }
       }
     }
-  }
+}
 }
 
 // Visibility of the 16 columns from `col` for the thread's key (bit j = column
 // col + j), from the block's per-token key masks.
-__device__ __forceinline__ uint32_t q8_chunk_vis(const AttnQ8Meta& m, int buf, int col, int G, int ntok, int quarter,
+__device__ __forceinline__ uint32_t q8_chunk_vis(const uint32_t* vis_buf, int col, int G, int ntok, int quarter,
                                                  int lane) {
   uint32_t vis = 0u;
   const int last = min((col + 15) / G, ntok - 1);
   for (int t = col / G; t <= last; ++t)
-    if ((m.vis[buf][t][quarter] >> lane) & 1u) {
+    if ((vis_buf[t * 4 + quarter] >> lane) & 1u) {
       const int lo = max(t * G - col, 0), hi = min((t + 1) * G - col, 16);
       vis |= ((1u << hi) - 1u) & ~((1u << lo) - 1u);
     }
@@ -644,12 +668,6 @@ __device__ __forceinline__ float q8_columns_reduce(float* v, int lane) {
   }
   const float got = __shfl_xor_sync(0xffffffffu, v[0], 16);
   return MAX ? fmaxf(v[0], got) : v[0] + got;
-}
-
-// The last move of M, as a factor of O and l.
-__device__ __forceinline__ float q8_shift_factor(uint32_t bytes, int i) {
-  const uint32_t k = (bytes >> (8 * i)) & 0xffu;
-  return k > 126u ? 0.f : __uint_as_float((127u - k) << 23);
 }
 
 // TMEM load without its wait; the wait takes the registers along so that
@@ -685,30 +703,49 @@ __device__ __forceinline__ void q8_scores(const float* rowc, float* x, uint64_t 
     for (int j = 0; j < 16; ++j) x[j] = (vis >> j) & 1u ? x[j] : -INFINITY;
   }
 }
+// A counter in shared memory that one warp raises and others wait for.
+__device__ __forceinline__ void st_release_cta(int* p, int v) {
+  asm volatile("st.release.cta.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
+__device__ __forceinline__ bool wait_above(int* p, int v) {
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    int x;
+    asm volatile("ld.acquire.cta.shared::cta.b32 %0, [%1];" : "=r"(x) : "r"(smem_u32(p)) : "memory");
+    if (x > v) return true;
+  }
+  return false;
+}
 __device__ __forceinline__ float q8_warp_max(float v) {  // NaN gives way to numbers, as in fmaxf
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 
-template <int HD, int CH, bool ALT>
-__global__ void __launch_bounds__(kQ8Threads, 1)
-    attn_q8_tc_kernel(const __grid_constant__ AttnQ8Maps maps, const AttnQ8Args a, const int n_chunks,
+template <int HD, int CH, int A>
+__global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
+    attn_q8_tc_kernel(const __grid_constant__ AttnQ8Maps maps, const AttnQ8Args a, const int n_chunks, const int cgs,
                       const int tok_per_group, const int stages, const int unit_shift) {
   constexpr int TILE = kQ8Keys * HD;              // bytes of a K or V block
   constexpr uint32_t SW = HD == 128 ? 2u : 4u;    // 128-byte or 64-byte swizzle: one atom row per cache row
   constexpr uint32_t SBO = 8 * HD;                // 8 rows of HD bytes
-  constexpr int KEEP = CH <= 3 ? CH : 1;          // chunks whose exponents fit the registers next to l
+  constexpr int BUFS = q8_buffers(A);             // a power of two
+  constexpr int BSH = BUFS == 4 ? 2 : 1;
+  constexpr int WC = 16 * CH;                     // columns of a warpgroup
   extern __shared__ uint8_t q8_smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(q8_smem_raw) + 1023) & ~uintptr_t(1023));
   const int N = 16 * n_chunks;
   const int p_bytes = q8_p_bytes(N), atoms = (N + 31) / 32;
+  const int wgs = cgs * A;
   uint8_t* k_ring = sm;
   uint8_t* v_ring = k_ring + stages * TILE;
-  uint8_t* p_buf = v_ring + stages * TILE;        // [2 buffers][hi, lo][keys / 8][atoms][8 keys x 32 rows]
-  uint8_t* q_hi = p_buf + 4 * p_bytes;            // [N][HD]
+  uint8_t* p_buf = v_ring + stages * TILE;        // [BUFS][hi, lo][keys / 8][atoms][8 keys x 32 rows]
+  uint8_t* q_hi = p_buf + BUFS * 2 * p_bytes;     // [N][HD]
   uint8_t* q_lo = q_hi + N * HD;
   AttnQ8Meta& m = *reinterpret_cast<AttnQ8Meta*>(q_lo + N * HD);
+  float* refs = reinterpret_cast<float*>(&m + 1);                            // [softmax warps][WC]
+  float* wmax = refs + 4 * wgs * WC;                                         // [warpgroups][4][WC]
+  uint32_t* vis = reinterpret_cast<uint32_t*>(wmax + 4 * wgs * WC);          // [BUFS][N tokens][4]
+  uint16_t* factors = reinterpret_cast<uint16_t*>(vis + BUFS * N * 4);       // [softmax warps][WC]
   volatile int* abort_flag = &m.abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -717,12 +754,11 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
   const int t0 = group * tok_per_group;
   const int ntok = min(tok_per_group, a.T - t0);
   const int nrows = ntok * a.G;
-  const bool two = ALT || n_chunks > CH;          // both warpgroups have columns
-  const uint32_t per_buffer = !ALT && two ? 8 : 4;  // softmax warps that work on one block
 
   if (threadIdx.x == 0) {
     m.max_start = 0;
     m.min_len = INT32_MAX;
+    m.ready = 0;
     m.abort = 0;
     for (int i = 0; i < stages; ++i) {
       mbar_init(&m.k_full[i], 1);
@@ -731,31 +767,30 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       mbar_init(&m.v_clean[i], 1);
       mbar_init(&m.v_empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < BUFS; ++i) {
       mbar_init(&m.s_full[i], 1);
-      mbar_init(&m.s_free[i], per_buffer);
-      mbar_init(&m.p_full[i], per_buffer);
+      mbar_init(&m.s_free[i], 4 * cgs);
+      mbar_init(&m.p_full[i], 4 * cgs);
       mbar_init(&m.p_free[i], 1);
-      mbar_init(&m.vis_full[i], 1);
     }
     mbar_init(&m.meta_ready, 1);
-    mbar_init(&m.q_ready, 8);
+    mbar_init(&m.q_ready, 4 * wgs);
     mbar_init(&m.o_full, 1);
     fence_mbar_init();
   }
-  for (int i = threadIdx.x; i < kQ8MapWords; i += kQ8Threads) m.map[i] = 0u;
-  if (warp == 10) {
+  if (threadIdx.x < kQ8MapWords) m.map[threadIdx.x] = 0u;
+  if (warp == 2) {
     tmem_alloc(&m.tmem, 512);
     tmem_relinquish();
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.v);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = m.tmem;
+  const uint32_t tmem = m.tmem, tmem_o = tmem + BUFS * N;  // BUFS S^T buffers, then A O^T, N columns each
   pdl_wait();
   pdl_trigger();
   const uint32_t p_s = smem_u32(p_buf);
@@ -764,24 +799,24 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
     *abort_flag = 1;
   };
 
-  if (warp >= 8) {
+  if (warp < 4) {
     const int sb = a.mask ? a.spec_base[0] : 0;
     q8_tokens(a, m, t0, ntok, sb, unit_shift);
     __syncwarp();
-    named_bar_sync(4, 128);
+    named_bar_sync(kQ8BarHelpers, kQ8Helpers);
     int first, count;
     q8_slice(m, split, a.n_splits, first, count);
     const int nblocks = count << unit_shift;
     const int max_start = m.max_start, min_len = m.min_len;
-    if (warp == 11 && lane == 0) {
+    if (warp == 3 && lane == 0) {
       m.first = first;
       m.count = count;
       mbar_arrive(&m.meta_ready);
     }
     Q8Blocks it(m.map, first, count, unit_shift);
-    if (warp == 8 || warp == 9) {
+    if (warp < 2) {
       if (lane == 0) {
-        const bool is_v = warp == 9;
+        const bool is_v = warp == 1;
         uint64_t* full = is_v ? m.v_full : m.k_full;
         uint64_t* empty = is_v ? m.v_empty : m.k_empty;
         uint8_t* ring = is_v ? v_ring : k_ring;
@@ -802,7 +837,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
         if (*abort_flag)  // copies in flight land before the CTA leaves
           for (int b = max(issued - stages, 0); b < issued; ++b) (void)mbar_wait(&full[b % stages], (b / stages) & 1);
       }
-    } else if (warp == 10) {
+    } else if (warp == 2) {
       // The whole warp runs the loop (its addresses stay uniform), one lane
       // issues. Descriptors of later parts of an operand add to the low word.
       const bool leader = elect_one();
@@ -819,18 +854,18 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
         while (ready && nP < nblocks) {
           bool prog = false;
           bool go = nS < nblocks && mbar_test(&m.k_full[sS], phS) &&
-                    (nS < 2 || mbar_test(&m.s_free[nS & 1], ((nS >> 1) - 1) & 1));
+                    (nS < BUFS || mbar_test(&m.s_free[nS & (BUFS - 1)], ((nS >> BSH) - 1) & 1));
           if (__all_sync(0xffffffffu, go)) {
             tc_fence_after();
             if (leader) {
-              const uint32_t d = tmem + (nS & 1) * kQ8MaxRows, k = k_lo + sS * (TILE >> 4);
+              const uint32_t d = tmem + (nS & (BUFS - 1)) * N, k = k_lo + sS * (TILE >> 4);
 #pragma unroll
               for (int ks = 0; ks < HD / 32; ++ks)
                 umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(qh_lo + ks * 2, rows_hi), id_s, ks > 0);
 #pragma unroll
               for (int ks = 0; ks < HD / 32; ++ks)
                 umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(ql_lo + ks * 2, rows_hi), id_s, 1u);
-              umma_commit(&m.s_full[nS & 1]);
+              umma_commit(&m.s_full[nS & (BUFS - 1)]);
               umma_commit(&m.k_empty[sS]);
             }
             __syncwarp();
@@ -838,22 +873,22 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
             if (++sS == stages) sS = 0, phS ^= 1u;
             prog = true;
           }
-          go = nP < nS && mbar_test(&m.p_full[nP & 1], (nP >> 1) & 1) && mbar_test(&m.v_clean[sP], phP);
+          go = nP < nS && mbar_test(&m.p_full[nP & (BUFS - 1)], (nP >> BSH) & 1) && mbar_test(&m.v_clean[sP], phP);
           if (__all_sync(0xffffffffu, go)) {
             tc_fence_after();
             if (leader) {
               // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
               // M = 128 repeats the first (lanes 64 .. 127 are not read). P': MN-major, atoms of 32 rows x 8 keys.
-              const uint32_t d = tmem + kQ8ColO + (ALT ? (nP & 1) * kQ8AltRows : 0);
-              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + (nP & 1) * (2 * p_bytes >> 4);
+              const uint32_t d = tmem_o + (nP & (A - 1)) * N;
+              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + (nP & (BUFS - 1)) * (2 * p_bytes >> 4);
 #pragma unroll
               for (int term = 0; term < 2; ++term)
 #pragma unroll
                 for (int kk = 0; kk < kQ8Keys / 32; ++kk)
                   umma_f8(d, q8_desc(v + kk * 2 * HD, rows_hi),
                           q8_desc(pl + term * (p_bytes >> 4) + kk * (atoms * 64), p_hi), id_o,
-                          (nP >= (ALT ? 2 : 1) || term > 0 || kk > 0) ? 1u : 0u);
-              umma_commit(&m.p_free[nP & 1]);
+                          (nP >= A || term > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&m.p_free[nP & (BUFS - 1)]);
               umma_commit(&m.v_empty[sP]);
             }
             __syncwarp();
@@ -870,14 +905,32 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       }
       if (leader) umma_commit(&m.o_full);
     } else {
-      // Blocks that not every row sees whole: the keys that each token sees,
-      // for the softmax warps, and zeros in the V rows that none does.
+      // Scale bytes of every block (loaded one block ahead); for blocks that not
+      // every row sees whole, the keys that each token sees, for the softmax
+      // warps, and zeros in the V rows that none does.
+      const uint8_t* ksc = a.ks + (int64_t)h * a.scale_head_stride;
+      const uint8_t* vsc = a.vs + (int64_t)h * a.scale_head_stride;
+      uint32_t bytes[4] = {0u, 0u, 0u, 0u};
+      int next_kb = 0;
+      auto fetch = [&] {
+        next_kb = it.next();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int slot = next_kb + i * 32 + lane;
+          bytes[i] = slot < a.kv_end ? ksc[slot] | (static_cast<uint32_t>(vsc[slot]) << 8) : 0u;
+        }
+      };
+      if (nblocks > 0) fetch();
       int st = 0;
       uint32_t phase = 0;
       for (int b = 0; b < nblocks; ++b) {
-        const int kb = it.next();
+        const int kb = next_kb, buf = b & (BUFS - 1);
         const bool part = kb < max_start || kb + kQ8Keys > min_len;
-        bool bad = b >= 2 && !mbar_wait(&m.s_free[b & 1], ((b >> 1) - 1) & 1);  // vis[b & 1] was read for b - 2
+        bool bad = b >= BUFS && !mbar_wait(&m.s_free[buf], ((b >> BSH) - 1) & 1);  // block b - BUFS is done with them
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m.scales[buf][i * 32 + lane] = static_cast<uint16_t>(bytes[i]);
+        if (b + 1 < nblocks) fetch();
+        if (lane == 0) m.part[buf] = part;
         uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
         if (part) {
           seen[0] = seen[1] = seen[2] = seen[3] = 0u;
@@ -886,15 +939,16 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const uint64_t v = q8_seen_bits(kb + 64 * half, m.start[i], m.len[i], mask, a.mask_words, sb, a.kv_end);
-              m.vis[b & 1][i][2 * half] = static_cast<uint32_t>(v);
-              m.vis[b & 1][i][2 * half + 1] = static_cast<uint32_t>(v >> 32);
+              vis[(buf * N + i) * 4 + 2 * half] = static_cast<uint32_t>(v);
+              vis[(buf * N + i) * 4 + 2 * half + 1] = static_cast<uint32_t>(v >> 32);
               seen[2 * half] |= static_cast<uint32_t>(v);
               seen[2 * half + 1] |= static_cast<uint32_t>(v >> 32);
             }
           }
         }
+        __threadfence_block();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&m.vis_full[b & 1]);
+        if (lane == 0) st_release_cta(&m.ready, b + 1);
         bad = bad || !mbar_wait(&m.v_full[st], phase);
         if (__any_sync(0xffffffffu, bad || *abort_flag)) {
           if (lane == 0) give_up();
@@ -920,125 +974,105 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
     }
   } else {
     // ---- softmax warps: the queries, then thread = key
-    const int wg = warp >> 2, quarter = warp & 3;
-    const int my_chunks = ALT ? n_chunks : wg == 0 ? CH : n_chunks - CH;
-    const int col_base = ALT || wg == 0 ? 0 : 16 * CH;
-    float* const my_ref = m.bias_ref[warp];
+    const int sw = warp - 4, wg = sw >> 2, quarter = warp & 3;
+    const int cg = wg % cgs, turn = wg / cgs;     // columns [WC cg, ..), blocks turn, turn + A, ..
+    const int my_chunks = min(CH, n_chunks - cg * CH);
+    const int col_base = cg * WC;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t to = tmem + kQ8ColO + (ALT ? wg * kQ8AltRows : 0) + lane_base + col_base;
+    const uint32_t to = tmem_o + turn * N + lane_base + col_base;
     const int key = quarter * 32 + lane;
-    const uint8_t* ksc = a.ks + (int64_t)h * a.scale_head_stride;
-    const uint8_t* vsc = a.vs + (int64_t)h * a.scale_head_stride;
-    const uint32_t p_at = (key >> 3) * atoms * 256 + (key & 7) * 32;
+    float* const my_ref = refs + sw * WC;
+    float* const my_max = wmax + (wg * 4 + quarter) * WC;
+    const float* const all_max = wmax + wg * 4 * WC;
+    uint16_t* const my_fac = factors + sw * WC;
+    const uint32_t p_at = p_s + (key >> 3) * atoms * 256 + (key & 7) * 32;
     const uint32_t p_flip = (key >> 2) & 1;
-    const uint64_t minus1 = f2_pack(-1.f, -1.f);
-    q8_queries<HD, ALT ? 16 * CH : 32 * CH>(a, m, q_hi, q_lo, N, nrows, t0, h);
-    for (int i = lane; i < 16 * CH; i += 32)  // columns past the rows: P' = 0
+    q8_queries<HD>(a, m, q_hi, q_lo, N, nrows, t0, h);
+    for (int i = lane; i < WC; i += 32)  // columns past the rows: P' = 0
       my_ref[i] = col_base + i < nrows ? kQ8Unset : -kQ8Unset;
     fence_proxy_async_smem();
     __syncwarp();
-    named_bar_sync(3, 256);  // the rows' scales are read by other warps than wrote them
+    named_bar_sync(kQ8BarSoftmax, 128 * wgs);  // the rows' scales are read by other warps than wrote them
     if (lane == 0) mbar_arrive(&m.q_ready);
     bool bad = !mbar_wait(&m.meta_ready, 0);
     if (bad) give_up();
-    const int count = bad ? 0 : m.count;
-    const int nblocks = count << unit_shift;
-    const int max_start = m.max_start, min_len = m.min_len;
-    Q8Blocks it(m.map, bad ? 0 : m.first, count, unit_shift);
-    constexpr int STEP = ALT ? 2 : 1;
-    const int b0 = ALT ? wg : 0;
-    int kb = 0, kbyte = 0, vbyte = 0;
-    auto fetch = [&](int b) {  // block b's slot and the key's scale bytes
-      if (b >= nblocks || my_chunks == 0) return;
-      if (ALT && b > 0) (void)it.next();  // the other warpgroup's
-      kb = it.next();
-      const bool in = kb + key < a.kv_end;
-      kbyte = in ? ksc[kb + key] : 0;
-      vbyte = in ? vsc[kb + key] : 0;
-    };
-    fetch(b0);
-    float l[16 * CH];
+    const int nblocks = bad ? 0 : m.count << unit_shift;
+    float l[WC];
 #pragma unroll
-    for (int i = 0; i < 16 * CH; ++i) l[i] = 0.f;
-    for (int b = b0; b < (my_chunks > 0 ? nblocks : 0); b += STEP) {
-      const int buf = b & 1;
-      const bool part = kb < max_start || kb + kQ8Keys > min_len;
-      const float ck = q8_scale(kbyte);
-      const int vb = max(vbyte, kQ8MinScale);
-      const float ev = static_cast<float>(vb - 127);
-      const float inv_v = q8_inv_scale(vb);
-      const uint64_t ck2 = f2_pack(ck, ck), ev2 = f2_pack(ev, ev), iv2 = f2_pack(inv_v, inv_v);
-      fetch(b + STEP);
+    for (int i = 0; i < WC; ++i) l[i] = 0.f;
+    for (int b = turn; b < nblocks; b += A) {
+      const int buf = b & (BUFS - 1);
+      const uint32_t use = (b >> BSH) & 1;        // parity of the buffer's use by block b
       // After a timeout the loop runs on without waiting: the warpgroup's barriers stay matched.
-      if (!bad && (*abort_flag || !mbar_wait(&m.s_full[buf], (b >> 1) & 1))) {
+      if (!bad && !(wait_above(&m.ready, b) && mbar_wait(&m.s_full[buf], use))) {
         bad = true;
         give_up();
       }
-      // (every block: the barrier's parity tells one phase from the next, not from the one after)
-      if (!bad && !mbar_wait(&m.vis_full[buf], (b >> 1) & 1)) {
-        bad = true;
-        give_up();
-      }
+      const bool part = m.part[buf];
+      const uint32_t bytes = m.scales[buf][key];
+      const float ck = q8_scale(bytes & 0xffu);
+      const int vb = max(static_cast<int>(bytes >> 8), kQ8MinScale);
+      const float ev = static_cast<float>(vb - 127), inv_v = q8_inv_scale(vb);
+      const uint64_t ck2 = f2_pack(ck, ck), ev2 = f2_pack(ev, ev), iv2 = f2_pack(inv_v, inv_v);
       tc_fence_after();
-      const uint32_t ts = tmem + buf * kQ8MaxRows + lane_base + col_base;
-      const uint32_t pb = p_s + buf * 2 * p_bytes + p_at;
-      // t of every column and its maximum over the warp's keys. With up to KEEP
-      // chunks t stays in registers, with more it is computed again below.
-      float x[16 * KEEP];
-      if (CH <= KEEP) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-          if (c < my_chunks) q8_tmem_ld16(ts + c * 16, x + 16 * (c % KEEP));
-      }
-      // (halves: s_full(b) does not say that the other warps have read the last block's maxima)
-      if (!ALT) named_bar_sync(1 + wg, 128);
+      const uint32_t ts = tmem + buf * N + lane_base + col_base;
+      const uint32_t* vis_buf = vis + buf * N * 4;
+      // t of every column and its maximum over the warp's keys; t is computed
+      // again below rather than held in registers.
+      // (A == 1: s_full(b) does not say that the other warps have read the last block's maxima)
+      if (A == 1) named_bar_sync(1 + wg, 128);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
-          float* xc = x + 16 * (c % KEEP);
-          const uint32_t vis = part ? q8_chunk_vis(m, buf, col_base + c * 16, a.G, ntok, quarter, lane) : 0xffffu;
-          if (CH > KEEP) q8_tmem_ld16(ts + c * 16, xc);
-          q8_tmem_wait16(xc);
-          q8_scores(m.rowc + col_base + c * 16, xc, ck2, ev2, part, vis);
+          const uint32_t see = part ? q8_chunk_vis(vis_buf, col_base + c * 16, a.G, ntok, quarter, lane) : 0xffffu;
+          float x[16];
+          q8_tmem_ld16(ts + c * 16, x);
+          q8_tmem_wait16(x);
+          q8_scores(m.rowc + col_base + c * 16, x, ck2, ev2, part, see);
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
-            const float4 top = make_float4(q8_warp_max(xc[j]), q8_warp_max(xc[j + 1]), q8_warp_max(xc[j + 2]),
-                                           q8_warp_max(xc[j + 3]));
-            if (lane == 0) *reinterpret_cast<float4*>(&m.wmax[wg][quarter][c * 16 + j]) = top;
+            const float4 top = make_float4(q8_warp_max(x[j]), q8_warp_max(x[j + 1]), q8_warp_max(x[j + 2]),
+                                           q8_warp_max(x[j + 3]));
+            if (lane == 0) *reinterpret_cast<float4*>(my_max + c * 16 + j) = top;
           }
         }
       }
       __syncwarp();
       named_bar_sync(1 + wg, 128);
-      // lane i: columns i, i + 32, ... (each warp for itself, all alike)
-      float now[(16 * CH + 31) / 32];
-      uint32_t by[(16 * CH + 31) / 32];
+      // lane i: columns i, i + 32 (each warp for itself, all alike)
+      constexpr int PER = (WC + 31) / 32;
+      float now[PER], factor[PER];
       bool moves = false;
 #pragma unroll
-      for (int k = 0; k < (16 * CH + 31) / 32; ++k) {
+      for (int k = 0; k < PER; ++k) {
         const int i = lane + 32 * k;
-        by[k] = 0u;
+        factor[k] = 1.f;
+        now[k] = 0.f;
         if (i < 16 * my_chunks) {
-          const float mx = fmaxf(fmaxf(m.wmax[wg][0][i], m.wmax[wg][1][i]), fmaxf(m.wmax[wg][2][i], m.wmax[wg][3][i]));
+          const float mx = fmaxf(fmaxf(all_max[i], all_max[WC + i]), fmaxf(all_max[2 * WC + i], all_max[3 * WC + i]));
           const float old = my_ref[i];
-          now[k] = kQ8Bias - ceilf(mx);
-          if (mx + old > kQ8Bias + kQ8Grow) by[k] = old == kQ8Unset ? 255u : static_cast<uint32_t>(fminf(old - now[k], 255.f));
-          moves = moves || by[k];
+          now[k] = old;
+          if (mx + old > kQ8Bias + kQ8Grow) {
+            now[k] = kQ8Bias - ceilf(mx);
+            const float by = old - now[k];  // a whole number
+            factor[k] = old == kQ8Unset || by > 126.f ? 0.f : __uint_as_float((127u - static_cast<uint32_t>(by)) << 23);
+            moves = true;
+          }
         }
       }
       if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
-        for (int k = 0; k < (16 * CH + 31) / 32; ++k) {
+        for (int k = 0; k < PER; ++k) {
           const int i = lane + 32 * k;
           if (i < 16 * my_chunks) {
-            if (by[k]) my_ref[i] = now[k];
-            m.shift[warp][i] = static_cast<uint8_t>(by[k]);
+            my_ref[i] = now[k];
+            my_fac[i] = static_cast<uint16_t>(__float_as_uint(factor[k]) >> 16);  // a power of two or 0: exact
           }
         }
         __syncwarp();
-        const bool has_o = b >= (ALT ? 2 : 1);
-        // the last P V into this O: block b - 2 of this warpgroup, or block b - 1
-        if (has_o && !bad && !mbar_wait(&m.p_free[ALT ? buf : buf ^ 1], (ALT ? (b >> 1) - 1 : (b - 1) >> 1) & 1)) {
+        const bool has_o = b >= A;
+        // the last P V into this O is block b - A's
+        if (has_o && !bad && !mbar_wait(&m.p_free[(b - A) & (BUFS - 1)], ((b - A) >> BSH) & 1)) {
           bad = true;
           give_up();
         }
@@ -1046,43 +1080,39 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           if (c < my_chunks) {
-            const uint4 sh = *reinterpret_cast<const uint4*>(&m.shift[warp][c * 16]);
-            if (sh.x | sh.y | sh.z | sh.w) {
-              const uint32_t w[4] = {sh.x, sh.y, sh.z, sh.w};
-              float o[16];
-              if (has_o) tmem_ld16(to + c * 16, o);
+            const uint4 f0 = *reinterpret_cast<const uint4*>(my_fac + c * 16);
+            const uint4 f1 = *reinterpret_cast<const uint4*>(my_fac + c * 16 + 8);
+            const uint32_t w[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+            float o[16];
+            if (has_o) tmem_ld16(to + c * 16, o);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float f = q8_shift_factor(w[j >> 2], j & 3);
-                l[c * 16 + j] *= f;
-                o[j] = has_o && f != 0.f ? o[j] * f : 0.f;
+            for (int j = 0; j < 8; ++j) {
+              const float f[2] = {__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)};
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                l[c * 16 + 2 * j + e] *= f[e];
+                if (has_o) o[2 * j + e] *= f[e];
               }
-              if (has_o) tmem_st16(to + c * 16, o);
             }
+            if (has_o) tmem_st16(to + c * 16, o);
           }
         }
         tmem_wait_st();
       }
-      if (CH <= KEEP) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m.s_free[buf]);
-      }
-      if (b >= 2 && !bad && !mbar_wait(&m.p_free[buf], ((b >> 1) - 1) & 1)) {  // P V of block b - 2 read this buffer
+      if (b >= BUFS && !bad && !mbar_wait(&m.p_free[buf], use ^ 1u)) {  // P V of block b - BUFS read this buffer
         bad = true;
         give_up();
       }
+      const uint32_t pb = p_at + buf * 2 * p_bytes;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
           const int col = col_base + c * 16;
-          float* xc = x + 16 * (c % KEEP);
-          if (CH > KEEP) {
-            const uint32_t vis = part ? q8_chunk_vis(m, buf, col, a.G, ntok, quarter, lane) : 0xffffu;
-            q8_tmem_ld16(ts + c * 16, xc);
-            q8_tmem_wait16(xc);
-            q8_scores(m.rowc + col, xc, ck2, ev2, part, vis);
-          }
+          const uint32_t see = part ? q8_chunk_vis(vis_buf, col, a.G, ntok, quarter, lane) : 0xffffu;
+          float x[16];
+          q8_tmem_ld16(ts + c * 16, x);
+          q8_tmem_wait16(x);
+          q8_scores(m.rowc + col, x, ck2, ev2, part, see);
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -1091,16 +1121,15 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
             float t4[4], r4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              xc[4 * j + e] = q8_ex2(xc[4 * j + e] + r[e]);
-              t4[e] = __uint_as_float(__float_as_uint(xc[4 * j + e]) & 0xfff00000u);  // 4 significant bits
+              x[4 * j + e] = q8_ex2(x[4 * j + e] + r[e]);
+              t4[e] = __uint_as_float(__float_as_uint(x[4 * j + e]) & 0xfff00000u);  // 4 significant bits
+              r4[e] = x[4 * j + e] - t4[e];
             }
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const uint64_t p2 = f2_pack(xc[4 * j + e], xc[4 * j + e + 1]);
-              f2_unpack(f2_fma(f2_pack(t4[e], t4[e + 1]), minus1, p2), r4[e], r4[e + 1]);
-              f2_unpack(f2_fma(p2, iv2, f2_pack(l[c * 16 + 4 * j + e], l[c * 16 + 4 * j + e + 1])),
+            for (int e = 0; e < 4; e += 2)
+              f2_unpack(f2_fma(f2_pack(x[4 * j + e], x[4 * j + e + 1]), iv2,
+                               f2_pack(l[c * 16 + 4 * j + e], l[c * 16 + 4 * j + e + 1])),
                         l[c * 16 + 4 * j + e], l[c * 16 + 4 * j + e + 1]);
-            }
             hi[j] = q8_pack4(t4[0], t4[1], t4[2], t4[3]);
             lo[j] = q8_pack4(r4[0], r4[1], r4[2], r4[3]);
           }
@@ -1117,91 +1146,86 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if (CH > KEEP) mbar_arrive(&m.s_free[buf]);
+        mbar_arrive(&m.s_free[buf]);
         mbar_arrive(&m.p_full[buf]);
       }
     }
     // ---- results: l summed over the 128 keys' threads, O^T read back (lane = head dim)
-    if (two || wg == 0) {
-      const int parties = two ? 256 : 128;
-      if (!mbar_wait(&m.o_full, 0)) give_up();
-      tc_fence_after();
-      __syncwarp();
-      named_bar_sync(3, parties);
-      float* s_l = reinterpret_cast<float*>(p_buf);  // [ALT: 2][4][N]: the P buffers are free once every MMA retired
-      float* s_f = s_l + 8 * N;                       // [2][N] factors of the O accumulators
+    const int parties = 128 * wgs;
+    if (!mbar_wait(&m.o_full, 0)) give_up();
+    tc_fence_after();
+    __syncwarp();
+    named_bar_sync(kQ8BarSoftmax, parties);
+    float* s_l = reinterpret_cast<float*>(p_buf);  // [softmax warps][WC]: the P buffers are free once every MMA retired
+    float* s_f = s_l + 4 * wgs * WC;                // [A][N] factors of the O accumulators
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (c < my_chunks) {
-          const float sum = q8_columns_reduce<false>(l + c * 16, lane);
-          if (lane < 16) s_l[((ALT ? wg * 4 : 0) + quarter) * N + col_base + c * 16 + lane] = sum;
-        }
+    for (int c = 0; c < CH; ++c) {
+      const float sum = q8_columns_reduce<false>(l + c * 16, lane);
+      if (lane < 16) s_l[sw * WC + c * 16 + lane] = sum;
+    }
+    __syncwarp();
+    named_bar_sync(kQ8BarSoftmax, parties);
+    // thread i: row i's factors, and the record {M, l} of a slice
+    const int64_t rec0 = ((int64_t)blockIdx.x * a.n_splits + split) * kQ8MaxRows;
+    const int i = threadIdx.x - kQ8Helpers;
+    if (i < N) {
+      const int g = i / WC, c = i - g * WC;
+      float ls[A], ms[A], top = -kQ8Unset, sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < A; ++u) {  // join the sets' shares of the slice
+        const float* pl = s_l + (u * cgs + g) * 4 * WC + c;
+        ls[u] = (pl[0] + pl[WC]) + (pl[2 * WC] + pl[3 * WC]);
+        ms[u] = kQ8Bias - refs[(u * cgs + g) * 4 * WC + c];
+        if (ls[u] != 0.f) top = fmaxf(top, ms[u]);
       }
-      __syncwarp();
-      named_bar_sync(3, parties);
-      // thread i: row i's factors, and the record {M, l} of a slice
-      const int64_t rec0 = ((int64_t)blockIdx.x * a.n_splits + split) * kQ8MaxRows;
-      const int i = threadIdx.x;
-      if (i < N) {
-        float sum = (s_l[i] + s_l[N + i]) + (s_l[2 * N + i] + s_l[3 * N + i]), f0 = 1.f, f1 = 0.f;
-        const float* refs = ALT || i < 16 * CH ? m.bias_ref[0] + i : m.bias_ref[4] + (i - 16 * CH);
-        float ref = kQ8Bias - *refs;
-        if (ALT) {  // join the warpgroups' halves of the slice
-          const float* s1 = s_l + 4 * N;
-          const float other = (s1[i] + s1[N + i]) + (s1[2 * N + i] + s1[3 * N + i]);
-          const float ref1 = kQ8Bias - m.bias_ref[4][i];
-          const float top = other == 0.f ? ref : sum == 0.f ? ref1 : fmaxf(ref, ref1);
-          f0 = sum == 0.f ? 0.f : exp2f(ref - top);
-          f1 = other == 0.f ? 0.f : exp2f(ref1 - top);
-          sum = fmaf(f0, sum, f1 * other);
-          ref = top;
-        }
-        if (a.n_splits > 1) {
-          if (i < nrows) {
-            float* ml = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD + (rec0 + i) * 2;
-            *reinterpret_cast<float2*>(ml) = make_float2(ref, sum);
-          }
-        } else {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          f0 *= inv;
-          f1 *= inv;
-        }
-        s_f[i] = nblocks > 0 ? f0 : 0.f;  // (an O that no block wrote is not read)
-        s_f[N + i] = ALT && nblocks > 1 ? f1 : 0.f;
+#pragma unroll
+      for (int u = 0; u < A; ++u) {
+        ms[u] = ls[u] == 0.f ? 0.f : exp2f(ms[u] - top);
+        sum = fmaf(ls[u], ms[u], sum);
       }
-      __syncwarp();
-      named_bar_sync(3, parties);
-      const int d = quarter * 32 + lane;
-      if (quarter * 32 < HD) {
-        const uint32_t o0 = tmem + kQ8ColO + lane_base;
+      float scale = 1.f;
+      if (a.n_splits > 1) {
+        if (i < nrows) {
+          float* ml = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD + (rec0 + i) * 2;
+          *reinterpret_cast<float2*>(ml) = make_float2(top, sum);
+        }
+      } else {
+        scale = sum == 0.f ? 0.f : 1.f / sum;
+      }
+#pragma unroll
+      for (int u = 0; u < A; ++u) s_f[u * N + i] = nblocks > u ? ms[u] * scale : 0.f;  // (O without a block: not read)
+    }
+    __syncwarp();
+    named_bar_sync(kQ8BarSoftmax, parties);
+    const int d = quarter * 32 + lane;
+    if (quarter * 32 < HD) {
 #pragma unroll 1
-        for (int c = ALT ? wg : col_base / 16; c < (ALT ? n_chunks : col_base / 16 + my_chunks); c += STEP) {
-          const int col = c * 16;
-          float o[16], u[16];
-          tmem_ld16(o0 + col, o);
-          if (ALT) tmem_ld16(o0 + kQ8AltRows + col, u);
+      for (int c = wg; c < n_chunks; c += wgs) {
+        const int col = c * 16;
+        float o[16];
+#pragma unroll
+        for (int u = 0; u < A; ++u) {
+          float x[16];
+          tmem_ld16(tmem_o + u * N + lane_base + col, x);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float f0 = s_f[col + j];
-            o[j] = f0 == 0.f ? 0.f : f0 * o[j];
-            if (ALT) {
-              const float f1 = s_f[N + col + j];
-              o[j] = f1 == 0.f ? o[j] : fmaf(f1, u[j], o[j]);
-            }
+            const float f = s_f[u * N + col + j];
+            const float y = f == 0.f ? 0.f : f * x[j];
+            o[j] = u == 0 ? y : o[j] + y;
           }
-          if (a.n_splits > 1) {
-            float* dst = a.part + (rec0 + col) * HD + d;
+        }
+        if (a.n_splits > 1) {
+          float* dst = a.part + (rec0 + col) * HD + d;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (col + j < nrows) dst[j * HD] = o[j];
-          } else {
-            int tok = col / a.G, g = col - tok * a.G;
-            bf16* base = static_cast<bf16*>(a.out) + (int64_t)h * a.G * HD + d;
+          for (int j = 0; j < 16; ++j)
+            if (col + j < nrows) dst[j * HD] = o[j];
+        } else {
+          int tok = col / a.G, g = col - tok * a.G;
+          bf16* base = static_cast<bf16*>(a.out) + (int64_t)h * a.G * HD + d;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (col + j < nrows) base[(int64_t)(t0 + tok) * a.ldo + g * HD] = f2bf(o[j]);
-              if (++g == a.G) g = 0, ++tok;
-            }
+          for (int j = 0; j < 16; ++j) {
+            if (col + j < nrows) base[(int64_t)(t0 + tok) * a.ldo + g * HD] = f2bf(o[j]);
+            if (++g == a.G) g = 0, ++tok;
           }
         }
       }
@@ -1210,7 +1234,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 10) {
+  if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -1312,24 +1336,23 @@ static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64
   AttnQ8Maps maps;
   if (const int rc = q8_tensor_map(cache.k, cache, &maps.k)) return rc;
   if (const int rc = q8_tensor_map(cache.v, cache, &maps.v)) return rc;
-  const int fixed = q8_fixed_smem(HD, chunks * 16);
+  const Q8Shape f = q8_shape(chunks);
+  const int fixed = q8_fixed_smem(HD, chunks * 16, f);
   int stages = (232448 - fixed) / (2 * kQ8Keys * HD);
   if (stages > kQ8MaxStages) stages = kQ8MaxStages;
   const size_t smem = (size_t)fixed + (size_t)stages * 2 * kQ8Keys * HD;
-  typedef void (*Kern)(const AttnQ8Maps, const AttnQ8Args, int, int, int, int);
-  const Kern alt[5] = {attn_q8_tc_kernel<HD, 1, true>, attn_q8_tc_kernel<HD, 2, true>, attn_q8_tc_kernel<HD, 3, true>,
-                       attn_q8_tc_kernel<HD, 4, true>, attn_q8_tc_kernel<HD, 5, true>};
-  const Kern half[3] = {attn_q8_tc_kernel<HD, 3, false>, attn_q8_tc_kernel<HD, 4, false>,
-                        attn_q8_tc_kernel<HD, 5, false>};
+  typedef void (*Kern)(const AttnQ8Maps, const AttnQ8Args, int, int, int, int, int);
+  const Kern kerns[5] = {attn_q8_tc_kernel<HD, 1, 4>, attn_q8_tc_kernel<HD, 2, 4>, attn_q8_tc_kernel<HD, 2, 2>,
+                         attn_q8_tc_kernel<HD, 2, 1>, attn_q8_tc_kernel<HD, 3, 1>};
   static bool set = false;
   if (!set) {
-    for (Kern k : alt) allow_max_dynamic_smem(k);
-    for (Kern k : half) allow_max_dynamic_smem(k);
+    for (Kern k : kerns) allow_max_dynamic_smem(k);
     set = true;
   }
-  const Kern kern = chunks * 16 <= kQ8AltRows ? alt[chunks - 1] : half[(chunks + 1) / 2 - 3];
-  int rc = launch_kernel("attn_q8_tc_kernel", kern, dim3((unsigned)blocks, (unsigned)splits), dim3(kQ8Threads), smem,
-                         stream, 1u, 1u, maps, a, chunks, tpg, stages, shift);
+  const Kern kern = kerns[f.ch == 3 ? 4 : f.sets == 4 ? f.ch - 1 : f.sets == 2 ? 2 : 3];
+  int rc = launch_kernel("attn_q8_tc_kernel", kern, dim3((unsigned)blocks, (unsigned)splits),
+                         dim3((unsigned)(kQ8Helpers + 128 * f.cg * f.sets)), smem, stream, 1u, 1u, maps, a, chunks, f.cg,
+                         tpg, stages, shift);
   if (rc || splits == 1) return rc;
   return launch_kernel("attn_q8_join_kernel", attn_q8_join_kernel<HD>,
                        dim3((unsigned)blocks, (unsigned)((tpg * a.G + 7) / 8)), dim3(256), 0, stream, 1u, 1u, a, tpg);

@@ -257,66 +257,72 @@ class KVLayerQ8:
     [n_kv, max_slots] uint8 (views with any head stride; slots and elements
     contiguous). Element i of a row stands for code[i] * 2^(scale - 127)."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "n_kv", "max_slots", "head_dim", "device", "_c", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_kv", "max_slots", "head_dim", "index", "_c", "_ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        n_kv, slots, hd = k.shape
-        if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+        shape, strides, s_strides, index = k.shape, k.stride(), k_scale.stride(), k.get_device()
+        n_kv, slots, hd = shape
+        if k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn:
             raise ValueError("KVLayerQ8: codes must be float8_e4m3fn")
-        if k_scale.dtype != torch.uint8 or v_scale.dtype != torch.uint8:
+        if k_scale.dtype is not torch.uint8 or v_scale.dtype is not torch.uint8:
             raise ValueError("KVLayerQ8: scale bytes must be uint8")
-        if v.shape != k.shape or k_scale.shape != (n_kv, slots) or v_scale.shape != (n_kv, slots):
+        if v.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
             raise ValueError("KVLayerQ8: k, v [n_kv, max_slots, head_dim] and scales [n_kv, max_slots] do not match")
-        if (k.stride(1), k.stride(2)) != (hd, 1) or v.stride() != k.stride():
+        if strides[1:] != (hd, 1) or v.stride() != strides:
             raise ValueError("KVLayerQ8: k and v need contiguous slots and equal strides")
-        if k_scale.stride(1) != 1 or v_scale.stride() != k_scale.stride():
+        if s_strides[1] != 1 or v_scale.stride() != s_strides:
             raise ValueError("KVLayerQ8: k_scale and v_scale need contiguous slots and equal strides")
-        if not k.is_cuda or not (k.device == v.device == k_scale.device == v_scale.device):
+        if index < 0 or not (v.get_device() == k_scale.get_device() == v_scale.get_device() == index):
             raise ValueError("KVLayerQ8: the cache must live on one CUDA device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_kv, self.max_slots, self.head_dim, self.device = n_kv, slots, hd, k.device
+        self.n_kv, self.max_slots, self.head_dim, self.index = n_kv, slots, hd, index
         # the stride of a single head is never used; give the C side one that cannot overlap
-        hs = k.stride(0) if n_kv > 1 else slots * hd
-        ss = k_scale.stride(0) if n_kv > 1 else slots
-        self._c = L.SsdKvQ8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), hs, ss, slots, n_kv, hd)
+        self._c = L.SsdKvQ8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                            strides[0] if n_kv > 1 else slots * hd, s_strides[0] if n_kv > 1 else slots, slots, n_kv, hd)
         self._ref = C.byref(self._c)
 
 
-def _q8_ptr(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, dev, numel: int) -> Optional[int]:
-    """Pointer of a contiguous index / table argument of an 8-bit cache op."""
+# The 8-bit cache's wrappers sit on the decode path (one launch of a few
+# microseconds each), so they read each tensor property once.
+def _q8_ptr(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, index: int, numel: int) -> Optional[int]:
+    """Pointer of a contiguous index / table argument on CUDA device `index`."""
     if t is None:
         return None
-    if t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.numel() < numel:
-        raise ValueError(f"{name}: expected >= {numel} contiguous {dtype} values on {dev}, got "
+    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous() or t.numel() < numel:
+        raise ValueError(f"{name}: expected >= {numel} contiguous {dtype} values on cuda:{index}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-def _q8_rows(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, dev, rows: int, width: int) -> tuple:
-    """(pointer, row stride) of a [rows, width] activation argument."""
+def _q8_rows(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, index: int, rows: int, width: int) -> tuple:
+    """(pointer, row stride) of a [>= rows, width] activation argument."""
     if t is None:
         return None, 0
-    if t.dim() != 2 or t.dtype != dtype or t.device != dev or t.shape[0] < rows or t.shape[1] != width or \
-            (width > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: expected [>= {rows}, {width}] {dtype} rows on {dev}, got {tuple(t.shape)} {t.dtype} "
-                         f"on {t.device} with strides {t.stride()}")
-    return t.data_ptr(), t.stride(0)
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or t.dtype is not dtype or t.get_device() != index or shape[0] < rows or shape[1] != width or \
+            (strides[1] != 1 and width > 1):
+        raise ValueError(f"{name}: expected [>= {rows}, {width}] {dtype} rows on cuda:{index}, got {tuple(shape)} "
+                         f"{t.dtype} on {t.device} with strides {strides}")
+    return t.data_ptr(), strides[0]
 
 
-def _q8_call(name: str, dev, *args) -> None:
+def _q8_call(name: str, index: int, *args) -> None:
     """Launch on the tensors' device and that device's current stream."""
-    if dev.index == torch.cuda.current_device():
-        L.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = getattr(L.load(), name)(*args, stream)
     else:
-        with torch.cuda.device(dev):
-            L.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.device(index):
+            rc = getattr(L.load(), name)(*args, stream)
+    if rc:
+        L.check(rc, name)
 
 
-def _q8_status(ws: Optional[Workspace], dev) -> Optional[int]:
+def _q8_status(ws: Optional[Workspace], index: int) -> Optional[int]:
     if ws is None:
         return None
-    if ws.status.device != dev:
-        raise ValueError(f"the workspace lives on {ws.status.device}, the cache on {dev}")
+    if ws.status.get_device() != index:
+        raise ValueError(f"the workspace lives on {ws.status.device}, the cache on cuda:{index}")
     return ws.status.data_ptr()
 
 
@@ -334,7 +340,7 @@ def rope_kv_write_q8(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor
     q_out may be q. The slots of one call must be distinct. Bad slots and
     positions are reported by ws.check_status()."""
     T = k.shape[0] if T is None else T
-    dev, dt = layer.device, k.dtype
+    dev, dt = layer.index, k.dtype
     if n_kv != layer.n_kv or head_dim != layer.head_dim:
         raise ValueError(f"rope_kv_write_q8: cache of {layer.n_kv} heads x {layer.head_dim}, got {n_kv} x {head_dim}")
     if rot_dim is None:
@@ -368,7 +374,7 @@ def kv_read_q8(layer: KVLayerQ8, slots: Optional[torch.Tensor], k_out: Optional[
         raise ValueError("kv_read_q8: k_out or v_out is needed")
     if n is None:
         n = slots.numel() if slots is not None else out.shape[0]
-    dev, dt, width = layer.device, out.dtype, layer.n_kv * layer.head_dim
+    dev, dt, width = layer.index, out.dtype, layer.n_kv * layer.head_dim
     pk, ldk = _q8_rows("k_out", k_out, dt, dev, n, width)
     pv, ldv = _q8_rows("v_out", v_out, dt, dev, n, width)
     _q8_call("ssd_kv_read_q8", dev, layer._ref, _q8_ptr("slots", slots, torch.int32, dev, n), first, n, pk, ldk, pv, ldv,
@@ -384,7 +390,7 @@ def tree_attention_q8(q: torch.Tensor, layer: KVLayerQ8, n_heads: int, n_kv: int
     attends slots [prefix_start[t] (0 if None), prefix_len[t]) plus its mask
     bits from spec_base[0]; a row that sees nothing gives zeros."""
     T = q.shape[0] if T is None else T
-    dev, dt = layer.device, q.dtype
+    dev, dt = layer.index, q.dtype
     if n_kv != layer.n_kv or head_dim != layer.head_dim:
         raise ValueError(f"tree_attention_q8: cache of {layer.n_kv} heads x {layer.head_dim}, got {n_kv} x {head_dim}")
     pq, ldq = _q8_rows("q", q, dt, dev, T, n_heads * head_dim)
@@ -402,11 +408,11 @@ def kv_compact_q8(codes: torch.Tensor, scales: torch.Tensor, start, keep_slots, 
     """kv_compact for an 8-bit cache: codes [L, 2, n_kv, max_slots, head_dim]
     float8_e4m3fn, scales [L, 2, n_kv, max_slots] uint8 (ssd_kv_compact_q8)."""
     Ln, two, n_kv, slots, hd = codes.shape
-    dev, i32 = codes.device, torch.int32
+    dev, i32 = codes.get_device(), torch.int32
     if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8 or scales.shape != (Ln, two, n_kv, slots):
         raise ValueError("kv_compact_q8: codes float8_e4m3fn [L, 2, n_kv, max_slots, head_dim], scales uint8 "
                          "[L, 2, n_kv, max_slots]")
-    if two != 2 or not codes.is_cuda or scales.device != dev or codes.stride()[3:] != (hd, 1) or scales.stride(3) != 1:
+    if two != 2 or dev < 0 or scales.get_device() != dev or codes.stride()[3:] != (hd, 1) or scales.stride(3) != 1:
         raise ValueError("kv_compact_q8: K and V on one CUDA device with contiguous slots")
     _q8_call("ssd_kv_compact_q8", dev, codes.data_ptr(), scales.data_ptr(), Ln, codes.stride(0), codes.stride(1),
              codes.stride(2), scales.stride(0), scales.stride(1), scales.stride(2), n_kv, hd, slots,
