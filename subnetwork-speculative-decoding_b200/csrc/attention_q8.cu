@@ -372,14 +372,13 @@ struct AttnQ8Meta {
   uint32_t map[kQ8MapWords];
   int max_start, min_len;                      // a block inside [max_start, min_len) is visible to every row
   int first, count;                            // this CTA's units of the bitmap
-  int ready;                                   // blocks whose scales and visibility are in place
   int part[4];                                 // per block buffer: not every row sees the whole block
   uint16_t scales[4][kQ8Keys];                 // per block buffer and key: K's scale byte, V's in the high half
   int abort;
-  uint32_t tmem, pad;
+  uint32_t tmem;
   uint64_t k_full[kQ8MaxStages], k_empty[kQ8MaxStages], v_full[kQ8MaxStages], v_clean[kQ8MaxStages],
       v_empty[kQ8MaxStages];
-  uint64_t s_full[4], s_free[4], p_full[4], p_free[4], meta_ready, q_ready, o_full, pad2;
+  uint64_t s_full[4], s_free[4], p_full[4], p_free[4], info_full[4], meta_ready, q_ready, o_full;
 };
 static_assert(sizeof(AttnQ8Meta) % 16 == 0, "the arrays behind it are read 16 bytes at a time");
 
@@ -703,18 +702,6 @@ __device__ __forceinline__ void q8_scores(const float* rowc, float* x, uint64_t 
     for (int j = 0; j < 16; ++j) x[j] = (vis >> j) & 1u ? x[j] : -INFINITY;
   }
 }
-// A counter in shared memory that one warp raises and others wait for.
-__device__ __forceinline__ void st_release_cta(int* p, int v) {
-  asm volatile("st.release.cta.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
-}
-__device__ __forceinline__ bool wait_above(int* p, int v) {
-  for (uint32_t i = 0; i < kWaitLimit; ++i) {
-    int x;
-    asm volatile("ld.acquire.cta.shared::cta.b32 %0, [%1];" : "=r"(x) : "r"(smem_u32(p)) : "memory");
-    if (x > v) return true;
-  }
-  return false;
-}
 __device__ __forceinline__ float q8_warp_max(float v) {  // NaN gives way to numbers, as in fmaxf
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -732,7 +719,8 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   constexpr int BSH = BUFS == 4 ? 2 : 1;
   constexpr int WC = 16 * CH;                     // columns of a warpgroup
   extern __shared__ uint8_t q8_smem_raw[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(q8_smem_raw) + 1023) & ~uintptr_t(1023));
+  // (an offset, not a rounded address: the compiler keeps knowing that this is shared memory)
+  uint8_t* sm = q8_smem_raw + ((1024u - (smem_u32(q8_smem_raw) & 1023u)) & 1023u);
   const int N = 16 * n_chunks;
   const int p_bytes = q8_p_bytes(N), atoms = (N + 31) / 32;
   const int wgs = cgs * A;
@@ -758,7 +746,6 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   if (threadIdx.x == 0) {
     m.max_start = 0;
     m.min_len = INT32_MAX;
-    m.ready = 0;
     m.abort = 0;
     for (int i = 0; i < stages; ++i) {
       mbar_init(&m.k_full[i], 1);
@@ -772,6 +759,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       mbar_init(&m.s_free[i], 4 * cgs);
       mbar_init(&m.p_full[i], 4 * cgs);
       mbar_init(&m.p_free[i], 1);
+      mbar_init(&m.info_full[i], 1);
     }
     mbar_init(&m.meta_ready, 1);
     mbar_init(&m.q_ready, 4 * wgs);
@@ -839,7 +827,11 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       }
     } else if (warp == 2) {
       // The whole warp runs the loop (its addresses stay uniform), one lane
-      // issues. Descriptors of later parts of an operand add to the low word.
+      // issues. The softmax frees S^T's buffer and fills P' at the same time, so
+      // a fixed order loses nothing: S^T runs BUFS blocks ahead of O. (A loop
+      // that polled for whichever is ready cost the softmax warps their
+      // instruction fetch: 20 % of the kernel.) Descriptors of later parts of an
+      // operand add to the low word.
       const bool leader = elect_one();
       if (nblocks > 0) {
         const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true);
@@ -847,40 +839,44 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         const uint32_t k_lo = q8_desc_lo(smem_u32(k_ring), 16), v_lo = q8_desc_lo(smem_u32(v_ring), 0);
         const uint32_t qh_lo = q8_desc_lo(smem_u32(q_hi), 16), ql_lo = q8_desc_lo(smem_u32(q_lo), 16);
         const uint32_t p_lo = q8_desc_lo(p_s, 256);
-        int nS = 0, nP = 0, sS = 0, sP = 0;
-        uint32_t phS = 0, phP = 0, idle = 0;
-        const bool ready = __all_sync(0xffffffffu, mbar_wait(&m.q_ready, 0));
-        if (!ready && lane == 0) give_up();
-        while (ready && nP < nblocks) {
-          bool prog = false;
-          bool go = nS < nblocks && mbar_test(&m.k_full[sS], phS) &&
-                    (nS < BUFS || mbar_test(&m.s_free[nS & (BUFS - 1)], ((nS >> BSH) - 1) & 1));
-          if (__all_sync(0xffffffffu, go)) {
-            tc_fence_after();
+        int sS = 0, sP = 0;
+        uint32_t phS = 0, phP = 0;
+        bool ok = mbar_wait(&m.q_ready, 0);
+#pragma unroll 1
+        for (int nS = 0; nS < nblocks + BUFS; ++nS) {
+          const int nP = nS - BUFS;  // its P' buffer is the S^T buffer's number
+          const int buf = nS & (BUFS - 1);
+          const uint32_t use = ((nP >> BSH) & 1);
+          if (nP >= 0) ok = ok && mbar_wait(&m.s_free[buf], use) && mbar_wait(&m.p_full[buf], use);
+          if (nS < nblocks) ok = ok && mbar_wait(&m.k_full[sS], phS);
+          if (__any_sync(0xffffffffu, !ok || *abort_flag)) {
+            if (lane == 0) give_up();
+            break;
+          }
+          tc_fence_after();
+          if (nS < nblocks) {
             if (leader) {
-              const uint32_t d = tmem + (nS & (BUFS - 1)) * N, k = k_lo + sS * (TILE >> 4);
+              const uint32_t d = tmem + buf * N, k = k_lo + sS * (TILE >> 4);
 #pragma unroll
               for (int ks = 0; ks < HD / 32; ++ks)
                 umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(qh_lo + ks * 2, rows_hi), id_s, ks > 0);
 #pragma unroll
               for (int ks = 0; ks < HD / 32; ++ks)
                 umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(ql_lo + ks * 2, rows_hi), id_s, 1u);
-              umma_commit(&m.s_full[nS & (BUFS - 1)]);
+              umma_commit(&m.s_full[buf]);
               umma_commit(&m.k_empty[sS]);
             }
             __syncwarp();
-            ++nS;
             if (++sS == stages) sS = 0, phS ^= 1u;
-            prog = true;
           }
-          go = nP < nS && mbar_test(&m.p_full[nP & (BUFS - 1)], (nP >> BSH) & 1) && mbar_test(&m.v_clean[sP], phP);
-          if (__all_sync(0xffffffffu, go)) {
+          if (nP >= 0) {
+            ok = mbar_wait(&m.v_clean[sP], phP);
             tc_fence_after();
             if (leader) {
               // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
               // M = 128 repeats the first (lanes 64 .. 127 are not read). P': MN-major, atoms of 32 rows x 8 keys.
               const uint32_t d = tmem_o + (nP & (A - 1)) * N;
-              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + (nP & (BUFS - 1)) * (2 * p_bytes >> 4);
+              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + buf * (2 * p_bytes >> 4);
 #pragma unroll
               for (int term = 0; term < 2; ++term)
 #pragma unroll
@@ -888,18 +884,11 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
                   umma_f8(d, q8_desc(v + kk * 2 * HD, rows_hi),
                           q8_desc(pl + term * (p_bytes >> 4) + kk * (atoms * 64), p_hi), id_o,
                           (nP >= A || term > 0 || kk > 0) ? 1u : 0u);
-              umma_commit(&m.p_free[nP & (BUFS - 1)]);
+              umma_commit(&m.p_free[buf]);
               umma_commit(&m.v_empty[sP]);
             }
             __syncwarp();
-            ++nP;
             if (++sP == stages) sP = 0, phP ^= 1u;
-            prog = true;
-          }
-          idle = prog ? 0u : idle + 1u;
-          if (__any_sync(0xffffffffu, idle > kWaitLimit || *abort_flag)) {
-            if (lane == 0) give_up();
-            break;
           }
         }
       }
@@ -946,9 +935,8 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
             }
           }
         }
-        __threadfence_block();
         __syncwarp();
-        if (lane == 0) st_release_cta(&m.ready, b + 1);
+        if (lane == 0) mbar_arrive(&m.info_full[buf]);
         bad = bad || !mbar_wait(&m.v_full[st], phase);
         if (__any_sync(0xffffffffu, bad || *abort_flag)) {
           if (lane == 0) give_up();
@@ -1004,7 +992,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       const int buf = b & (BUFS - 1);
       const uint32_t use = (b >> BSH) & 1;        // parity of the buffer's use by block b
       // After a timeout the loop runs on without waiting: the warpgroup's barriers stay matched.
-      if (!bad && !(wait_above(&m.ready, b) && mbar_wait(&m.s_full[buf], use))) {
+      if (!bad && !(mbar_wait(&m.info_full[buf], use) && mbar_wait(&m.s_full[buf], use))) {
         bad = true;
         give_up();
       }
