@@ -338,7 +338,7 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 // several run side by side: CG of them share a block's columns, 16 CH each, and
 // A such sets take the blocks in turn, each with its own S^T and P' buffers,
 // references, l and O^T, joined at the end. What CH, CG and A are for N columns
-// follows from registers (l: 16 CH), TMEM (N (max(A, 2) + A) <= 512 columns)
+// follows from registers (l: 16 CH), TMEM (N (2 A + A) <= 512 columns)
 // and threads: see q8_shape.
 constexpr int kQ8Keys = 128;
 constexpr int kQ8MaxRows = 144;       // query rows per CTA: three ring stages fit next to their Q and P'
@@ -372,25 +372,27 @@ struct AttnQ8Meta {
   uint32_t map[kQ8MapWords];
   int max_start, min_len;                      // a block inside [max_start, min_len) is visible to every row
   int first, count;                            // this CTA's units of the bitmap
-  int part[4];                                 // per block buffer: not every row sees the whole block
-  uint16_t scales[4][kQ8Keys];                 // per block buffer and key: K's scale byte, V's in the high half
+  int part[8];                                 // per block buffer: not every row sees the whole block
   int abort;
   uint32_t tmem;
   uint64_t k_full[kQ8MaxStages], k_empty[kQ8MaxStages], v_full[kQ8MaxStages], v_clean[kQ8MaxStages],
       v_empty[kQ8MaxStages];
-  uint64_t s_full[4], s_free[4], p_full[4], p_free[4], info_full[4], meta_ready, q_ready, o_full;
+  uint64_t s_full[8], s_free[8], info_full[8], p_full[4], p_free[4], meta_ready, q_ready, o_full;
 };
 static_assert(sizeof(AttnQ8Meta) % 16 == 0, "the arrays behind it are read 16 bytes at a time");
 
-__host__ __device__ constexpr int q8_buffers(int sets) { return sets > 2 ? sets : 2; }  // of S^T and P'
+// S^T runs one block of each set ahead of the softmax; P' has a buffer a set.
+__host__ __device__ constexpr int q8_s_buffers(int sets) { return 2 * sets; }
+__host__ __device__ constexpr int q8_p_buffers(int sets) { return sets > 2 ? sets : 2; }
 __host__ __device__ constexpr int q8_p_bytes(int n) { return (n + 31) / 32 * 4096; }    // one term of one buffer
 // Behind AttnQ8Meta: per softmax warp and column {kBias - M, the last move as
 // a bf16 factor}, per warpgroup {column maxima of each warp's 32 keys}, and per
-// block buffer and token the 128 bits of which of the block's keys it sees.
+// block buffer {per token, the 128 bits of which of the block's keys it sees;
+// per key, K's scale byte and V's in the high half}.
 static int q8_fixed_smem(int hd, int n, const Q8Shape& f) {
   const int state = 4 * f.cg * f.sets * 16 * f.ch;
-  return 1024 + 2 * n * hd + q8_buffers(f.sets) * 2 * q8_p_bytes(n) + (int)sizeof(AttnQ8Meta) + state * 10 +
-         q8_buffers(f.sets) * n * 16;
+  return 1024 + 2 * n * hd + q8_p_buffers(f.sets) * 2 * q8_p_bytes(n) + (int)sizeof(AttnQ8Meta) + state * 10 +
+         q8_s_buffers(f.sets) * (n * 16 + kQ8Keys * 2);
 }
 
 // D[tmem] (+)= A[smem] * B[smem]^T, e4m3 in, fp32 accumulate.
@@ -421,6 +423,22 @@ __device__ __forceinline__ uint64_t q8_desc(uint32_t lo, uint32_t hi) {
 __host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool mn) {
   return (1u << 4) | (mn ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
+}
+// mbar_wait that sleeps longer per poll (up to the hint, 20 us): a dozen warps
+// that poll take instruction fetch from those that work. Gives up after seconds.
+__device__ __forceinline__ bool q8_wait(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < 1u << 17; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
 }
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -715,8 +733,8 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   constexpr int TILE = kQ8Keys * HD;              // bytes of a K or V block
   constexpr uint32_t SW = HD == 128 ? 2u : 4u;    // 128-byte or 64-byte swizzle: one atom row per cache row
   constexpr uint32_t SBO = 8 * HD;                // 8 rows of HD bytes
-  constexpr int BUFS = q8_buffers(A);             // a power of two
-  constexpr int BSH = BUFS == 4 ? 2 : 1;
+  constexpr int SB = q8_s_buffers(A), PB = q8_p_buffers(A);  // powers of two
+  constexpr int SSH = SB == 8 ? 3 : SB == 4 ? 2 : 1, PSH = PB == 4 ? 2 : 1;
   constexpr int WC = 16 * CH;                     // columns of a warpgroup
   extern __shared__ uint8_t q8_smem_raw[];
   // (an offset, not a rounded address: the compiler keeps knowing that this is shared memory)
@@ -726,14 +744,15 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   const int wgs = cgs * A;
   uint8_t* k_ring = sm;
   uint8_t* v_ring = k_ring + stages * TILE;
-  uint8_t* p_buf = v_ring + stages * TILE;        // [BUFS][hi, lo][keys / 8][atoms][8 keys x 32 rows]
-  uint8_t* q_hi = p_buf + BUFS * 2 * p_bytes;     // [N][HD]
+  uint8_t* p_buf = v_ring + stages * TILE;        // [PB][hi, lo][keys / 8][atoms][8 keys x 32 rows]
+  uint8_t* q_hi = p_buf + PB * 2 * p_bytes;       // [N][HD]
   uint8_t* q_lo = q_hi + N * HD;
   AttnQ8Meta& m = *reinterpret_cast<AttnQ8Meta*>(q_lo + N * HD);
   float* refs = reinterpret_cast<float*>(&m + 1);                            // [softmax warps][WC]
   float* wmax = refs + 4 * wgs * WC;                                         // [warpgroups][4][WC]
-  uint32_t* vis = reinterpret_cast<uint32_t*>(wmax + 4 * wgs * WC);          // [BUFS][N tokens][4]
-  uint16_t* factors = reinterpret_cast<uint16_t*>(vis + BUFS * N * 4);       // [softmax warps][WC]
+  uint32_t* vis = reinterpret_cast<uint32_t*>(wmax + 4 * wgs * WC);          // [SB][N tokens][4]
+  uint16_t* scales = reinterpret_cast<uint16_t*>(vis + SB * N * 4);          // [SB][keys]
+  uint16_t* factors = scales + SB * kQ8Keys;                                 // [softmax warps][WC]
   volatile int* abort_flag = &m.abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -754,12 +773,14 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       mbar_init(&m.v_clean[i], 1);
       mbar_init(&m.v_empty[i], 1);
     }
-    for (int i = 0; i < BUFS; ++i) {
+    for (int i = 0; i < SB; ++i) {
       mbar_init(&m.s_full[i], 1);
       mbar_init(&m.s_free[i], 4 * cgs);
+      mbar_init(&m.info_full[i], 1);
+    }
+    for (int i = 0; i < PB; ++i) {
       mbar_init(&m.p_full[i], 4 * cgs);
       mbar_init(&m.p_free[i], 1);
-      mbar_init(&m.info_full[i], 1);
     }
     mbar_init(&m.meta_ready, 1);
     mbar_init(&m.q_ready, 4 * wgs);
@@ -778,7 +799,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = m.tmem, tmem_o = tmem + BUFS * N;  // BUFS S^T buffers, then A O^T, N columns each
+  const uint32_t tmem = m.tmem, tmem_o = tmem + SB * N;  // SB S^T buffers, then A O^T, N columns each
   pdl_wait();
   pdl_trigger();
   const uint32_t p_s = smem_u32(p_buf);
@@ -813,7 +834,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         int st = 0, issued = 0;
         uint32_t phase = 0;
         for (int b = 0; b < nblocks; ++b) {
-          if ((b >= stages && !mbar_wait(&empty[st], phase ^ 1u)) || *abort_flag) {
+          if ((b >= stages && !q8_wait(&empty[st], phase ^ 1u)) || *abort_flag) {
             give_up();
             break;
           }
@@ -828,7 +849,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
     } else if (warp == 2) {
       // The whole warp runs the loop (its addresses stay uniform), one lane
       // issues. The softmax frees S^T's buffer and fills P' at the same time, so
-      // a fixed order loses nothing: S^T runs BUFS blocks ahead of O. (A loop
+      // a fixed order loses nothing: S^T runs SB blocks ahead of O. (A loop
       // that polled for whichever is ready cost the softmax warps their
       // instruction fetch: 20 % of the kernel.) Descriptors of later parts of an
       // operand add to the low word.
@@ -841,14 +862,13 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         const uint32_t p_lo = q8_desc_lo(p_s, 256);
         int sS = 0, sP = 0;
         uint32_t phS = 0, phP = 0;
-        bool ok = mbar_wait(&m.q_ready, 0);
+        bool ok = q8_wait(&m.q_ready, 0);
 #pragma unroll 1
-        for (int nS = 0; nS < nblocks + BUFS; ++nS) {
-          const int nP = nS - BUFS;  // its P' buffer is the S^T buffer's number
-          const int buf = nS & (BUFS - 1);
-          const uint32_t use = ((nP >> BSH) & 1);
-          if (nP >= 0) ok = ok && mbar_wait(&m.s_free[buf], use) && mbar_wait(&m.p_full[buf], use);
-          if (nS < nblocks) ok = ok && mbar_wait(&m.k_full[sS], phS);
+        for (int nS = 0; nS < nblocks + SB; ++nS) {
+          const int nP = nS - SB, buf = nS & (SB - 1), pbuf = nP & (PB - 1);
+          if (nP >= 0)
+            ok = ok && q8_wait(&m.s_free[buf], (nP >> SSH) & 1) && q8_wait(&m.p_full[pbuf], (nP >> PSH) & 1);
+          if (nS < nblocks) ok = ok && q8_wait(&m.k_full[sS], phS);
           if (__any_sync(0xffffffffu, !ok || *abort_flag)) {
             if (lane == 0) give_up();
             break;
@@ -870,13 +890,13 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
             if (++sS == stages) sS = 0, phS ^= 1u;
           }
           if (nP >= 0) {
-            ok = mbar_wait(&m.v_clean[sP], phP);
+            ok = q8_wait(&m.v_clean[sP], phP);
             tc_fence_after();
             if (leader) {
               // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
               // M = 128 repeats the first (lanes 64 .. 127 are not read). P': MN-major, atoms of 32 rows x 8 keys.
               const uint32_t d = tmem_o + (nP & (A - 1)) * N;
-              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + buf * (2 * p_bytes >> 4);
+              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + pbuf * (2 * p_bytes >> 4);
 #pragma unroll
               for (int term = 0; term < 2; ++term)
 #pragma unroll
@@ -884,7 +904,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
                   umma_f8(d, q8_desc(v + kk * 2 * HD, rows_hi),
                           q8_desc(pl + term * (p_bytes >> 4) + kk * (atoms * 64), p_hi), id_o,
                           (nP >= A || term > 0 || kk > 0) ? 1u : 0u);
-              umma_commit(&m.p_free[buf]);
+              umma_commit(&m.p_free[pbuf]);
               umma_commit(&m.v_empty[sP]);
             }
             __syncwarp();
@@ -913,11 +933,11 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       int st = 0;
       uint32_t phase = 0;
       for (int b = 0; b < nblocks; ++b) {
-        const int kb = next_kb, buf = b & (BUFS - 1);
+        const int kb = next_kb, buf = b & (SB - 1);
         const bool part = kb < max_start || kb + kQ8Keys > min_len;
-        bool bad = b >= BUFS && !mbar_wait(&m.s_free[buf], ((b >> BSH) - 1) & 1);  // block b - BUFS is done with them
+        bool bad = b >= SB && !q8_wait(&m.s_free[buf], ((b >> SSH) - 1) & 1);  // block b - SB is done with them
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m.scales[buf][i * 32 + lane] = static_cast<uint16_t>(bytes[i]);
+        for (int i = 0; i < 4; ++i) scales[buf * kQ8Keys + i * 32 + lane] = static_cast<uint16_t>(bytes[i]);
         if (b + 1 < nblocks) fetch();
         if (lane == 0) m.part[buf] = part;
         uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
@@ -937,7 +957,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.info_full[buf]);
-        bad = bad || !mbar_wait(&m.v_full[st], phase);
+        bad = bad || !q8_wait(&m.v_full[st], phase);
         if (__any_sync(0xffffffffu, bad || *abort_flag)) {
           if (lane == 0) give_up();
           break;
@@ -982,22 +1002,22 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
     __syncwarp();
     named_bar_sync(kQ8BarSoftmax, 128 * wgs);  // the rows' scales are read by other warps than wrote them
     if (lane == 0) mbar_arrive(&m.q_ready);
-    bool bad = !mbar_wait(&m.meta_ready, 0);
+    bool bad = !q8_wait(&m.meta_ready, 0);
     if (bad) give_up();
     const int nblocks = bad ? 0 : m.count << unit_shift;
     float l[WC];
 #pragma unroll
     for (int i = 0; i < WC; ++i) l[i] = 0.f;
     for (int b = turn; b < nblocks; b += A) {
-      const int buf = b & (BUFS - 1);
-      const uint32_t use = (b >> BSH) & 1;        // parity of the buffer's use by block b
+      const int buf = b & (SB - 1), pbuf = b & (PB - 1);
+      const uint32_t use = (b >> SSH) & 1;        // parity of the S^T buffer's use by block b
       // After a timeout the loop runs on without waiting: the warpgroup's barriers stay matched.
-      if (!bad && !(mbar_wait(&m.info_full[buf], use) && mbar_wait(&m.s_full[buf], use))) {
+      if (!bad && !(q8_wait(&m.info_full[buf], use) && q8_wait(&m.s_full[buf], use))) {
         bad = true;
         give_up();
       }
       const bool part = m.part[buf];
-      const uint32_t bytes = m.scales[buf][key];
+      const uint32_t bytes = scales[buf * kQ8Keys + key];
       const float ck = q8_scale(bytes & 0xffu);
       const int vb = max(static_cast<int>(bytes >> 8), kQ8MinScale);
       const float ev = static_cast<float>(vb - 127), inv_v = q8_inv_scale(vb);
@@ -1060,7 +1080,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         __syncwarp();
         const bool has_o = b >= A;
         // the last P V into this O is block b - A's
-        if (has_o && !bad && !mbar_wait(&m.p_free[(b - A) & (BUFS - 1)], ((b - A) >> BSH) & 1)) {
+        if (has_o && !bad && !q8_wait(&m.p_free[(b - A) & (PB - 1)], ((b - A) >> PSH) & 1)) {
           bad = true;
           give_up();
         }
@@ -1087,11 +1107,11 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         }
         tmem_wait_st();
       }
-      if (b >= BUFS && !bad && !mbar_wait(&m.p_free[buf], use ^ 1u)) {  // P V of block b - BUFS read this buffer
+      if (b >= PB && !bad && !q8_wait(&m.p_free[pbuf], ((b >> PSH) - 1) & 1)) {  // P V of block b - PB read this buffer
         bad = true;
         give_up();
       }
-      const uint32_t pb = p_at + buf * 2 * p_bytes;
+      const uint32_t pb = p_at + pbuf * 2 * p_bytes;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
@@ -1135,12 +1155,12 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&m.s_free[buf]);
-        mbar_arrive(&m.p_full[buf]);
+        mbar_arrive(&m.p_full[pbuf]);
       }
     }
     // ---- results: l summed over the 128 keys' threads, O^T read back (lane = head dim)
     const int parties = 128 * wgs;
-    if (!mbar_wait(&m.o_full, 0)) give_up();
+    if (!q8_wait(&m.o_full, 0)) give_up();
     tc_fence_after();
     __syncwarp();
     named_bar_sync(kQ8BarSoftmax, parties);
