@@ -454,31 +454,6 @@ __device__ __forceinline__ float q8_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Two fp32 lanes per instruction.
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // Which of the slots kb .. kb + 63 a token sees: its range [start, len) plus
 // the mask bits (bit i = slot sb + i) below kv_end.
 __device__ __forceinline__ uint64_t q8_low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
@@ -687,6 +662,20 @@ __device__ __forceinline__ float q8_columns_reduce(float* v, int lane) {
   return MAX ? fmaxf(v[0], got) : v[0] + got;
 }
 
+// 8 columns of O^T, with the wait, and back.
+__device__ __forceinline__ void q8_tmem_ld8(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void q8_tmem_st8(uint32_t taddr, const float* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "f"(v[0]),
+               "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
 // TMEM load without its wait; the wait takes the registers along so that
 // nothing reads them before it.
 __device__ __forceinline__ void q8_tmem_ld16(uint32_t taddr, float* v) {
@@ -705,15 +694,16 @@ __device__ __forceinline__ void q8_tmem_wait16(float* v) {
                : "memory");
 }
 
-// t of 16 columns from their raw products x, in place.
-__device__ __forceinline__ void q8_scores(const float* rowc, float* x, uint64_t ck2, uint64_t ev2, bool part,
-                                          uint32_t vis) {
-  const ulonglong2* rc = reinterpret_cast<const ulonglong2*>(rowc);
+// t of 16 columns from their raw products x, in place. (Paired fp32
+// instructions measured no faster: same rate, more register moves.)
+__device__ __forceinline__ void q8_scores(const float* rowc, float* x, float ck, float ev, bool part, uint32_t vis) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const ulonglong2 r = rc[j];
-    f2_unpack(f2_fma(f2_mul(f2_pack(x[4 * j], x[4 * j + 1]), r.x), ck2, ev2), x[4 * j], x[4 * j + 1]);
-    f2_unpack(f2_fma(f2_mul(f2_pack(x[4 * j + 2], x[4 * j + 3]), r.y), ck2, ev2), x[4 * j + 2], x[4 * j + 3]);
+  for (int j = 0; j < 16; j += 4) {
+    const float4 r = *reinterpret_cast<const float4*>(rowc + j);
+    x[j] = fmaf(x[j] * r.x, ck, ev);
+    x[j + 1] = fmaf(x[j + 1] * r.y, ck, ev);
+    x[j + 2] = fmaf(x[j + 2] * r.z, ck, ev);
+    x[j + 3] = fmaf(x[j + 3] * r.w, ck, ev);
   }
   if (part) {
 #pragma unroll
@@ -736,6 +726,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   constexpr int SB = q8_s_buffers(A), PB = q8_p_buffers(A);  // powers of two
   constexpr int SSH = SB == 8 ? 3 : SB == 4 ? 2 : 1, PSH = PB == 4 ? 2 : 1;
   constexpr int WC = 16 * CH;                     // columns of a warpgroup
+  constexpr bool KEEP = CH < 3;
   extern __shared__ uint8_t q8_smem_raw[];
   // (an offset, not a rounded address: the compiler keeps knowing that this is shared memory)
   uint8_t* sm = q8_smem_raw + ((1024u - (smem_u32(q8_smem_raw) & 1023u)) & 1023u);
@@ -1021,31 +1012,37 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       const float ck = q8_scale(bytes & 0xffu);
       const int vb = max(static_cast<int>(bytes >> 8), kQ8MinScale);
       const float ev = static_cast<float>(vb - 127), inv_v = q8_inv_scale(vb);
-      const uint64_t ck2 = f2_pack(ck, ck), ev2 = f2_pack(ev, ev), iv2 = f2_pack(inv_v, inv_v);
       tc_fence_after();
       const uint32_t ts = tmem + buf * N + lane_base + col_base;
       const uint32_t* vis_buf = vis + buf * N * 4;
-      // t of every column and its maximum over the warp's keys; t is computed
-      // again below rather than held in registers.
-      // (A == 1: s_full(b) does not say that the other warps have read the last block's maxima)
-      if (A == 1) named_bar_sync(1 + wg, 128);
+      // t of every column and its maximum over the warp's keys (with three chunks
+      // the registers do not hold t next to l: it is computed again below)
+      float x[KEEP ? WC : 16];
+      if (KEEP) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          if (c < my_chunks) q8_tmem_ld16(ts + c * 16, x + c * 16);
+      }
+      named_bar_sync(1 + wg, 128);  // the other warps have read the last block's maxima
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
           const uint32_t see = part ? q8_chunk_vis(vis_buf, col_base + c * 16, a.G, ntok, quarter, lane) : 0xffffu;
-          float x[16];
-          q8_tmem_ld16(ts + c * 16, x);
-          q8_tmem_wait16(x);
-          q8_scores(m.rowc + col_base + c * 16, x, ck2, ev2, part, see);
+          float* t = x + (KEEP ? c * 16 : 0);
+          if (!KEEP) q8_tmem_ld16(ts + c * 16, t);
+          q8_tmem_wait16(t);
+          q8_scores(m.rowc + col_base + c * 16, t, ck, ev, part, see);
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
-            const float4 top = make_float4(q8_warp_max(x[j]), q8_warp_max(x[j + 1]), q8_warp_max(x[j + 2]),
-                                           q8_warp_max(x[j + 3]));
-            if (lane == 0) *reinterpret_cast<float4*>(my_max + c * 16 + j) = top;
+            const float4 top = make_float4(q8_warp_max(t[j]), q8_warp_max(t[j + 1]), q8_warp_max(t[j + 2]),
+                                           q8_warp_max(t[j + 3]));
+            *reinterpret_cast<float4*>(my_max + c * 16 + j) = top;  // (all lanes the same: no branch)
           }
         }
       }
+      tc_fence_before();
       __syncwarp();
+      if (KEEP && lane == 0) mbar_arrive(&m.s_free[buf]);  // the scores are in registers
       named_bar_sync(1 + wg, 128);
       // lane i: columns i, i + 32 (each warp for itself, all alike)
       constexpr int PER = (WC + 31) / 32;
@@ -1088,21 +1085,25 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           if (c < my_chunks) {
-            const uint4 f0 = *reinterpret_cast<const uint4*>(my_fac + c * 16);
-            const uint4 f1 = *reinterpret_cast<const uint4*>(my_fac + c * 16 + 8);
-            const uint32_t w[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
-            float o[16];
-            if (has_o) tmem_ld16(to + c * 16, o);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float f[2] = {__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)};
+            for (int part8 = 0; part8 < 2; ++part8) {
+              const int col8 = c * 16 + part8 * 8;
+              const uint4 f = *reinterpret_cast<const uint4*>(my_fac + col8);
+              constexpr uint32_t one = 0x3f803f80u;
+              if (f.x == one && f.y == one && f.z == one && f.w == one) continue;  // none of the eight moved
+              const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+              float o[8];
+              if (has_o) q8_tmem_ld8(to + col8, o);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                l[c * 16 + 2 * j + e] *= f[e];
-                if (has_o) o[2 * j + e] *= f[e];
+              for (int j = 0; j < 4; ++j) {
+                const float f0 = __uint_as_float(w[j] << 16), f1 = __uint_as_float(w[j] & 0xffff0000u);
+                l[col8 + 2 * j] *= f0;
+                l[col8 + 2 * j + 1] *= f1;
+                o[2 * j] *= f0;
+                o[2 * j + 1] *= f1;
               }
+              if (has_o) q8_tmem_st8(to + col8, o);
             }
-            if (has_o) tmem_st16(to + c * 16, o);
           }
         }
         tmem_wait_st();
@@ -1116,11 +1117,13 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
           const int col = col_base + c * 16;
-          const uint32_t see = part ? q8_chunk_vis(vis_buf, col, a.G, ntok, quarter, lane) : 0xffffu;
-          float x[16];
-          q8_tmem_ld16(ts + c * 16, x);
-          q8_tmem_wait16(x);
-          q8_scores(m.rowc + col, x, ck2, ev2, part, see);
+          float* p = x + (KEEP ? c * 16 : 0);
+          if (!KEEP) {
+            const uint32_t see = part ? q8_chunk_vis(vis_buf, col, a.G, ntok, quarter, lane) : 0xffffu;
+            q8_tmem_ld16(ts + c * 16, p);
+            q8_tmem_wait16(p);
+            q8_scores(m.rowc + col, p, ck, ev, part, see);
+          }
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -1129,15 +1132,11 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
             float t4[4], r4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              x[4 * j + e] = q8_ex2(x[4 * j + e] + r[e]);
-              t4[e] = __uint_as_float(__float_as_uint(x[4 * j + e]) & 0xfff00000u);  // 4 significant bits
-              r4[e] = x[4 * j + e] - t4[e];
+              p[4 * j + e] = q8_ex2(p[4 * j + e] + r[e]);
+              t4[e] = __uint_as_float(__float_as_uint(p[4 * j + e]) & 0xfff00000u);  // 4 significant bits
+              r4[e] = p[4 * j + e] - t4[e];
+              l[c * 16 + 4 * j + e] = fmaf(p[4 * j + e], inv_v, l[c * 16 + 4 * j + e]);
             }
-#pragma unroll
-            for (int e = 0; e < 4; e += 2)
-              f2_unpack(f2_fma(f2_pack(x[4 * j + e], x[4 * j + e + 1]), iv2,
-                               f2_pack(l[c * 16 + 4 * j + e], l[c * 16 + 4 * j + e + 1])),
-                        l[c * 16 + 4 * j + e], l[c * 16 + 4 * j + e + 1]);
             hi[j] = q8_pack4(t4[0], t4[1], t4[2], t4[3]);
             lo[j] = q8_pack4(r4[0], r4[1], r4[2], r4[3]);
           }
@@ -1154,7 +1153,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&m.s_free[buf]);
+        if (!KEEP) mbar_arrive(&m.s_free[buf]);
         mbar_arrive(&m.p_full[pbuf]);
       }
     }

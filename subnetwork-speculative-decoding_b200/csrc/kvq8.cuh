@@ -37,7 +37,14 @@ __device__ __forceinline__ uint32_t q8_pack2(float lo, float hi) {
   return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3));
 }
 __device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d) {
-  return q8_pack2(a, b) | (q8_pack2(c, d) << 16);
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
 }
 // Two codes (the low 16 bits of v) to their fp32 values, exact.
 __device__ __forceinline__ float2 q8_unpack2(uint32_t v) {
