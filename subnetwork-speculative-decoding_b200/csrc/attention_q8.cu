@@ -644,6 +644,24 @@ __device__ __forceinline__ uint32_t q8_chunk_vis(const uint32_t* vis_buf, int co
   return vis;
 }
 
+// Scores of a block that not every row sees whole: -inf where the thread's key
+// is not seen, in place in TMEM. Out of line, like q8_rescale: the main loop's
+// instructions have to fit the instruction cache (with this code in it the
+// loop ran 20 % longer on blocks that never execute it).
+__device__ __noinline__ void q8_mask_scores(uint32_t ts, const uint32_t* vis_buf, int col, int chunks, int G, int ntok,
+                                            int quarter, int lane) {
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    const uint32_t vis = q8_chunk_vis(vis_buf, col + c * 16, G, ntok, quarter, lane);
+    float x[16];
+    tmem_ld16(ts + c * 16, x);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = (vis >> j) & 1u ? x[j] : -INFINITY;
+    tmem_st16(ts + c * 16, x);
+  }
+  tmem_wait_st();
+}
+
 // Maximum (or sum) of 16 columns over 32 lanes, halving the columns a lane
 // holds at every step: lane i (and i + 16) returns column i & 15's.
 template <bool MAX>
@@ -676,6 +694,26 @@ __device__ __forceinline__ void q8_tmem_st8(uint32_t taddr, const float* v) {
                "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
                : "memory");
 }
+// O^T's columns times the last moves' factors (bf16 pairs in shared memory).
+__device__ __noinline__ void q8_rescale(uint32_t to, const uint16_t* factors, int chunks) {
+  constexpr uint32_t one = 0x3f803f80u;
+#pragma unroll 1
+  for (int c = 0; c < 2 * chunks; ++c) {
+    const uint4 f = *reinterpret_cast<const uint4*>(factors + c * 8);
+    if (f.x == one && f.y == one && f.z == one && f.w == one) continue;  // none of the eight moved
+    const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+    float o[8];
+    q8_tmem_ld8(to + c * 8, o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[2 * j] *= __uint_as_float(w[j] << 16);
+      o[2 * j + 1] *= __uint_as_float(w[j] & 0xffff0000u);
+    }
+    q8_tmem_st8(to + c * 8, o);
+  }
+  tmem_wait_st();
+}
+
 // TMEM load without its wait; the wait takes the registers along so that
 // nothing reads them before it.
 __device__ __forceinline__ void q8_tmem_ld16(uint32_t taddr, float* v) {
@@ -696,7 +734,7 @@ __device__ __forceinline__ void q8_tmem_wait16(float* v) {
 
 // t of 16 columns from their raw products x, in place. (Paired fp32
 // instructions measured no faster: same rate, more register moves.)
-__device__ __forceinline__ void q8_scores(const float* rowc, float* x, float ck, float ev, bool part, uint32_t vis) {
+__device__ __forceinline__ void q8_scores(const float* rowc, float* x, float ck, float ev) {
 #pragma unroll
   for (int j = 0; j < 16; j += 4) {
     const float4 r = *reinterpret_cast<const float4*>(rowc + j);
@@ -704,10 +742,6 @@ __device__ __forceinline__ void q8_scores(const float* rowc, float* x, float ck,
     x[j + 1] = fmaf(x[j + 1] * r.y, ck, ev);
     x[j + 2] = fmaf(x[j + 2] * r.z, ck, ev);
     x[j + 3] = fmaf(x[j + 3] * r.w, ck, ev);
-  }
-  if (part) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = (vis >> j) & 1u ? x[j] : -INFINITY;
   }
 }
 __device__ __forceinline__ float q8_warp_max(float v) {  // NaN gives way to numbers, as in fmaxf
@@ -726,7 +760,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   constexpr int SB = q8_s_buffers(A), PB = q8_p_buffers(A);  // powers of two
   constexpr int SSH = SB == 8 ? 3 : SB == 4 ? 2 : 1, PSH = PB == 4 ? 2 : 1;
   constexpr int WC = 16 * CH;                     // columns of a warpgroup
-  constexpr bool KEEP = CH < 3;
+  constexpr bool KEEP = CH == 1;
   extern __shared__ uint8_t q8_smem_raw[];
   // (an offset, not a rounded address: the compiler keeps knowing that this is shared memory)
   uint8_t* sm = q8_smem_raw + ((1024u - (smem_u32(q8_smem_raw) & 1023u)) & 1023u);
@@ -1009,13 +1043,13 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       }
       const bool part = m.part[buf];
       const uint32_t bytes = scales[buf * kQ8Keys + key];
-      const float ck = q8_scale(bytes & 0xffu);
+      const float ck = q8_scale(max(bytes & 0xffu, 1u));  // (not 0: a masked score is -inf times this)
       const int vb = max(static_cast<int>(bytes >> 8), kQ8MinScale);
       const float ev = static_cast<float>(vb - 127), inv_v = q8_inv_scale(vb);
       tc_fence_after();
       const uint32_t ts = tmem + buf * N + lane_base + col_base;
-      const uint32_t* vis_buf = vis + buf * N * 4;
-      // t of every column and its maximum over the warp's keys (with three chunks
+      if (part) q8_mask_scores(ts, vis + buf * N * 4, col_base, my_chunks, a.G, ntok, quarter, lane);
+      // t of every column and its maximum over the warp's keys (with more than one chunk
       // the registers do not hold t next to l: it is computed again below)
       float x[KEEP ? WC : 16];
       if (KEEP) {
@@ -1027,11 +1061,10 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
-          const uint32_t see = part ? q8_chunk_vis(vis_buf, col_base + c * 16, a.G, ntok, quarter, lane) : 0xffffu;
           float* t = x + (KEEP ? c * 16 : 0);
           if (!KEEP) q8_tmem_ld16(ts + c * 16, t);
           q8_tmem_wait16(t);
-          q8_scores(m.rowc + col_base + c * 16, t, ck, ev, part, see);
+          q8_scores(m.rowc + col_base + c * 16, t, ck, ev);
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
             const float4 top = make_float4(q8_warp_max(t[j]), q8_warp_max(t[j + 1]), q8_warp_max(t[j + 2]),
@@ -1052,7 +1085,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       for (int k = 0; k < PER; ++k) {
         const int i = lane + 32 * k;
         factor[k] = 1.f;
-        now[k] = 0.f;
+        now[k] = -kQ8Unset;
         if (i < 16 * my_chunks) {
           const float mx = fmaxf(fmaxf(all_max[i], all_max[WC + i]), fmaxf(all_max[2 * WC + i], all_max[3 * WC + i]));
           const float old = my_ref[i];
@@ -1069,44 +1102,26 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
           const int i = lane + 32 * k;
-          if (i < 16 * my_chunks) {
+          if (i < WC) {
             my_ref[i] = now[k];
             my_fac[i] = static_cast<uint16_t>(__float_as_uint(factor[k]) >> 16);  // a power of two or 0: exact
           }
         }
         __syncwarp();
-        const bool has_o = b >= A;
-        // the last P V into this O is block b - A's
-        if (has_o && !bad && !q8_wait(&m.p_free[(b - A) & (PB - 1)], ((b - A) >> PSH) & 1)) {
-          bad = true;
-          give_up();
-        }
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          if (c < my_chunks) {
-#pragma unroll
-            for (int part8 = 0; part8 < 2; ++part8) {
-              const int col8 = c * 16 + part8 * 8;
-              const uint4 f = *reinterpret_cast<const uint4*>(my_fac + col8);
-              constexpr uint32_t one = 0x3f803f80u;
-              if (f.x == one && f.y == one && f.z == one && f.w == one) continue;  // none of the eight moved
-              const uint32_t w[4] = {f.x, f.y, f.z, f.w};
-              float o[8];
-              if (has_o) q8_tmem_ld8(to + col8, o);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float f0 = __uint_as_float(w[j] << 16), f1 = __uint_as_float(w[j] & 0xffff0000u);
-                l[col8 + 2 * j] *= f0;
-                l[col8 + 2 * j + 1] *= f1;
-                o[2 * j] *= f0;
-                o[2 * j + 1] *= f1;
-              }
-              if (has_o) q8_tmem_st8(to + col8, o);
-            }
+        if (b >= A) {  // the last P V into this O is block b - A's
+          if (!bad && !q8_wait(&m.p_free[(b - A) & (PB - 1)], ((b - A) >> PSH) & 1)) {
+            bad = true;
+            give_up();
           }
+          tc_fence_after();
+          q8_rescale(to, my_fac, my_chunks);
         }
-        tmem_wait_st();
+#pragma unroll
+        for (int i = 0; i < WC; i += 2) {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(my_fac)[i / 2];  // (columns past my_chunks: l = 0)
+          l[i] *= __uint_as_float(w << 16);
+          l[i + 1] *= __uint_as_float(w & 0xffff0000u);
+        }
       }
       if (b >= PB && !bad && !q8_wait(&m.p_free[pbuf], ((b >> PSH) - 1) & 1)) {  // P V of block b - PB read this buffer
         bad = true;
@@ -1119,10 +1134,9 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
           const int col = col_base + c * 16;
           float* p = x + (KEEP ? c * 16 : 0);
           if (!KEEP) {
-            const uint32_t see = part ? q8_chunk_vis(vis_buf, col, a.G, ntok, quarter, lane) : 0xffffu;
             q8_tmem_ld16(ts + c * 16, p);
             q8_tmem_wait16(p);
-            q8_scores(m.rowc + col, p, ck, ev, part, see);
+            q8_scores(m.rowc + col, p, ck, ev);
           }
           uint32_t hi[4], lo[4];
 #pragma unroll
