@@ -1049,28 +1049,21 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       tc_fence_after();
       const uint32_t ts = tmem + buf * N + lane_base + col_base;
       if (part) q8_mask_scores(ts, vis + buf * N * 4, col_base, my_chunks, a.G, ntok, quarter, lane);
-      // t of every column and its maximum over the warp's keys (with more than one chunk
-      // the registers do not hold t next to l: it is computed again below)
-      float x[KEEP ? WC : 16];
-      if (KEEP) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-          if (c < my_chunks) q8_tmem_ld16(ts + c * 16, x + c * 16);
-      }
+      // t of every column and its maximum over the warp's keys. (With more than
+      // one chunk the registers do not hold t next to l: it is computed again
+      // below. The loop is rolled for the instruction cache.)
+      float x[16];
       named_bar_sync(1 + wg, 128);  // the other warps have read the last block's maxima
+#pragma unroll 1
+      for (int c = 0; c < my_chunks; ++c) {
+        q8_tmem_ld16(ts + c * 16, x);
+        q8_tmem_wait16(x);
+        q8_scores(m.rowc + col_base + c * 16, x, ck, ev);
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (c < my_chunks) {
-          float* t = x + (KEEP ? c * 16 : 0);
-          if (!KEEP) q8_tmem_ld16(ts + c * 16, t);
-          q8_tmem_wait16(t);
-          q8_scores(m.rowc + col_base + c * 16, t, ck, ev);
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const float4 top = make_float4(q8_warp_max(t[j]), q8_warp_max(t[j + 1]), q8_warp_max(t[j + 2]),
-                                           q8_warp_max(t[j + 3]));
-            *reinterpret_cast<float4*>(my_max + c * 16 + j) = top;  // (all lanes the same: no branch)
-          }
+        for (int j = 0; j < 16; j += 4) {
+          const float4 top = make_float4(q8_warp_max(x[j]), q8_warp_max(x[j + 1]), q8_warp_max(x[j + 2]),
+                                         q8_warp_max(x[j + 3]));
+          *reinterpret_cast<float4*>(my_max + c * 16 + j) = top;  // (all lanes the same: no branch)
         }
       }
       tc_fence_before();
@@ -1132,7 +1125,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
           const int col = col_base + c * 16;
-          float* p = x + (KEEP ? c * 16 : 0);
+          float* p = x;
           if (!KEEP) {
             q8_tmem_ld16(ts + c * 16, p);
             q8_tmem_wait16(p);
