@@ -424,8 +424,10 @@ __host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool mn) {
   return (1u << 4) | (mn ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
 }
-// mbar_wait that sleeps longer per poll (up to the hint, 20 us): a dozen warps
-// that poll take instruction fetch from those that work. Gives up after seconds.
+// mbar_wait that sleeps between polls, for the warps that run ahead of the
+// others (the copies, the scale bytes): polling takes instruction fetch from the
+// warps that work. Waking up is slow, so the warps on the critical path poll.
+// Gives up after seconds.
 __device__ __forceinline__ bool q8_wait(uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < 1u << 17; ++i) {
     uint32_t ok;
@@ -887,13 +889,13 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         const uint32_t p_lo = q8_desc_lo(p_s, 256);
         int sS = 0, sP = 0;
         uint32_t phS = 0, phP = 0;
-        bool ok = q8_wait(&m.q_ready, 0);
+        bool ok = mbar_wait(&m.q_ready, 0);
 #pragma unroll 1
         for (int nS = 0; nS < nblocks + SB; ++nS) {
           const int nP = nS - SB, buf = nS & (SB - 1), pbuf = nP & (PB - 1);
           if (nP >= 0)
-            ok = ok && q8_wait(&m.s_free[buf], (nP >> SSH) & 1) && q8_wait(&m.p_full[pbuf], (nP >> PSH) & 1);
-          if (nS < nblocks) ok = ok && q8_wait(&m.k_full[sS], phS);
+            ok = ok && mbar_wait(&m.s_free[buf], (nP >> SSH) & 1) && mbar_wait(&m.p_full[pbuf], (nP >> PSH) & 1);
+          if (nS < nblocks) ok = ok && mbar_wait(&m.k_full[sS], phS);
           if (__any_sync(0xffffffffu, !ok || *abort_flag)) {
             if (lane == 0) give_up();
             break;
@@ -915,7 +917,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
             if (++sS == stages) sS = 0, phS ^= 1u;
           }
           if (nP >= 0) {
-            ok = q8_wait(&m.v_clean[sP], phP);
+            ok = mbar_wait(&m.v_clean[sP], phP);
             tc_fence_after();
             if (leader) {
               // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
@@ -1027,7 +1029,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
     __syncwarp();
     named_bar_sync(kQ8BarSoftmax, 128 * wgs);  // the rows' scales are read by other warps than wrote them
     if (lane == 0) mbar_arrive(&m.q_ready);
-    bool bad = !q8_wait(&m.meta_ready, 0);
+    bool bad = !mbar_wait(&m.meta_ready, 0);
     if (bad) give_up();
     const int nblocks = bad ? 0 : m.count << unit_shift;
     float l[WC];
@@ -1037,7 +1039,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       const int buf = b & (SB - 1), pbuf = b & (PB - 1);
       const uint32_t use = (b >> SSH) & 1;        // parity of the S^T buffer's use by block b
       // After a timeout the loop runs on without waiting: the warpgroup's barriers stay matched.
-      if (!bad && !(q8_wait(&m.info_full[buf], use) && q8_wait(&m.s_full[buf], use))) {
+      if (!bad && !(mbar_wait(&m.info_full[buf], use) && mbar_wait(&m.s_full[buf], use))) {
         bad = true;
         give_up();
       }
@@ -1102,7 +1104,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         }
         __syncwarp();
         if (b >= A) {  // the last P V into this O is block b - A's
-          if (!bad && !q8_wait(&m.p_free[(b - A) & (PB - 1)], ((b - A) >> PSH) & 1)) {
+          if (!bad && !mbar_wait(&m.p_free[(b - A) & (PB - 1)], ((b - A) >> PSH) & 1)) {
             bad = true;
             give_up();
           }
@@ -1116,7 +1118,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
           l[i + 1] *= __uint_as_float(w & 0xffff0000u);
         }
       }
-      if (b >= PB && !bad && !q8_wait(&m.p_free[pbuf], ((b >> PSH) - 1) & 1)) {  // P V of block b - PB read this buffer
+      if (b >= PB && !bad && !mbar_wait(&m.p_free[pbuf], ((b >> PSH) - 1) & 1)) {  // P V of block b - PB read this buffer
         bad = true;
         give_up();
       }
@@ -1166,7 +1168,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
     }
     // ---- results: l summed over the 128 keys' threads, O^T read back (lane = head dim)
     const int parties = 128 * wgs;
-    if (!q8_wait(&m.o_full, 0)) give_up();
+    if (!mbar_wait(&m.o_full, 0)) give_up();
     tc_fence_after();
     __syncwarp();
     named_bar_sync(kQ8BarSoftmax, parties);
