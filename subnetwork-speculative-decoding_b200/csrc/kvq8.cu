@@ -14,7 +14,7 @@ struct WriteQ8Args {
   int n_q, n_kv, hd;  // n_q: query heads to rotate (0: cache write only)
   const float* cos;
   const float* sin;
-  int max_pos, rot, interleaved;
+  int max_pos, rot, interleaved, wide_tables;  // wide_tables: a lane's 8 elements' entries are aligned float4s
   const int32_t* positions;
   const int32_t* slots;
   uint8_t* kc;
@@ -28,23 +28,38 @@ struct WriteQ8Args {
   uint32_t* status;
 };
 
+// Eight elements as loaded, and their values.
+template <typename T>
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, float* x) {
-  if constexpr (!VEC) {
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+  Raw8<T> r;
+  if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
-  } else if constexpr (sizeof(T) == 2) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    T* e = reinterpret_cast<T*>(r.u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = p[i];
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void values8(const Raw8<T>& r, float* x) {
+#pragma unroll
+  for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+    const uint32_t w[4] = {r.u[h].x, r.u[h].y, r.u[h].z, r.u[h].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      if constexpr (sizeof(T) == 2) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        x[4 * h + i] = __uint_as_float(w[i]);
+      }
     }
-  } else {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   }
 }
 template <typename T, bool VEC>
@@ -86,91 +101,136 @@ __global__ void __launch_bounds__(256) rope_kv_write_q8_kernel(const WriteQ8Args
   const int i0 = l * 8;
   const bool on = i0 < a.hd;
   const int half = a.rot >> 1;
-  int slot = a.slots[t];
-  const bool slot_ok = slot >= 0 && slot < a.max_slots;
-  int pos = 0;
-  if (a.rot) {
-    pos = a.positions[t];
-    if (pos < 0 || pos >= a.max_pos) {
-      if (threadIdx.x == 0 && blockIdx.y == 0) report_error(a.status, kErrBadIndex);
-      pos = 0;
-    }
-  }
-  if (!slot_ok && threadIdx.x == 0 && blockIdx.y == 0) report_error(a.status, kErrBadIndex);
-  // cos / sin and the pair's other element of each of the lane's elements
-  float c[8], s[8];
-  int other[8];
+  const int slot = a.slots[t];
+  int pos = a.rot ? a.positions[t] : 0;
+  // Passes of RPC rows, U at a time, a batch's loads before its first use and
+  // the first batch's before the position is needed (one pass at a time waited
+  // out the memory latency for each; four cost occupancy: 66 and 85 us where
+  // two take 50, 4096 tokens of the 70B shape). A row's loads come before its
+  // stores: q_out may be q. Every lane of a warp runs the same passes.
+  constexpr int U = 2;
+  const int n_rows = a.n_q + 2 * a.n_kv, step = gridDim.y * RPC;
   const bool turns = on && i0 < a.rot;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int i = i0 + j;
-    c[j] = 1.f;
-    s[j] = 0.f;
-    other[j] = i;
-    if (turns && i < a.rot) {
-      const bool second = a.interleaved ? (i & 1) : i >= half;
-      const int f = a.interleaved ? i >> 1 : (second ? i - half : i);
-      c[j] = a.cos[(int64_t)pos * half + f];
-      const float sv = a.sin[(int64_t)pos * half + f];
-      s[j] = second ? sv : -sv;
-      other[j] = a.interleaved ? i ^ 1 : (second ? i - half : i + half);
-    }
-  }
   // the other halves of 8 elements are 8 contiguous, aligned elements
   const bool vec_pair = VEC && !a.interleaved && (half & 7) == 0;
-  const int n_rows = a.n_q + 2 * a.n_kv;
-  const int row0 = blockIdx.y * RPC + threadIdx.x / LPR;
-  // every lane of a warp runs the same number of passes (shuffles below)
-  for (int base = blockIdx.y * RPC; base < n_rows; base += gridDim.y * RPC) {
-    const int r = row0 + (base - blockIdx.y * RPC);
-    const bool live = r < n_rows;
-    const int kind = r < a.n_q ? 0 : (r < a.n_q + a.n_kv ? 1 : 2);
-    const int head = kind == 0 ? r : (kind == 1 ? r - a.n_q : r - a.n_q - a.n_kv);
-    const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
-                   (int64_t)t * (kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv) + (int64_t)head * a.hd;
-    float x[8];
+  // (outside the rotated part a pair's other element is the element itself)
+  auto other = [&](int j) {
+    const int i = i0 + j;
+    return i >= a.rot ? i : a.interleaved ? i ^ 1 : i >= half ? i - half : i + half;
+  };
+  Raw8<T> raw[U], pair[U];
+  auto load_batch = [&](int base) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (live && on) {
-      load8<T, VEC>(src + i0, x);
-      if (kind < 2 && turns) {
-        float y[8];
-        if (vec_pair) {
-          load8<T, VEC>(src + other[0], y);
-        } else if (a.interleaved) {
+    for (int u = 0; u < U; ++u) {
+      const int r = base + u * step + threadIdx.x / LPR;
+      if (r < n_rows && on) {
+        const int kind = r < a.n_q ? 0 : (r < a.n_q + a.n_kv ? 1 : 2);
+        const int head = kind == 0 ? r : (kind == 1 ? r - a.n_q : r - a.n_q - a.n_kv);
+        const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
+                       (int64_t)t * (kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv) + (int64_t)head * a.hd;
+        raw[u] = load8<T, VEC>(src + i0);
+        if (kind < 2 && turns && !a.interleaved) {
+          if (vec_pair) {
+            pair[u] = load8<T, VEC>(src + other(0));
+          } else {
+            T* e = reinterpret_cast<T*>(pair[u].u);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = to_f32<T>(src[other[j]]);
+            for (int j = 0; j < 8; ++j) e[j] = src[other(j)];
+          }
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (other[j] != i0 + j) x[j] = __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(y[j], s[j]));
       }
     }
-    __syncwarp();  // a row's loads come before its stores: q_out may be q
-    if (kind == 0) {
-      if (live && on) store8<T, VEC>(static_cast<T*>(a.q_out) + (int64_t)t * a.ldqo + (int64_t)head * a.hd + i0, x);
+  };
+  load_batch(blockIdx.y * RPC);
+  const bool slot_ok = slot >= 0 && slot < a.max_slots;
+  if (a.rot && (pos < 0 || pos >= a.max_pos)) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) report_error(a.status, kErrBadIndex);
+    pos = 0;
+  }
+  if (!slot_ok && threadIdx.x == 0 && blockIdx.y == 0) report_error(a.status, kErrBadIndex);
+  // cos / sin of each of the lane's elements (sin signed: first of a pair -,
+  // second +)
+  const bool second = !a.interleaved && i0 >= half;  // (where a lane lies in one half)
+  float c[8], s[8];
+  if (turns && a.wide_tables) {
+    const float* ct = a.cos + (int64_t)pos * half + (a.interleaved ? i0 >> 1 : second ? i0 - half : i0);
+    const float* st = a.sin + (ct - a.cos);
+    const float4 c0 = *reinterpret_cast<const float4*>(ct), s0 = *reinterpret_cast<const float4*>(st);
+    if (a.interleaved) {
+      c[0] = c[1] = c0.x, c[2] = c[3] = c0.y, c[4] = c[5] = c0.z, c[6] = c[7] = c0.w;
+      s[0] = -s0.x, s[1] = s0.x, s[2] = -s0.y, s[3] = s0.y, s[4] = -s0.z, s[5] = s0.z, s[6] = -s0.w, s[7] = s0.w;
+    } else {
+      const float4 c1 = reinterpret_cast<const float4*>(ct)[1], s1 = reinterpret_cast<const float4*>(st)[1];
+      const float sg = second ? 1.f : -1.f;
+      c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+      s[0] = sg * s0.x, s[1] = sg * s0.y, s[2] = sg * s0.z, s[3] = sg * s0.w;
+      s[4] = sg * s1.x, s[5] = sg * s1.y, s[6] = sg * s1.z, s[7] = sg * s1.w;
     }
-    float amax = 0.f;
+  } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float m = fabsf(x[j]);
-      amax = m <= 3.402823466e38f ? fmaxf(amax, m) : amax;  // Inf and NaN do not set the scale
-    }
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (live && kind != 0 && slot_ok) {
-      const int byte = q8_scale_byte(amax);
-      const float inv = q8_inv_scale(byte);
-      if (on) {
-        uint8_t* dst = (kind == 1 ? a.kc : a.vc) + (int64_t)head * a.head_stride + (int64_t)slot * a.hd + i0;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(q8_pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
-                                                    q8_pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv));
+      const int i = i0 + j;
+      c[j] = 1.f;
+      s[j] = 0.f;
+      if (turns && i < a.rot) {
+        const bool sec = a.interleaved ? (i & 1) : i >= half;
+        const int64_t f = (int64_t)pos * half + (a.interleaved ? i >> 1 : (sec ? i - half : i));
+        c[j] = a.cos[f];
+        s[j] = sec ? a.sin[f] : -a.sin[f];
       }
-      if (l == 0) (kind == 1 ? a.ks : a.vs)[(int64_t)head * a.scale_head_stride + slot] = static_cast<uint8_t>(byte);
     }
+  }
+  for (int base = blockIdx.y * RPC; base < n_rows; base += U * step) {
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (base + u * step >= n_rows) break;  // uniform
+      const int r = base + u * step + threadIdx.x / LPR;
+      const bool live = r < n_rows;
+      const int kind = r < a.n_q ? 0 : (r < a.n_q + a.n_kv ? 1 : 2);
+      const int head = kind == 0 ? r : (kind == 1 ? r - a.n_q : r - a.n_q - a.n_kv);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      if (live && on) {
+        values8<T>(raw[u], x);
+        if (kind < 2 && turns) {
+          float y[8];
+          if (a.interleaved) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
+          } else {
+            values8<T>(pair[u], y);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (i0 + j < a.rot) x[j] = __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(y[j], s[j]));
+        }
+      }
+      if (kind == 0) {
+        if (live && on) store8<T, VEC>(static_cast<T*>(a.q_out) + (int64_t)t * a.ldqo + (int64_t)head * a.hd + i0, x);
+      }
+      if (__all_sync(0xffffffffu, kind == 0)) continue;
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float m = fabsf(x[j]);
+        amax = m <= 3.402823466e38f ? fmaxf(amax, m) : amax;  // Inf and NaN do not set the scale
+      }
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (live && kind != 0 && slot_ok) {
+        const int byte = q8_scale_byte(amax);
+        const float inv = q8_inv_scale(byte);
+        if (on) {
+          uint8_t* dst = (kind == 1 ? a.kc : a.vc) + (int64_t)head * a.head_stride + (int64_t)slot * a.hd + i0;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(q8_pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
+                                                      q8_pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv));
+        }
+        if (l == 0) (kind == 1 ? a.ks : a.vs)[(int64_t)head * a.scale_head_stride + slot] = static_cast<uint8_t>(byte);
+      }
+    }
+    if (base + U * step < n_rows) load_batch(base + U * step);
   }
 }
 
@@ -360,6 +420,8 @@ int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk,
   a.sin = rope_sin;
   a.max_pos = (int)(max_pos > INT32_MAX ? INT32_MAX : max_pos);
   a.rot = (int)rot_dim;
+  a.wide_tables = rot_dim % 16 == 0 && (reinterpret_cast<uintptr_t>(rope_cos) & 15) == 0 &&
+                  (reinterpret_cast<uintptr_t>(rope_sin) & 15) == 0;
   a.interleaved = interleaved ? 1 : 0;
   a.positions = positions;
   a.slots = slots;
