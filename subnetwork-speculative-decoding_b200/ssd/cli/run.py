@@ -64,6 +64,8 @@ def parser() -> argparse.ArgumentParser:
     src.add_argument("--prompt-file")
     p.add_argument("--mode", choices=["sd", "target"], default="sd")
     p.add_argument("--max-new-tokens", type=int, default=256)
+    p.add_argument("--kv-dtype", choices=["e4m3"], help="hold the key/value cache in 8-bit rows (default: the config's "
+                                                        "model.kv_dtype; not in the reference)")
     p.add_argument("--raw", action="store_true", help="don't wrap the prompt in the chat template")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--no-warmup", action="store_true")
@@ -120,6 +122,7 @@ def _load(args, prompt: str):
         raise SystemExit("ssd-run: --config is required (or --synthetic NAME)")
     cfg = SSDConfig.from_yaml(args.config)
     cfg.drafting = replace(cfg.drafting, **tree_overrides(args))
+    args.kv_dtype = args.kv_dtype or cfg.model.kv_dtype
     base = runtime.load_base_model(cfg)
     tokenizer = runtime.load_tokenizer(cfg)
     draft = None
@@ -158,11 +161,13 @@ def main(argv: Optional[list[str]] = None) -> None:
     dev = runtime.input_device(base)
     ids = ids.to(dev)
     n_layers = base.config.num_hidden_layers
-    target = TargetRunner(base)
+    target = TargetRunner(base, kv_dtype=args.kv_dtype)
     print(f"\nprompt: {ids.shape[1]} tokens | device: {dev} | draft layers {profile_name(layers)} "
           f"({len(layers)}/{n_layers})")
     print(f"tree: depth={dcfg.depth} branch={dcfg.branch} width={dcfg.width} max_nodes={dcfg.max_nodes} "
           f"temperature={dcfg.temperature} top_p={dcfg.top_p} draft_vocab={dcfg.draft_vocab or 'full'}")
+    if args.kv_dtype:
+        print(f"key/value cache: {args.kv_dtype}")
 
     def run_ar(n: int):
         return autoregressive_generate(target, ids, n, eos_ids, dcfg.temperature, dcfg.top_p, args.seed)

@@ -17,6 +17,15 @@ from typing import Any, Optional, Union
 import yaml
 
 
+KV_DTYPES = (None, "e4m3")  # of the key/value cache: the model's dtype, or 8-bit rows
+
+
+def check_kv_dtype(kv_dtype: Optional[str]) -> Optional[str]:
+    if kv_dtype not in KV_DTYPES:
+        raise ValueError(f"kv_dtype must be one of {KV_DTYPES}, got {kv_dtype!r}")
+    return kv_dtype
+
+
 @dataclass
 class BridgeConfig:
     mlp_type: str = "mlp"  # "mlp" | "swiglu"
@@ -36,6 +45,7 @@ class ModelConfig:
     device_map: Optional[str] = None
     device: str = "auto"
     attn_implementation: str = "sdpa"
+    kv_dtype: Optional[str] = None  # key/value cache: None = torch_dtype, "e4m3" = 8-bit rows (not in the reference)
 
 
 @dataclass
@@ -218,6 +228,7 @@ class SSDConfig:
                              f"got {layers!r}")
         cfg = _section(cls, raw, "config")
         cfg.drafting.validate()
+        check_kv_dtype(cfg.model.kv_dtype)
         return cfg
 
     def validate_against(self, num_hidden_layers: int) -> None:

@@ -37,6 +37,8 @@ class BatchDecoder:
         self.cache = target.new_cache(batch * region)
         self.cache.allocate(w.Hkv, w.hd, w.dtype, w.device)
         self.scratch = R.Scratch(w, max(max_rows, batch))
+        if self.cache.quantized:
+            self.scratch.qkv(1)
         self.ws = ops.Workspace(self.device, max_rows=max(max_rows, 64), vocab=w.V, max_head_rows=max(batch, 1))
         self.fwd = R.ForwardInputs(max(max_rows, batch), self.device, mask_words=1)
         self.starts = torch.zeros(max(max_rows, batch), dtype=torch.int32, device=self.device)

@@ -110,7 +110,11 @@ class _Decoder:
         self.out_cap = max_new + 64
         self.out_tokens = torch.zeros(self.out_cap, **i32)
         self.round_log = torch.zeros(1 + self.out_cap, **i32)
+        if w.tp is not None and cache.quantized:
+            raise NotImplementedError("an 8-bit KVCache is not supported with tensor parallelism")
         self.scratch = R.Scratch(w, max(fwd_rows, 1))
+        if cache.quantized:
+            self.scratch.qkv(1)  # before any graph capture
         self.ws = ops.Workspace(self.device, max_rows=max(fwd_rows, 64), vocab=w.V, max_head_rows=max(head_rows, 1))
         self.argmax = torch.zeros(max(head_rows, 1), **i32)
         self.amax = torch.zeros(max(head_rows, 1), dtype=torch.float32, device=self.device)
@@ -303,8 +307,12 @@ class GreedyRound(_Decoder):
     def commit_phase(self) -> None:
         """keep_positions + append accepted + bonus (speculative.py:165-172)."""
         st = self.state
-        ops.kv_compact(self.cache.buf, st[SEQ:SEQ + 1], self.keep_slots, st[N_KEEP:N_KEEP + 1],
-                       max_keep=self.plan.depth + 1, status=self.ws.status)
+        if self.cache.quantized:
+            ops.kv_compact_q8(self.cache.buf, self.cache.scales, st[SEQ:SEQ + 1], self.keep_slots,
+                              st[N_KEEP:N_KEEP + 1], self.plan.depth + 1, self.ws)
+        else:
+            ops.kv_compact(self.cache.buf, st[SEQ:SEQ + 1], self.keep_slots, st[N_KEEP:N_KEEP + 1],
+                           max_keep=self.plan.depth + 1, status=self.ws.status)
         ops.round_commit(st[N_ACC:N_ACC + 1], self.accepted, self.tree.tokens, st[BONUS:BONUS + 1], st[SEQ:SEQ + 1],
                          st[ROOT_TOK:ROOT_TOK + 1], self.out_tokens, st[N_OUT:N_OUT + 1], self.round_log,
                          self.ws.status)

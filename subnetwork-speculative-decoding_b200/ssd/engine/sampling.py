@@ -285,7 +285,7 @@ def sampled_autoregressive(target, input_ids: torch.Tensor, max_new_tokens: int,
     dev = target.weights.device
     n_prompt = int(input_ids.shape[-1])
     cap = max_cache or cache_capacity(n_prompt, max_new_tokens)
-    key = ("ar_sample", n_prompt, max_new_tokens, cap, float(temperature), float(top_p))
+    key = ("ar_sample", n_prompt, max_new_tokens, cap, float(temperature), float(top_p), target.kv_dtype)
     eng = _engine_cache(target, key, lambda: SampledTargetStep(target, target.new_cache(cap), max_new_tokens,
                                                                temperature, top_p, 0))
     eng.set_seed(seed_from(seed))
@@ -306,7 +306,7 @@ def sampled_speculative(gen, input_ids: torch.Tensor, max_new_tokens: int, eos_i
     dev = gen.target.weights.device
     n_prompt = int(input_ids.shape[-1])
     cap = max_cache or cache_capacity(n_prompt, max_new_tokens, gen.plan)
-    key = ("sd_sample", id(gen.draft), n_prompt, max_new_tokens, cap, repr(cfg))
+    key = ("sd_sample", id(gen.draft), n_prompt, max_new_tokens, cap, repr(cfg), gen.target.kv_dtype)
     eng = _engine_cache(gen, key, lambda: SampledRound(gen.target, gen.draft, cfg, gen.target.new_cache(cap),
                                                        max_new_tokens, 0))
     eng.set_seed(seed_from(seed))

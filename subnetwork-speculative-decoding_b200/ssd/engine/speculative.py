@@ -22,7 +22,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from ssd.config import DraftingConfig
+from ssd.config import DraftingConfig, check_kv_dtype
 from ssd.engine.round import GreedyRound, TargetStep, TreePlan, cache_capacity
 from ssd.engine.kv_cache import KVCache
 from ssd.models.subnetwork_draft import SubnetworkDraftModel
@@ -53,10 +53,13 @@ def _finish(tokens: list[int], eos_ids: set[int], max_new: int) -> tuple[list[in
 
 
 class TargetRunner(SubnetworkDraftModel):
-    """The full target through the same layer kernels (speculative.py:94-98)."""
+    """The full target through the same layer kernels (speculative.py:94-98).
+    kv_dtype: of the key/value caches that decoding with it makes; "e4m3" holds
+    them in 8-bit rows (not in the reference)."""
 
-    def __init__(self, base: nn.Module):
+    def __init__(self, base: nn.Module, kv_dtype: Optional[str] = None):
         super().__init__(base, list(range(base.config.num_hidden_layers)))
+        self.kv_dtype = check_kv_dtype(kv_dtype)
 
 
 def _sync(dev) -> None:
@@ -111,7 +114,7 @@ def autoregressive_generate(target: TargetRunner, input_ids: torch.Tensor, max_n
     dev = target.weights.device
     n_prompt = int(input_ids.shape[-1])
     cap = max_cache or cache_capacity(n_prompt, max_new_tokens)
-    eng = _engine_cache(target, ("ar", n_prompt, max_new_tokens, cap),
+    eng = _engine_cache(target, ("ar", n_prompt, max_new_tokens, cap, target.kv_dtype),
                         lambda: TargetStep(target, target.new_cache(cap), max_new_tokens))
     times: dict[str, float] = {}
     _sync(dev)
@@ -169,7 +172,7 @@ class SpeculativeGenerator:
         dev = self.target.weights.device
         n_prompt = int(input_ids.shape[-1])
         cap = max_cache or cache_capacity(n_prompt, max_new_tokens, self.plan)
-        key = ("sd", id(self.draft), n_prompt, max_new_tokens, cap, repr(cfg))
+        key = ("sd", id(self.draft), n_prompt, max_new_tokens, cap, repr(cfg), self.target.kv_dtype)
         eng = _engine_cache(self, key, lambda: GreedyRound(self.target, self.draft, cfg, self.target.new_cache(cap),
                                                            max_new_tokens))
         times: dict[str, float] = {}

@@ -6,6 +6,8 @@ Per layer (all launches on the current stream, no host syncs):
   rmsnorm -> QKV GEMM (+RoPE, K/V written into the cache) -> tree attention
   -> o_proj GEMM (+residual) -> rmsnorm -> gate/up GEMM (+SwiGLU)
   -> down GEMM (+residual)
+Over an 8-bit cache the q/k/v GEMM writes plain rows, which one kernel then
+rotates and quantises into the cache, and attention reads the 8-bit rows.
 The residual stream is fp32; GEMM operands use the weights' dtype (bf16:
 tcgen05 tensor cores, fp32: CUDA cores). Every buffer is allocated once and
 reused, so a forward can be captured in a CUDA graph.
@@ -206,6 +208,7 @@ class Scratch:
         self.attn = torch.zeros(rows, w.H * w.hd, dtype=w.dtype, device=dev)
         self._xn: dict = {}
         self._hid: dict = {}
+        self._qkv = None
         self.width = max(w.d, w.F)
 
     def xn(self, dtype: torch.dtype, cols: int) -> torch.Tensor:
@@ -222,6 +225,13 @@ class Scratch:
             t = torch.zeros(self.rows, max(cols, self.w.F), dtype=dtype, device=self.w.device)
             self._hid[key] = t
         return t
+
+    def qkv(self, rows: int) -> torch.Tensor:
+        """q | k | v rows of a forward over an 8-bit cache (before the rotation)."""
+        if self._qkv is None:
+            w = self.w
+            self._qkv = torch.zeros(self.rows, (w.H + 2 * w.Hkv) * w.hd, dtype=w.dtype, device=w.device)
+        return self._qkv[:rows]
 
     def reserve_bridges(self, bridges) -> None:
         """Allocate bridge buffers up front (before any graph capture)."""
@@ -257,19 +267,44 @@ def run_bridge(bridge, scratch: Scratch, T: int, ws: ops.Workspace) -> None:
                resid=scratch.resid[:T])
 
 
+def write_kv_q8(w: ModelWeights, qkv: torch.Tensor, fwd: ForwardInputs, T: int, layer, scratch: Scratch,
+                ws: ops.Workspace) -> None:
+    """Projected q | k | v rows -> rotated q in scratch.q, rotated and quantised
+    k / v in the 8-bit cache layer."""
+    nq, nkv = w.H * w.hd, w.Hkv * w.hd
+    ops.rope_kv_write_q8(qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:], w.H, w.Hkv, w.hd, w.rope_cos, w.rope_sin,
+                         fwd.positions, fwd.slots, layer, scratch.q, ws, T=T)
+
+
+def attend(w: ModelWeights, li: int, fwd: ForwardInputs, T: int, cache, scratch: Scratch, ws: ops.Workspace,
+           kv_bound: int) -> None:
+    """scratch.attn[:T] <- attention of scratch.q[:T] over layer li of the cache."""
+    masked = dict(spec_base=fwd.spec_base if fwd.use_mask else None, spec_mask=fwd.mask if fwd.use_mask else None,
+                  kv_bound=kv_bound, T=T, prefix_start=fwd.prefix_start)
+    if cache.quantized:
+        ops.tree_attention_q8(scratch.q[:T], cache.layer_q8(li), w.H, w.Hkv, w.hd, fwd.prefix_len, scratch.attn[:T], ws,
+                              **masked)
+    else:
+        kc, vc = cache.layer(li)
+        ops.tree_attention(scratch.q[:T], kc, vc, w.H, w.Hkv, w.hd, fwd.prefix_len, scratch.attn[:T], ws, **masked)
+
+
 def run_layer(w: ModelWeights, li: int, fwd: ForwardInputs, T: int, cache, scratch: Scratch, ws: ops.Workspace,
               kv_bound: int) -> None:
     """One decoder layer (subnetwork_draft.py:193-246) through the kernels."""
     lw = w.layers[li]
-    kc, vc = cache.layer(li)
     xn = scratch.xn(w.dtype, w.d)[:T, : w.d]
     resid = scratch.resid[:T]
     ops.rmsnorm(resid, lw.ln1, lw.eps1, xn)
-    ops.qkv_rope(xn, lw.q, lw.k, lw.v, w.H, w.Hkv, w.hd, w.rope_cos, w.rope_sin, fwd.positions, fwd.slots, kc, vc,
-                 scratch.q[:T], ws, T=T)
-    ops.tree_attention(scratch.q[:T], kc, vc, w.H, w.Hkv, w.hd, fwd.prefix_len, scratch.attn[:T], ws,
-                       spec_base=fwd.spec_base if fwd.use_mask else None, spec_mask=fwd.mask if fwd.use_mask else None,
-                       kv_bound=kv_bound, T=T, prefix_start=fwd.prefix_start)
+    if cache.quantized:
+        qkv = scratch.qkv(T)
+        ops.linear(xn, [lw.q, lw.k, lw.v], ws, out=qkv)
+        write_kv_q8(w, qkv, fwd, T, cache.layer_q8(li), scratch, ws)
+    else:
+        kc, vc = cache.layer(li)
+        ops.qkv_rope(xn, lw.q, lw.k, lw.v, w.H, w.Hkv, w.hd, w.rope_cos, w.rope_sin, fwd.positions, fwd.slots, kc, vc,
+                     scratch.q[:T], ws, T=T)
+    attend(w, li, fwd, T, cache, scratch, ws, kv_bound)
     ops.linear(scratch.attn[:T], [lw.o], ws, epilogue=L.EPI_RESIDUAL, resid=resid)
     ops.rmsnorm(resid, lw.ln2, lw.eps2, xn)
     hid = scratch.hid(w.dtype, w.F, 0)[:T, : w.F]
@@ -346,14 +381,17 @@ def run_stack_folded(w: ModelWeights, layer_indices, pre_layer_bridges, pre_norm
             _bridge_folded(b, scratch, T, chain, xg, in_for(k), out_for(k + 1))
             k += 1
         lw = w.layers[li]
-        kc, vc = cache.layer(li)
-        chain.qkv(xg, lw.q, lw.k, lw.v, w.H, w.Hkv, w.hd, w.rope_cos, w.rope_sin, fwd.positions, fwd.slots, kc, vc,
-                  scratch.q[:T], in_norm=in_for(k))
-        chain.flush()
-        ops.tree_attention(scratch.q[:T], kc, vc, w.H, w.Hkv, w.hd, fwd.prefix_len, scratch.attn[:T], ws,
-                           spec_base=fwd.spec_base if fwd.use_mask else None,
-                           spec_mask=fwd.mask if fwd.use_mask else None, kv_bound=kv_bound, T=T,
-                           prefix_start=fwd.prefix_start)
+        if cache.quantized:
+            qkv = scratch.qkv(T)
+            chain.linear(xg, [lw.q, lw.k, lw.v], out=qkv, in_norm=in_for(k))
+            chain.flush()
+            write_kv_q8(w, qkv, fwd, T, cache.layer_q8(li), scratch, ws)
+        else:
+            kc, vc = cache.layer(li)
+            chain.qkv(xg, lw.q, lw.k, lw.v, w.H, w.Hkv, w.hd, w.rope_cos, w.rope_sin, fwd.positions, fwd.slots, kc, vc,
+                      scratch.q[:T], in_norm=in_for(k))
+            chain.flush()
+        attend(w, li, fwd, T, cache, scratch, ws, kv_bound)
         _residual_linear(w, scratch.attn[:T], lw.o, chain, resid, out_for(k + 1), T)
         hid = scratch.hid(w.dtype, w.F, 0)[:T, : w.F]
         chain.linear(xg, [lw.gate, lw.up], epilogue=L.EPI_SWIGLU, layout=L.SEG_PAIRS, out=hid, in_norm=in_for(k + 1))

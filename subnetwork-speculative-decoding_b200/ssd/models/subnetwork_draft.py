@@ -107,6 +107,7 @@ class SubnetworkDraftModel(nn.Module):
         self.place_bridges()
         self.vocab_ids: Optional[torch.Tensor] = None
         self._sub_head: Optional[torch.Tensor] = None
+        self.kv_dtype: Optional[str] = None  # of the caches new_cache makes (not in the reference)
         self._scratch: Optional[R.Scratch] = None
         self._ws: Optional[ops.Workspace] = None
 
@@ -144,8 +145,9 @@ class SubnetworkDraftModel(nn.Module):
         return self._sub_head if self._sub_head is not None else self.base.lm_head.weight
 
     def new_cache(self, max_length: int) -> KVCache:
-        """One slot per base layer, so the cache is shared with the target."""
-        return KVCache(self.num_base_layers, max_length)
+        """One slot per base layer, so the cache is shared with the target
+        (in ``self.kv_dtype``: None = the model's dtype, "e4m3" = 8-bit rows)."""
+        return KVCache(self.num_base_layers, max_length, self.kv_dtype)
 
     def pre_layer_bridge_modules(self) -> list:
         return [self.bridges[n] if n is not None else None for n in self._pre_layer_bridge]

@@ -90,3 +90,22 @@ def test_layer_wrapper_refuses_what_is_no_cache():
                  (k.transpose(0, 1), k.transpose(0, 1), s, s), (k, k, s, s)):  # the last: not on a CUDA device
         with pytest.raises(ValueError):
             ops.KVLayerQ8(*args)
+
+
+def test_kv_dtype_is_checked_where_it_is_given():
+    from ssd.cli import run
+    from ssd.config import SSDConfig
+    from ssd.engine.kv_cache import KVCache
+
+    raw = {"draft_layers": [0, 2], "model": {"kv_dtype": "e4m3"}}
+    assert SSDConfig.from_dict(raw).model.kv_dtype == "e4m3"
+    assert SSDConfig.from_dict({"draft_layers": [0, 2]}).model.kv_dtype is None
+    with pytest.raises(ValueError):
+        SSDConfig.from_dict({"draft_layers": [0, 2], "model": {"kv_dtype": "int8"}})
+    with pytest.raises(ValueError):
+        KVCache(1, 4, "fp8")
+    with pytest.raises(ValueError, match="CUDA"):  # no CPU form: its rows are written by the kernels
+        KVCache(1, 4, "e4m3").allocate(1, 16, torch.float32, "cpu")
+    assert run.parser().parse_args(["--synthetic", "c2", "--prompt", "a", "--kv-dtype", "e4m3"]).kv_dtype == "e4m3"
+    with pytest.raises(SystemExit):
+        run.parser().parse_args(["--synthetic", "c2", "--prompt", "a", "--kv-dtype", "int4"])
