@@ -561,6 +561,9 @@ __device__ __forceinline__ void q8_slice(const AttnQ8Meta& m, int split, int n_s
   first = who ? __shfl_sync(0xffffffffu, at, __ffs(who) - 1) : 0;
 }
 
+// Rows per token G: r / G for r < 2^20 / G as a product (0 <= r < 144, G <= 144).
+__device__ __forceinline__ int q8_token(int r, uint32_t inv_g) { return static_cast<int>((r * inv_g) >> 20); }
+
 // The CTA's query rows as two e4m3 terms per element, K-major rows of HD bytes
 // (by the softmax warps). A row is LPR lanes x 8 elements; a lane loads a batch
 // of rows (all it has, in every shape) before it converts the first.
@@ -571,6 +574,7 @@ __device__ __forceinline__ void q8_queries(const AttnQ8Args& a, AttnQ8Meta& m, u
   const int rows_per_pass = (blockDim.x - kQ8Helpers) / LPR;
   const bf16* qb = static_cast<const bf16*>(a.q);
   const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0;
+  const uint32_t inv_g = ((1u << 20) + a.G - 1) / a.G;
   const int l8 = threadIdx.x % LPR, r0 = (threadIdx.x - kQ8Helpers) / LPR;
   for (int rb = 0; rb < N; rb += rows_per_pass * BATCH) {
     uint32_t raw[BATCH][4];
@@ -579,7 +583,8 @@ __device__ __forceinline__ void q8_queries(const AttnQ8Args& a, AttnQ8Meta& m, u
       const int r = rb + u * rows_per_pass + r0;
       raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
       if (r < nrows) {
-        const bf16* src = qb + (int64_t)(t0 + r / a.G) * a.ldq + (int64_t)(h * a.G + r % a.G) * HD + l8 * 8;
+        const int tok = q8_token(r, inv_g);
+        const bf16* src = qb + (int64_t)(t0 + tok) * a.ldq + (int64_t)(h * a.G + r - tok * a.G) * HD + l8 * 8;
         if (wide) {
           const uint4 v = *reinterpret_cast<const uint4*>(src);
           raw[u][0] = v.x, raw[u][1] = v.y, raw[u][2] = v.z, raw[u][3] = v.w;
@@ -750,6 +755,69 @@ __device__ __forceinline__ float q8_warp_max(float v) {  // NaN gives way to num
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
+}
+
+// N floats of one lane, from L2 (another CTA of this launch may have written
+// them), zeros where `on` is false.
+template <int N>
+__device__ __forceinline__ void q8_ldcg(const float* p, bool on, float* v) {
+  if constexpr (N == 4) {
+    const float4 x = on ? __ldcg(reinterpret_cast<const float4*>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+    const float2 x = on ? __ldcg(reinterpret_cast<const float2*>(p)) : make_float2(0.f, 0.f);
+    v[0] = x.x, v[1] = x.y;
+  }
+}
+
+// Joins the key slices' records {O 2^(..M), M, l} of query row r of CTA column
+// `blk` of `blks` into dst: one warp, weights 2^(M_s - max M), in slice order. Slices that saw
+// nothing have l = 0 and no O.
+template <int HD>
+__device__ __noinline__ void q8_join_row(const float* part, int n_splits, int blk, int blks, int r, bf16* dst) {
+  constexpr int DPL = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const float* ml_part = part + (int64_t)blks * n_splits * kQ8MaxRows * HD;
+  const int64_t rec0 = (int64_t)blk * n_splits * kQ8MaxRows + r;
+  float top = -INFINITY;
+  for (int s = lane; s < n_splits; s += 32) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(ml_part + (rec0 + (int64_t)s * kQ8MaxRows) * 2));
+    if (ml.y != 0.f) top = fmaxf(top, ml.x);
+  }
+  top = warp_max(top);
+  float sum = 0.f, acc[DPL];
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
+  for (int s0 = 0; s0 < n_splits; s0 += 32) {
+    float w = 0.f, ls = 0.f;
+    if (s0 + lane < n_splits) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(ml_part + (rec0 + (int64_t)(s0 + lane) * kQ8MaxRows) * 2));
+      ls = ml.y;
+      w = ls != 0.f ? exp2f(ml.x - top) : 0.f;
+    }
+    sum += warp_sum(ls * w);
+    const uint32_t live = __ballot_sync(0xffffffffu, ls != 0.f);
+    const int n = min(32, n_splits - s0);
+    const float* o0 = part + (rec0 + (int64_t)s0 * kQ8MaxRows) * HD + lane * DPL;
+    for (int b = 0; b < n; b += 8) {  // eight records in flight
+      float v[8][DPL];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const bool on = b + u < n && ((live >> (b + u)) & 1u);
+        q8_ldcg<DPL>(o0 + (int64_t)(b + u) * kQ8MaxRows * HD, on, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float ws = __shfl_sync(0xffffffffu, w, (b + u) & 31);
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) acc[i] = fmaf(ws, v[u][i], acc[i]);
+      }
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  dst += lane * DPL;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) dst[i] = f2bf(acc[i] * inv);
 }
 
 template <int HD, int CH, int A>
@@ -1246,6 +1314,28 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         }
       }
     }
+    if constexpr (CH == 1) {  // few rows: the last slice to finish joins the column's records
+      if (a.n_splits > 1) {
+        __threadfence();
+        __syncwarp();
+        named_bar_sync(kQ8BarSoftmax, parties);
+        if (threadIdx.x == kQ8Helpers) {
+          const uint32_t before = atomicAdd(&a.counters[kAttnQ8CounterBase + blockIdx.x], 1u);
+          m.first = before == (uint32_t)(a.n_splits - 1);
+          if (m.first) a.counters[kAttnQ8CounterBase + blockIdx.x] = 0u;
+        }
+        __syncwarp();
+        named_bar_sync(kQ8BarSoftmax, parties);
+        if (m.first) {
+          __threadfence();
+          for (int r = sw; r < nrows; r += 4 * wgs) {
+            const int tok = r / a.G;
+            bf16* dst = static_cast<bf16*>(a.out) + (int64_t)(t0 + tok) * a.ldo + (int64_t)(h * a.G + r - tok * a.G) * HD;
+            q8_join_row<HD>(a.part, a.n_splits, blockIdx.x, gridDim.x, r, dst);
+          }
+        }
+      }
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -1256,56 +1346,23 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   }
 }
 
-// Joins the key slices' records {O 2^(..M), M, l} of one query row: one warp a
-// row, weights 2^(M_s - max M), in slice order. Slices that saw nothing have
-// l = 0 and no O.
+// The join as a launch of its own, one warp a row. With up to 16 query rows
+// the last CTA of a column joins its records itself, which the device hardly
+// notices (one token over 2k keys: 12.0 us against 12.1 replayed from a graph)
+// but the host does: 13.6 -> 11.9 us launched call by call, where the second
+// launch was the bound. With 48 rows over 32k keys, 18 slices, the one CTA
+// takes 1.8 us longer than the launch (39.7 us against 37.9).
 template <int HD>
 __global__ void __launch_bounds__(256) attn_q8_join_kernel(const AttnQ8Args a, const int tok_per_group) {
-  constexpr int DPL = HD / 32;
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = blockIdx.x % a.n_kv, group = a.tiles - 1 - blockIdx.x / a.n_kv;
   const int t0 = group * tok_per_group;
-  const int nrows = min(tok_per_group, a.T - t0) * a.G;
-  const int r = blockIdx.y * 8 + warp;
-  if (r >= nrows) return;
-  const float* o_part = a.part;
-  const float* ml_part = a.part + (int64_t)gridDim.x * a.n_splits * kQ8MaxRows * HD;
-  const int64_t rec0 = (int64_t)blockIdx.x * a.n_splits * kQ8MaxRows + r;
-  float top = -INFINITY;
-  for (int s = lane; s < a.n_splits; s += 32) {
-    const float2 ml = *reinterpret_cast<const float2*>(ml_part + (rec0 + (int64_t)s * kQ8MaxRows) * 2);
-    if (ml.y != 0.f) top = fmaxf(top, ml.x);
-  }
-  top = warp_max(top);
-  float sum = 0.f, acc[DPL];
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
-  for (int s0 = 0; s0 < a.n_splits; s0 += 32) {
-    float w = 0.f, ls = 0.f;
-    if (s0 + lane < a.n_splits) {
-      const float2 ml = *reinterpret_cast<const float2*>(ml_part + (rec0 + (int64_t)(s0 + lane) * kQ8MaxRows) * 2);
-      ls = ml.y;
-      w = ls != 0.f ? exp2f(ml.x - top) : 0.f;
-    }
-    sum += warp_sum(ls * w);
-    const uint32_t live = __ballot_sync(0xffffffffu, ls != 0.f);
-    const int n = min(32, a.n_splits - s0);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      if ((live >> s) & 1u) {
-        const float* o = o_part + (rec0 + (int64_t)(s0 + s) * kQ8MaxRows) * HD + lane * DPL;
-#pragma unroll
-        for (int i = 0; i < DPL; ++i) acc[i] = fmaf(ws, o[i], acc[i]);
-      }
-    }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  bf16* dst = static_cast<bf16*>(a.out) + (int64_t)(t0 + r / a.G) * a.ldo + (int64_t)(h * a.G + r % a.G) * HD + lane * DPL;
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) dst[i] = f2bf(acc[i] * inv);
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (r >= min(tok_per_group, a.T - t0) * a.G) return;
+  const int tok = r / a.G;
+  bf16* dst = static_cast<bf16*>(a.out) + (int64_t)(t0 + tok) * a.ldo + (int64_t)(h * a.G + r - tok * a.G) * HD;
+  q8_join_row<HD>(a.part, a.n_splits, blockIdx.x, gridDim.x, r, dst);
 }
 
 static int q8_tensor_map(const void* base, const SsdKvQ8& c, CUtensorMap* out) {
@@ -1348,6 +1405,7 @@ static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64
     if (!workspace || need > workspace_bytes)
       return fail(SSD_ERR_WORKSPACE, "ssd_tree_attention_q8: workspace too small (need %lld)", (long long)need);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+    a.counters = static_cast<uint32_t*>(workspace);
   }
   AttnQ8Maps maps;
   if (const int rc = q8_tensor_map(cache.k, cache, &maps.k)) return rc;
@@ -1369,7 +1427,7 @@ static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64
   int rc = launch_kernel("attn_q8_tc_kernel", kern, dim3((unsigned)blocks, (unsigned)splits),
                          dim3((unsigned)(kQ8Helpers + 128 * f.cg * f.sets)), smem, stream, 1u, 1u, maps, a, chunks, f.cg,
                          tpg, stages, shift);
-  if (rc || splits == 1) return rc;
+  if (rc || splits == 1 || chunks == 1) return rc;
   return launch_kernel("attn_q8_join_kernel", attn_q8_join_kernel<HD>,
                        dim3((unsigned)blocks, (unsigned)((tpg * a.G + 7) / 8)), dim3(256), 0, stream, 1u, 1u, a, tpg);
 }
