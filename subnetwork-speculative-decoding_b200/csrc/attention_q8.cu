@@ -1119,14 +1119,16 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       tc_fence_after();
       const uint32_t ts = tmem + buf * N + lane_base + col_base;
       if (part) q8_mask_scores(ts, vis + buf * N * 4, col_base, my_chunks, a.G, ntok, quarter, lane);
-      // t of every column and its maximum over the warp's keys. (With more than
-      // one chunk the registers do not hold t next to l: it is computed again
-      // below. The loop is rolled for the instruction cache.)
+      // t of every column and its maximum over the warp's keys. The registers
+      // hold one chunk's t next to l: the loop runs down to chunk 0, whose t stays
+      // for the weights below; the others' are computed again (all of them: 3 %
+      // longer). It is rolled for the instruction cache.
       float x[16];
+      q8_tmem_ld16(ts + (my_chunks - 1) * 16, x);
       named_bar_sync(1 + wg, 128);  // the other warps have read the last block's maxima
 #pragma unroll 1
-      for (int c = 0; c < my_chunks; ++c) {
-        q8_tmem_ld16(ts + c * 16, x);
+      for (int c = my_chunks - 1; c >= 0; --c) {
+        if (c + 1 < my_chunks) q8_tmem_ld16(ts + c * 16, x);
         q8_tmem_wait16(x);
         q8_scores(m.rowc + col_base + c * 16, x, ck, ev);
 #pragma unroll
@@ -1196,7 +1198,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         if (c < my_chunks) {
           const int col = col_base + c * 16;
           float* p = x;
-          if (!KEEP) {
+          if (c > 0) {
             q8_tmem_ld16(ts + c * 16, p);
             q8_tmem_wait16(p);
             q8_scores(m.rowc + col, p, ck, ev);
