@@ -314,18 +314,21 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 //   S^T [128 keys x N]  = K8 [128 x hd] Q^T          (K8: codes as stored)
 //   O^T [hd x N]       += V8^T [hd x 128] P'^T       (V8: codes as stored)
 // The cache's codes feed the tensor cores untouched (kind::f8f6f4); what they
-// multiply is split into two e4m3 terms: a bf16 query element has 8
+// multiply is split into two 8-bit terms: a bf16 query element has 8
 // significant bits, q = (hi + lo) 2^eq with hi its nearest e4m3 and lo the
-// exact rest, and P' = hi + lo keeps 7 .. 8 bits (hi truncated, lo rounded).
+// exact rest; of P' = hi + lo, hi is the nearest e5m2 and lo the rest in e4m3,
+// off by 2^-8 of P' at most from 2^-6 on, by 2^-3 down to 2^-14, by 2^-17 below.
+// (Both in e4m3 are as exact for large P', but flush all below 2^-10: beside a
+// key that holds 5/6 of the weight, 32768 others lost their share.)
 // Scales never touch the operands: a softmax thread owns one key (= TMEM
 // lane), so 2^ek is a factor of its scores and 2^ev an addend in its exponent,
 //   t = s log2 e + ev,  P' = 2^(t - M + kBias),  l += P' 2^-ev,
 // with M a whole number per row that scales O and l. A block's column maxima
 // (one warp reduction instruction per column and warp, joined in shared memory)
 // move M only when some t exceeds it by kGrow; then O and l shift by whole
-// powers of two. P' <= 2^(kBias + kGrow) < 448; its second term rounds at
-// 2^-10, i.e. 2^-13 of the weight at the reference, and l sums the unrounded
-// P' in fp32 per thread until the end.
+// powers of two. P' <= 2^(kBias + kGrow) keeps lo <= P' / 8 below 448. The
+// weight at the reference is above 2^(kBias - 1): what is flushed lies below
+// 2^-21 of it. l sums the unrounded P' in fp32 per thread until the end.
 //
 // A CTA = one KV head x up to 144 query rows (whole tokens) x one slice of the
 // key blocks that some row sees (a bitmap in shared memory: slot ranges of
@@ -345,8 +348,8 @@ constexpr int kQ8MaxRows = 144;       // query rows per CTA: three ring stages f
 constexpr int kQ8MaxStages = 6;
 constexpr int kQ8MapWords = 128;      // bitmap of key blocks (units of 2^unit_shift blocks)
 constexpr int kQ8Helpers = 128;       // threads of warps 0 .. 3
-constexpr float kQ8Bias = 3.f;
-constexpr float kQ8Grow = 5.75f;
+constexpr float kQ8Bias = 5.f;
+constexpr float kQ8Grow = 6.75f;
 constexpr float kQ8Unset = 1e30f;     // reference of a row that saw no key yet: every t exceeds it
 constexpr int kQ8BarSoftmax = 8, kQ8BarHelpers = 9;  // named barriers (1 .. 5: the warpgroups')
 
@@ -419,9 +422,9 @@ __device__ __forceinline__ uint64_t q8_desc(uint32_t lo, uint32_t hi) {
   asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
   return d;
 }
-// e4m3 A/B, fp32 D, M x N; mn: both operands MN-major.
-__host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool mn) {
-  return (1u << 4) | (mn ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
+// e4m3 A, e4m3 or e5m2 B, fp32 D, M x N; mn: both operands MN-major.
+__host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool mn, bool b_e5m2 = false) {
+  return (1u << 4) | (b_e5m2 ? 1u << 10 : 0u) | (mn ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 // mbar_wait that sleeps between polls, for the warps that run ahead of the
@@ -751,6 +754,32 @@ __device__ __forceinline__ void q8_scores(const float* rowc, float* x, float ck,
     x[j + 3] = fmaf(x[j + 3] * r.w, ck, ev);
   }
 }
+// Four weights as e5m2 codes (hi) plus e4m3 codes of the rest (lo). Through
+// fp16, whose upper byte is an e5m2 code: adding half a step and cutting the
+// lower byte off rounds to 3 significant bits. A NaN loses hi to the addition
+// and keeps lo.
+__device__ __forceinline__ void q8_split4(const float* p, uint32_t& hi, uint32_t& lo) {
+  const __half2 a = __floats2half2_rn(p[0], p[1]), b = __floats2half2_rn(p[2], p[3]);
+  uint32_t ab, bb;
+  memcpy(&ab, &a, 4);
+  memcpy(&bb, &b, 4);
+  ab = (ab + 0x00800080u) & 0xff00ff00u;
+  bb = (bb + 0x00800080u) & 0xff00ff00u;
+  __half2 ah, bh;
+  memcpy(&ah, &ab, 4);
+  memcpy(&bh, &bb, 4);
+  hi = __byte_perm(ab, bb, 0x7531);
+  const __half2 ar = __hsub2(a, ah), br = __hsub2(b, bh);
+  uint32_t x, y;
+  memcpy(&x, &ar, 4);
+  memcpy(&y, &br, 4);
+  asm("{\n\t.reg .b16 u, v;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 u, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 v, %2;\n\t"
+      "mov.b32 %0, {u, v};\n\t}"
+      : "=r"(lo)
+      : "r"(x), "r"(y));
+}
 __device__ __forceinline__ float q8_warp_max(float v) {  // NaN gives way to numbers, as in fmaxf
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -950,7 +979,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       // operand add to the low word.
       const bool leader = elect_one();
       if (nblocks > 0) {
-        const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true);
+        const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true), id_o5 = idesc_f8(128, N, true, true);
         const uint32_t rows_hi = q8_desc_hi(SBO, SW), p_hi = q8_desc_hi(atoms * 256, 6u);
         const uint32_t k_lo = q8_desc_lo(smem_u32(k_ring), 16), v_lo = q8_desc_lo(smem_u32(v_ring), 0);
         const uint32_t qh_lo = q8_desc_lo(smem_u32(q_hi), 16), ql_lo = q8_desc_lo(smem_u32(q_lo), 16);
@@ -997,7 +1026,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
 #pragma unroll
                 for (int kk = 0; kk < kQ8Keys / 32; ++kk)
                   umma_f8(d, q8_desc(v + kk * 2 * HD, rows_hi),
-                          q8_desc(pl + term * (p_bytes >> 4) + kk * (atoms * 64), p_hi), id_o,
+                          q8_desc(pl + term * (p_bytes >> 4) + kk * (atoms * 64), p_hi), term == 0 ? id_o5 : id_o,
                           (nP >= A || term > 0 || kk > 0) ? 1u : 0u);
               umma_commit(&m.p_free[pbuf]);
               umma_commit(&m.v_empty[sP]);
@@ -1208,16 +1237,12 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
           for (int j = 0; j < 4; ++j) {
             const float4 ref = *reinterpret_cast<const float4*>(my_ref + c * 16 + 4 * j);
             const float r[4] = {ref.x, ref.y, ref.z, ref.w};
-            float t4[4], r4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               p[4 * j + e] = q8_ex2(p[4 * j + e] + r[e]);
-              t4[e] = __uint_as_float(__float_as_uint(p[4 * j + e]) & 0xfff00000u);  // 4 significant bits
-              r4[e] = p[4 * j + e] - t4[e];
               l[c * 16 + 4 * j + e] = fmaf(p[4 * j + e], inv_v, l[c * 16 + 4 * j + e]);
             }
-            hi[j] = q8_pack4(t4[0], t4[1], t4[2], t4[3]);
-            lo[j] = q8_pack4(r4[0], r4[1], r4[2], r4[3]);
+            q8_split4(p + 4 * j, hi[j], lo[j]);
           }
           const uint32_t at = pb + (col >> 5) * 256 + ((((col >> 4) & 1u) ^ p_flip) << 4);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]),

@@ -378,6 +378,36 @@ def test_attention_extreme_values(ops, ws, dtype):
         check(out[t:t + 1], ref[t:t + 1], layer, see[t:t + 1], dtype)
 
 
+@pytest.mark.parametrize("slots,strong", [(4096, 10.0), (32768, 12.0)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_sink_beside_a_flat_tail(ops, ws, hd, slots, strong):
+    """One key with 5/6 of the weight, the rest spread evenly over thousands of
+    keys 2^-14 .. 2^-17 below it: the even part must not get lost. As many rows
+    as keep the keys of a head in one slice."""
+    H, T = 8, 1300
+    k = torch.zeros(H, slots, hd, device=DEV)
+    k[:, :, 1] = torch.linspace(0.25, 0.4375, H, device=DEV)[:, None]  # away from whole exponents
+    k[:, 77, 0] = strong
+    v = torch.ones_like(k)
+    v[:, 77] = -1
+    (kc, ks), (vc, vs) = quantise_ref(k), quantise_ref(v)
+    layer = ops.KVLayerQ8(kc, vc, ks, vs)
+    q = torch.zeros(T, H, hd, device=DEV)
+    q[:, :, :2] = math.sqrt(hd)
+    q = q.to(BF).view(T, H * hd)
+    plen = torch.full((T,), slots, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q)
+    ops.tree_attention_q8(q, layer, H, H, hd, plen, out, ws)
+    ws.check_status()
+    see = visible_ref(1, slots, plen[:1])
+    ref = attention_ref(q[:1], layer, H, see)
+    # all the rows are alike; the even keys hold (1 + ref) / 2 and are off by 2^-3 at most
+    # (the nearest of 3 significant bits, all to the same side), the strong one by 2^-8, the result by 2^-9
+    tol = (1 + ref.max().item()) / 2 * 2.0**-3 + 2.0**-8 + 2.0**-9
+    err = (out.double() - ref).abs().max().item()
+    assert err <= tol, (err, tol)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_attention_long_and_wide(ops, ws, dtype):
     """A cache beyond 2^31 code bytes per head set: the last slots of the last head."""
