@@ -4,6 +4,8 @@
 // the slots [prefix_start[t], prefix_len[t]) and slot spec_base + j for every
 // set bit j of token t's mask; a row that sees nothing gives zeros.
 //   s = (q . k8) 2^ek / sqrt(hd),  o = sum p 2^ev v8 / sum p,  p = 2^(s log2 e - m)
+#include <algorithm>
+
 #include "host.cuh"
 #include "kvq8.cuh"
 
@@ -1407,25 +1409,49 @@ static int q8_tensor_map(const void* base, const SsdKvQ8& c, CUtensorMap* out) {
   return SSD_OK;
 }
 
+// Query rows in groups of whole tokens, evenly, and key slices: one CTA per SM,
+// slices of at least two key blocks (one block each: 25 us against 19 for 33
+// tokens over 2k keys). Groups of up to 144 rows or of up to 128, whichever the
+// estimate takes for shorter: key blocks of a CTA, and two for the queries and
+// the results, x the measured time of one at that many columns, in 30 ns. (144
+// against 128 rows of 8 heads, us: 2048 tokens 125 and 114; 65 tokens over 2k
+// keys 23.7 and 20.4, 33 tokens 19.1 and 18.0, as SMs are left; 65 tokens over
+// 32k keys 100 and 102, as they fill two groups but not three; 33 tokens 64 and 68.)
+struct Q8Plan {
+  int tiles, tokens, chunks, key_blocks;
+  int64_t splits;
+};
+static Q8Plan q8_plan(int T, int G, int n_kv, int kv_end, int sms) {
+  constexpr int kCost[10] = {0, 18, 18, 35, 35, 60, 60, 71, 71, 87};
+  Q8Plan best{};
+  double least = 0.;
+  for (const int rows : {kQ8MaxRows, 128}) {
+    if (G > rows) break;
+    Q8Plan p;
+    const int fit = rows / G, few = (T + fit - 1) / fit;
+    p.tokens = (T + few - 1) / few;
+    p.tiles = (T + p.tokens - 1) / p.tokens;
+    p.chunks = (p.tokens * G + 15) / 16;
+    p.key_blocks = (kv_end + kQ8Keys - 1) / kQ8Keys;
+    const int64_t blocks = (int64_t)n_kv * p.tiles;
+    p.splits = std::max<int64_t>(1, std::min<int64_t>(sms / blocks, (p.key_blocks + 1) / 2));
+    const double waves = std::max(1., static_cast<double>(blocks) / sms);
+    const double cost = waves * static_cast<double>((p.key_blocks + p.splits - 1) / p.splits + 2) * kCost[p.chunks];
+    if (rows == kQ8MaxRows || cost < least) best = p, least = cost;
+  }
+  return best;
+}
+
 template <int HD>
 static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64_t workspace_bytes,
                      cudaStream_t stream) {
-  // Query rows in as few groups of whole tokens as fit the columns, evenly.
-  int tpg = kQ8MaxRows / a.G;
-  a.tiles = (a.T + tpg - 1) / tpg;
-  tpg = (a.T + a.tiles - 1) / a.tiles;
-  a.tiles = (a.T + tpg - 1) / tpg;
-  const int chunks = (tpg * a.G + 15) / 16;
-  const int64_t blocks = (int64_t)a.n_kv * a.tiles;
+  const Q8Plan plan = q8_plan(a.T, a.G, a.n_kv, a.kv_end, device_sms());
+  a.tiles = plan.tiles;
+  const int tpg = plan.tokens, chunks = plan.chunks, key_blocks = plan.key_blocks;
+  const int64_t blocks = (int64_t)a.n_kv * a.tiles, splits = plan.splits;
   if (blocks > INT32_MAX) return fail(SSD_ERR_UNSUPPORTED, "ssd_tree_attention_q8: too many row groups");
-  const int key_blocks = (a.kv_end + kQ8Keys - 1) / kQ8Keys;
   int shift = 0;
   while ((key_blocks >> shift) >= kQ8MapWords * 32) ++shift;
-  // One CTA per SM; slices of at least two key blocks.
-  int64_t splits = device_sms() / blocks;
-  const int64_t by_len = (key_blocks + 1) / 2;
-  if (splits > by_len) splits = by_len;
-  if (splits < 1) splits = 1;
   a.n_splits = (int)splits;
   if (splits > 1) {
     const int64_t need = kCounterBytes + blocks * splits * kQ8MaxRows * (HD + 2) * 4;
