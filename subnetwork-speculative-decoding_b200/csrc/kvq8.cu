@@ -14,7 +14,7 @@ struct WriteQ8Args {
   int n_q, n_kv, hd;  // n_q: query heads to rotate (0: cache write only)
   const float* cos;
   const float* sin;
-  int max_pos, rot, interleaved, wide_tables;  // wide_tables: a lane's 8 elements' entries are aligned float4s
+  int max_pos, rot, interleaved, kv_shift;
   const int32_t* positions;
   const int32_t* slots;
   uint8_t* kc;
@@ -28,39 +28,55 @@ struct WriteQ8Args {
   uint32_t* status;
 };
 
-// Eight elements as loaded, and their values.
+// Four elements as loaded or stored, and their values.
 template <typename T>
-struct Raw8 {
-  uint4 u[sizeof(T) / 2];
+struct Quad {
+  uint32_t w[sizeof(T)];
 };
-template <typename T, bool VEC>
-__device__ __forceinline__ Raw8<T> load8(const T* p) {
-  Raw8<T> r;
-  if constexpr (VEC) {
+template <typename T>
+__device__ __forceinline__ void quad_values(const Quad<T>& r, float* x) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else {
-    T* e = reinterpret_cast<T*>(r.u);
+  for (int i = 0; i < (int)sizeof(T); ++i) {
+    if constexpr (sizeof(T) == 2) {
+      x[2 * i] = __uint_as_float(r.w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+    } else {
+      x[i] = __uint_as_float(r.w[i]);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ Quad<T> quad_of(const float* x) {
+  Quad<T> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = p[i];
+  for (int i = 0; i < (int)sizeof(T); ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      r.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      r.w[i] = __float_as_uint(x[i]);
+    }
   }
   return r;
 }
 template <typename T>
-__device__ __forceinline__ void values8(const Raw8<T>& r, float* x) {
-#pragma unroll
-  for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-    const uint32_t w[4] = {r.u[h].x, r.u[h].y, r.u[h].z, r.u[h].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        x[4 * h + i] = __uint_as_float(w[i]);
-      }
-    }
+__device__ __forceinline__ Quad<T> load_quad(const T* p) {
+  Quad<T> r;
+  if constexpr (sizeof(T) == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    r.w[0] = u.x, r.w[1] = u.y;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
   }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_quad(T* p, const Quad<T>& r) {
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(p) = make_uint2(r.w[0], r.w[1]);
+  else
+    *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* p, const float* x) {
@@ -87,150 +103,167 @@ __device__ __forceinline__ void store8(T* p, const float* x) {
 //   (half layout) or (2i, 2i + 1) (interleaved), i < rot / 2; elements from
 //   rot on pass through. Products and sums round one by one, as the formula
 //   written out does, so that the codes do not depend on contraction.
-// Bound by bytes: 2 H hd + 2 Hkv hd elements and the codes of each token. A
-// row is LPR lanes x 8 elements (16-byte loads, 8-byte code stores), its amax
-// a shuffle reduction; a lane keeps its 8 cos / sin values for all rows of the
-// token, and re-reads the pair's other half from L1 instead of shuffling.
-template <typename T, int LPR, bool VEC>
-__global__ void __launch_bounds__(256) rope_kv_write_q8_kernel(const WriteQ8Args a) {
+// A row is LPR lanes x 4 pairs: a lane holds both elements of its pairs, so
+// that nothing is read twice and a row may be rotated in place, and keeps its
+// 4 cos / sin for all rows of the token. U passes of query rows and one of key
+// and value rows are loaded before the position is known. VEC: rows and tables
+// in aligned vectors (rot a multiple of 8).
+// Bound by bytes, 2 H hd + 2 Hkv hd elements and the codes of each token, once
+// the instructions are few (4096 tokens of 64 + 8 + 8 heads of 128, 178 MB, 27 us at
+// the copy rate: 32 us; lanes of 8 neighbouring elements that also read their
+// partners issued 1.6 times as many and took 47). Five CTAs per SM want 48
+// registers: U = 1 with six 34 us, U = 2 with four 34, U = 4 with two 48.
+template <typename T, int LPR, bool INTER, bool VEC>
+__global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 5 : 3) rope_kv_write_q8_kernel(const WriteQ8Args a) {
   constexpr int RPC = 256 / LPR;  // rows per pass of the CTA
+  constexpr int U = 2;
   pdl_wait();
   pdl_trigger();
   const int t = blockIdx.x;
-  const int l = threadIdx.x % LPR;
-  const int i0 = l * 8;
-  const bool on = i0 < a.hd;
+  const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+  const bool on = 8 * l < a.hd;
   const int half = a.rot >> 1;
   const int slot = a.slots[t];
   int pos = a.rot ? a.positions[t] : 0;
-  // Passes of RPC rows, U at a time, a batch's loads before its first use and
-  // the first batch's before the position is needed (one pass at a time waited
-  // out the memory latency for each; four cost occupancy: 66 and 85 us where
-  // two take 50, 4096 tokens of the 70B shape). A row's loads come before its
-  // stores: q_out may be q. Every lane of a warp runs the same passes.
-  constexpr int U = 2;
-  const int n_rows = a.n_q + 2 * a.n_kv, step = gridDim.y * RPC;
-  const bool turns = on && i0 < a.rot;
-  // the other halves of 8 elements are 8 contiguous, aligned elements
-  const bool vec_pair = VEC && !a.interleaved && (half & 7) == 0;
-  // (outside the rotated part a pair's other element is the element itself)
-  auto other = [&](int j) {
-    const int i = i0 + j;
-    return i >= a.rot ? i : a.interleaved ? i ^ 1 : i >= half ? i - half : i + half;
+  // Pair p = 4 l + j: elements (p, p + half), or (2p, 2p + 1) if interleaved or
+  // not rotated. VEC: the quads at lo and hi.
+  const bool split = !INTER && 4 * l < half;
+  const uint32_t lo = split ? 4 * l : 8 * l, hi = split ? half + 4 * l : 8 * l + 4;
+  auto first_of = [&](int p) { return !INTER && p < half ? p : 2 * p; };
+  auto second_of = [&](int p) { return !INTER && p < half ? p + half : 2 * p + 1; };
+  // x[0 .. 3], x[4 .. 7]: the quads, or without VEC the pairs' first and second elements
+  struct Raw {
+    Quad<T> q[2];
   };
-  Raw8<T> raw[U], pair[U];
-  auto load_batch = [&](int base) {
+  auto load = [&](const T* src, uint32_t at) {  // the row at element `at` of src
+    Raw r;
+    if constexpr (!VEC) {
+      T* e = reinterpret_cast<T*>(r.q);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = base + u * step + threadIdx.x / LPR;
-      if (r < n_rows && on) {
-        const int kind = r < a.n_q ? 0 : (r < a.n_q + a.n_kv ? 1 : 2);
-        const int head = kind == 0 ? r : (kind == 1 ? r - a.n_q : r - a.n_q - a.n_kv);
-        const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
-                       (int64_t)t * (kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv) + (int64_t)head * a.hd;
-        raw[u] = load8<T, VEC>(src + i0);
-        if (kind < 2 && turns && !a.interleaved) {
-          if (vec_pair) {
-            pair[u] = load8<T, VEC>(src + other(0));
-          } else {
-            T* e = reinterpret_cast<T*>(pair[u].u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = src[other(j)];
-          }
-        }
-      }
+      for (int j = 0; j < 4; ++j) e[j] = src[at + first_of(4 * l + j)], e[4 + j] = src[at + second_of(4 * l + j)];
+    } else if constexpr (INTER && sizeof(T) == 2) {
+      const uint4 w = *reinterpret_cast<const uint4*>(src + (at + lo));
+      r.q[0].w[0] = w.x, r.q[0].w[1] = w.y, r.q[1].w[0] = w.z, r.q[1].w[1] = w.w;
+    } else {
+      r.q[0] = load_quad(src + (at + lo));
+      r.q[1] = load_quad(src + (at + hi));
     }
+    return r;
   };
-  load_batch(blockIdx.y * RPC);
+  // Passes over the query rows and then the key and value rows (r < n_kv: key),
+  // pass i by the CTA i % gridDim.y (kv_shift: the query rows' passes % gridDim.y).
+  // The loads of the first ones come first.
+  const int step = gridDim.y * RPC;
+  int rq = blockIdx.y * RPC + sub;
+  int rkv = ((int)blockIdx.y - a.kv_shift + ((int)blockIdx.y < a.kv_shift ? (int)gridDim.y : 0)) * RPC + sub;
+  // (a token's own offsets are 32-bit: the entry point checks)
+  const T* q_src = static_cast<const T*>(a.q) + (int64_t)t * a.ldq;
+  T* q_dst = static_cast<T*>(a.q_out) + (int64_t)t * a.ldqo;
+  auto load_kv = [&](int r) {
+    const T* src = r < a.n_kv ? static_cast<const T*>(a.k) + (int64_t)t * a.ldk : static_cast<const T*>(a.v) + (int64_t)t * a.ldv;
+    return load(src, (r < a.n_kv ? r : r - a.n_kv) * a.hd);
+  };
+  Raw kv{}, q[U];
+  if (on && rkv < 2 * a.n_kv) kv = load_kv(rkv);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (on && rq + u * step < a.n_q) q[u] = load(q_src, (rq + u * step) * a.hd);
   const bool slot_ok = slot >= 0 && slot < a.max_slots;
   if (a.rot && (pos < 0 || pos >= a.max_pos)) {
     if (threadIdx.x == 0 && blockIdx.y == 0) report_error(a.status, kErrBadIndex);
     pos = 0;
   }
   if (!slot_ok && threadIdx.x == 0 && blockIdx.y == 0) report_error(a.status, kErrBadIndex);
-  // cos / sin of each of the lane's elements (sin signed: first of a pair -,
-  // second +)
-  const bool second = !a.interleaved && i0 >= half;  // (where a lane lies in one half)
-  float c[8], s[8];
-  if (turns && a.wide_tables) {
-    const float* ct = a.cos + (int64_t)pos * half + (a.interleaved ? i0 >> 1 : second ? i0 - half : i0);
-    const float* st = a.sin + (ct - a.cos);
-    const float4 c0 = *reinterpret_cast<const float4*>(ct), s0 = *reinterpret_cast<const float4*>(st);
-    if (a.interleaved) {
-      c[0] = c[1] = c0.x, c[2] = c[3] = c0.y, c[4] = c[5] = c0.z, c[6] = c[7] = c0.w;
-      s[0] = -s0.x, s[1] = s0.x, s[2] = -s0.y, s[3] = s0.y, s[4] = -s0.z, s[5] = s0.z, s[6] = -s0.w, s[7] = s0.w;
+  const bool turns = on && 4 * l < half;
+  float c[4] = {}, s[4] = {};
+  if (turns) {
+    const int64_t at = (int64_t)pos * half + 4 * l;
+    if constexpr (VEC) {
+      const float4 c4 = *reinterpret_cast<const float4*>(a.cos + at), s4 = *reinterpret_cast<const float4*>(a.sin + at);
+      c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
+      s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
     } else {
-      const float4 c1 = reinterpret_cast<const float4*>(ct)[1], s1 = reinterpret_cast<const float4*>(st)[1];
-      const float sg = second ? 1.f : -1.f;
-      c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
-      s[0] = sg * s0.x, s[1] = sg * s0.y, s[2] = sg * s0.z, s[3] = sg * s0.w;
-      s[4] = sg * s1.x, s[5] = sg * s1.y, s[6] = sg * s1.z, s[7] = sg * s1.w;
-    }
-  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = i0 + j;
-      c[j] = 1.f;
-      s[j] = 0.f;
-      if (turns && i < a.rot) {
-        const bool sec = a.interleaved ? (i & 1) : i >= half;
-        const int64_t f = (int64_t)pos * half + (a.interleaved ? i >> 1 : (sec ? i - half : i));
-        c[j] = a.cos[f];
-        s[j] = sec ? a.sin[f] : -a.sin[f];
-      }
+      for (int j = 0; j < 4; ++j)
+        if (4 * l + j < half) c[j] = a.cos[at + j], s[j] = a.sin[at + j];
     }
   }
-  for (int base = blockIdx.y * RPC; base < n_rows; base += U * step) {
-    __syncwarp();
+  auto values = [&](const Raw& r, bool turn, float* x) {
+    quad_values<T>(r.q[0], x);
+    quad_values<T>(r.q[1], x + 4);
+    if (!turn) return;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (base + u * step >= n_rows) break;  // uniform
-      const int r = base + u * step + threadIdx.x / LPR;
-      const bool live = r < n_rows;
-      const int kind = r < a.n_q ? 0 : (r < a.n_q + a.n_kv ? 1 : 2);
-      const int head = kind == 0 ? r : (kind == 1 ? r - a.n_q : r - a.n_q - a.n_kv);
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
-      if (live && on) {
-        values8<T>(raw[u], x);
-        if (kind < 2 && turns) {
-          float y[8];
-          if (a.interleaved) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
-          } else {
-            values8<T>(pair[u], y);
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (i0 + j < a.rot) x[j] = __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(y[j], s[j]));
-        }
-      }
-      if (kind == 0) {
-        if (live && on) store8<T, VEC>(static_cast<T*>(a.q_out) + (int64_t)t * a.ldqo + (int64_t)head * a.hd + i0, x);
-      }
-      if (__all_sync(0xffffffffu, kind == 0)) continue;
-      float amax = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float m = fabsf(x[j]);
-        amax = m <= 3.402823466e38f ? fmaxf(amax, m) : amax;  // Inf and NaN do not set the scale
-      }
-#pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      if (live && kind != 0 && slot_ok) {
-        const int byte = q8_scale_byte(amax);
-        const float inv = q8_inv_scale(byte);
-        if (on) {
-          uint8_t* dst = (kind == 1 ? a.kc : a.vc) + (int64_t)head * a.head_stride + (int64_t)slot * a.hd + i0;
-          *reinterpret_cast<uint2*>(dst) = make_uint2(q8_pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
-                                                      q8_pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv));
-        }
-        if (l == 0) (kind == 1 ? a.ks : a.vs)[(int64_t)head * a.scale_head_stride + slot] = static_cast<uint8_t>(byte);
+    for (int j = 0; j < 4; ++j) {
+      float& xa = VEC && INTER ? x[2 * j] : x[j];
+      float& xb = VEC && INTER ? x[2 * j + 1] : x[4 + j];
+      const float va = xa, vb = xb;
+      if (VEC || 4 * l + j < half) {
+        xa = __fsub_rn(__fmul_rn(va, c[j]), __fmul_rn(vb, s[j]));
+        xb = __fadd_rn(__fmul_rn(vb, c[j]), __fmul_rn(va, s[j]));
       }
     }
-    if (base + U * step < n_rows) load_batch(base + U * step);
+  };
+  while (rkv - sub < 2 * a.n_kv) {  // uniform
+    const bool live = on && rkv < 2 * a.n_kv, is_v = rkv >= a.n_kv;
+    const int head = is_v ? rkv - a.n_kv : rkv;
+    float x[8] = {};
+    if (live) values(kv, turns && !is_v, x);
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float m = fabsf(x[j]);
+      amax = m <= 3.402823466e38f ? fmaxf(amax, m) : amax;  // Inf and NaN do not set the scale
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (live && slot_ok) {
+      const int byte = q8_scale_byte(amax);
+      const float inv = q8_inv_scale(byte);
+      const uint32_t c0 = q8_pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+      const uint32_t c1 = q8_pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+      uint8_t* dst = (is_v ? a.vc : a.kc) + (int64_t)head * a.head_stride + (int64_t)slot * a.hd;
+      if constexpr (!VEC) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          dst[first_of(4 * l + j)] = static_cast<uint8_t>(c0 >> (8 * j));
+          dst[second_of(4 * l + j)] = static_cast<uint8_t>(c1 >> (8 * j));
+        }
+      } else if constexpr (INTER) {
+        *reinterpret_cast<uint2*>(dst + lo) = make_uint2(c0, c1);
+      } else {
+        *reinterpret_cast<uint32_t*>(dst + lo) = c0;
+        *reinterpret_cast<uint32_t*>(dst + hi) = c1;
+      }
+      if (l == 0) (is_v ? a.vs : a.ks)[(int64_t)head * a.scale_head_stride + slot] = static_cast<uint8_t>(byte);
+    }
+    rkv += step;
+    if (on && rkv < 2 * a.n_kv) kv = load_kv(rkv);
+  }
+  if (!on) return;
+  for (; rq < a.n_q; rq += U * step) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (rq + u * step >= a.n_q) break;
+      float x[8];
+      values(q[u], turns, x);
+      const uint32_t at = (rq + u * step) * a.hd;
+      if constexpr (!VEC) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          q_dst[at + first_of(4 * l + j)] = from_f32<T>(x[j]);
+          q_dst[at + second_of(4 * l + j)] = from_f32<T>(x[4 + j]);
+        }
+      } else {
+        const Quad<T> y0 = quad_of<T>(x), y1 = quad_of<T>(x + 4);
+        if constexpr (INTER && sizeof(T) == 2) {
+          *reinterpret_cast<uint4*>(q_dst + (at + lo)) = make_uint4(y0.w[0], y0.w[1], y1.w[0], y1.w[1]);
+        } else {
+          store_quad(q_dst + (at + lo), y0);
+          store_quad(q_dst + (at + hi), y1);
+        }
+      }
+      if (rq + (u + U) * step < a.n_q) q[u] = load(q_src, (rq + (u + U) * step) * a.hd);
+    }
   }
 }
 
@@ -361,25 +394,32 @@ int check_kv_q8(const SsdKvQ8* c, const char* who) {
   return SSD_OK;
 }
 
-template <typename T, bool VEC>
-int launch_write_q8(const WriteQ8Args& a, int64_t T_rows, cudaStream_t stream) {
+template <typename T, bool INTER, bool VEC>
+int launch_write_q8(WriteQ8Args& a, int64_t T_rows, cudaStream_t stream) {
   const int lanes = a.hd / 8;
-  const int rows = a.n_q + 2 * a.n_kv;
   auto go = [&](auto kern, int lpr) {
     // Few tokens: spread a token's rows over CTAs (one pass each) until the
     // SMs are covered; many tokens: one CTA walks all rows of its token and
     // reuses the cos / sin registers.
     const int rpc = 256 / lpr;
-    int64_t gy = (rows + rpc - 1) / rpc;
+    const int q_passes = (a.n_q + rpc - 1) / rpc;
+    int64_t gy = q_passes + (2 * a.n_kv + rpc - 1) / rpc;
     const int64_t cover = (2 * device_sms() + T_rows - 1) / T_rows;
     if (gy > cover) gy = cover;
+    a.kv_shift = (int)(q_passes % gy);
     return launch_kernel("rope_kv_write_q8_kernel", kern, dim3((unsigned)T_rows, (unsigned)gy), dim3(256), 0, stream,
                          1, 1, a);
   };
-  if (lanes <= 2) return go(rope_kv_write_q8_kernel<T, 2, VEC>, 2);
-  if (lanes <= 4) return go(rope_kv_write_q8_kernel<T, 4, VEC>, 4);
-  if (lanes <= 8) return go(rope_kv_write_q8_kernel<T, 8, VEC>, 8);
-  return go(rope_kv_write_q8_kernel<T, 16, VEC>, 16);
+  if (lanes <= 2) return go(rope_kv_write_q8_kernel<T, 2, INTER, VEC>, 2);
+  if (lanes <= 4) return go(rope_kv_write_q8_kernel<T, 4, INTER, VEC>, 4);
+  if (lanes <= 8) return go(rope_kv_write_q8_kernel<T, 8, INTER, VEC>, 8);
+  return go(rope_kv_write_q8_kernel<T, 16, INTER, VEC>, 16);
+}
+template <typename T>
+int launch_write_q8(WriteQ8Args& a, bool vec, int64_t T_rows, cudaStream_t stream) {
+  if (a.interleaved)
+    return vec ? launch_write_q8<T, true, true>(a, T_rows, stream) : launch_write_q8<T, true, false>(a, T_rows, stream);
+  return vec ? launch_write_q8<T, false, true>(a, T_rows, stream) : launch_write_q8<T, false, false>(a, T_rows, stream);
 }
 
 }  // namespace ssd
@@ -398,6 +438,8 @@ int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk,
   if (!k || !v || !slots) return fail(SSD_ERR_INVALID, "%s: NULL k, v or slots", who);
   if (q && (!q_out || n_heads <= 0)) return fail(SSD_ERR_INVALID, "%s: q needs q_out and n_heads", who);
   const int64_t hd = cache->head_dim;
+  if (n_heads * hd >= (1 << 30) || cache->n_kv_heads * hd >= (1 << 30))
+    return fail(SSD_ERR_UNSUPPORTED, "%s: rows too long", who);
   if (rot_dim < 0 || rot_dim > hd || (rot_dim & 1))
     return fail(SSD_ERR_INVALID, "%s: rot_dim must be even, 0 .. head_dim", who);
   if (rot_dim && (!rope_cos || !rope_sin || !positions || max_pos <= 0))
@@ -420,8 +462,6 @@ int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk,
   a.sin = rope_sin;
   a.max_pos = (int)(max_pos > INT32_MAX ? INT32_MAX : max_pos);
   a.rot = (int)rot_dim;
-  a.wide_tables = rot_dim % 16 == 0 && (reinterpret_cast<uintptr_t>(rope_cos) & 15) == 0 &&
-                  (reinterpret_cast<uintptr_t>(rope_sin) & 15) == 0;
   a.interleaved = interleaved ? 1 : 0;
   a.positions = positions;
   a.slots = slots;
@@ -436,11 +476,11 @@ int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk,
   a.ldqo = ldqo;
   a.status = status;
   const int64_t es = dtype == SSD_F32 ? 4 : 2;
-  const bool vec = aligned16(k, ldk * es) && aligned16(v, ldv * es) &&
+  const bool vec = rot_dim % 8 == 0 && aligned16(rope_cos, 0) && aligned16(rope_sin, 0) && aligned16(k, ldk * es) &&
+                   aligned16(v, ldv * es) &&
                    (!q || (aligned16(q, ldq * es) && aligned16(q_out, ldqo * es)));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == SSD_F32) return vec ? launch_write_q8<float, true>(a, T, s) : launch_write_q8<float, false>(a, T, s);
-  return vec ? launch_write_q8<bf16, true>(a, T, s) : launch_write_q8<bf16, false>(a, T, s);
+  return dtype == SSD_F32 ? launch_write_q8<float>(a, vec, T, s) : launch_write_q8<bf16>(a, vec, T, s);
 }
 
 int ssd_kv_read_q8(const SsdKvQ8* cache, const int32_t* slots, int64_t first, int64_t n, void* k_out, int64_t ldk,
