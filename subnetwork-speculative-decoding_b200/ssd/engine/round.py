@@ -20,6 +20,7 @@ round (ssd/engine/sampling.py) overrides the two head hooks, `_propose` and
 
 from __future__ import annotations
 
+import gc
 import math
 from typing import Optional
 
@@ -167,8 +168,16 @@ class _Decoder:
         g = torch.cuda.CUDAGraph()
         s = torch.cuda.Stream(device=self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
-        with torch.cuda.graph(g, stream=s):
-            fn()
+        # A graph of a dropped engine that the garbage collector destroys
+        # during a capture makes the capture fail.
+        collects = gc.isenabled()
+        gc.disable()
+        try:
+            with torch.cuda.graph(g, stream=s):
+                fn()
+        finally:
+            if collects:
+                gc.enable()
         torch.cuda.current_stream(self.device).wait_stream(s)
         return g
 

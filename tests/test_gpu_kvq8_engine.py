@@ -175,6 +175,44 @@ def test_a_change_of_kv_dtype_makes_a_new_engine(tiny):
     assert gen.generate(ids, 8, set()).tokens == plain and not gen.engine().cache.quantized
 
 
+def test_capture_outlives_the_graphs_of_dropped_engines(tiny):
+    """A captured graph in a reference cycle, collected while another engine
+    captures its own, does not disturb it."""
+    import gc
+
+    base, _ = tiny
+    ids = prompt(9, 128).to(DEV)
+    want = None
+    for litter in (False, True):
+        target = TargetRunner(base, kv_dtype="e4m3")
+        step = TargetStep(target, target.new_cache(64), 16)
+        step.prefill(ids)
+        if litter:
+            old, stream = [torch.cuda.CUDAGraph()], torch.cuda.Stream()
+            x = torch.zeros(8, device=DEV)
+            with torch.cuda.graph(old[0], stream=stream):
+                x += 1
+            real = step.step
+
+            def littered():
+                cycle = [old.pop()]
+                cycle.append(cycle)
+                del cycle
+                assert len([[] for _ in range(1000)]) == 1000  # enough to set a collection off
+                real()
+
+            step.step = littered
+        before = gc.get_threshold()
+        gc.set_threshold(10, 1, 1)
+        try:
+            step.run(6)
+        finally:
+            gc.set_threshold(*before)
+        torch.cuda.synchronize()
+        want = want or step.tokens()
+        assert step.tokens() == want
+
+
 def test_command_line_runs_over_the_8_bit_cache(capsys):
     from ssd.cli import run
 
