@@ -49,7 +49,10 @@ struct AttnQ8Args {
 // keys lane and lane + 32 (float4 reads, row pitch hd + 4 floats: conflict
 // free); outputs: a lane owns dims lane, lane + 32, ... Softmax statistics and
 // accumulators are fp32. Slices write (max, sum, acc) records; the last CTA of
-// a row tile merges them in slice order.
+// a row tile merges them in slice order. With few rows it is one block's chain
+// of latencies: 5 tokens of 32 + 8 heads of 64 over 160 keys take 20 us (31 with
+// slices of two blocks, integer divisions in the staging loops and a merge that
+// waits for each record in turn).
 constexpr int kSimtWarps = 8;
 constexpr int kSimtRows = 32;   // query rows per CTA
 constexpr int kSimtKeys = 64;   // keys per block
@@ -101,14 +104,15 @@ __global__ void __launch_bounds__(256) attn_q8_simt_kernel(const AttnQ8Args a) {
     atomicMin(&s_lo, (int)max(lo, (int64_t)0));
     atomicMax(&s_hi, (int)min(hi, (int64_t)a.kv_end));
   }
-  for (int i = threadIdx.x; i < kSimtRows * hd; i += blockDim.x) {
-    const int r = i / hd, d = i % hd;
-    float v = 0.f;
-    if (r < nq) {
-      const int qr = q0 + r;
-      v = to_f32<T>(static_cast<const T*>(a.q)[(int64_t)(qr / a.G) * a.ldq + (int64_t)(h * a.G + qr % a.G) * hd + d]);
+#pragma unroll
+  for (int r = warp; r < kSimtRows; r += kSimtWarps) {
+    const int qr = q0 + r, tok = qr / a.G;
+    const T* src = static_cast<const T*>(a.q) + (int64_t)tok * a.ldq + (int64_t)(h * a.G + qr - tok * a.G) * hd;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int d = lane + 32 * u;
+      if (d < hd) Qs[r * hd + d] = r < nq ? to_f32<T>(src[d]) * a.scale : 0.f;
     }
-    Qs[i] = v * a.scale;
   }
   __syncthreads();
   // the live range, cut into n_splits slices of whole key blocks
@@ -131,10 +135,11 @@ __global__ void __launch_bounds__(256) attn_q8_simt_kernel(const AttnQ8Args a) {
   const int cpr = hd >> 4;
   for (int kb = k_lo; kb < k_hi; kb += kSimtKeys) {
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * kSimtKeys * cpr; i += blockDim.x) {
-      const bool is_v = i >= kSimtKeys * cpr;
-      const int idx = is_v ? i - kSimtKeys * cpr : i;
-      const int j = idx / cpr, c = idx % cpr;
+#pragma unroll
+    for (int i = threadIdx.x; i < 2 * kSimtKeys * 8; i += 256) {  // 8 lanes a row, cpr of them with work
+      const bool is_v = i >= kSimtKeys * 8;
+      const int j = (i >> 3) & (kSimtKeys - 1), c = i & 7;
+      if (c >= cpr) continue;
       const int slot = kb + j;
       uint4 u = make_uint4(0, 0, 0, 0);
       float sc = 0.f;
@@ -158,6 +163,7 @@ __global__ void __launch_bounds__(256) attn_q8_simt_kernel(const AttnQ8Args a) {
     const float* k0 = Ks + lane * pitch;
     const float* k1 = k0 + 32 * pitch;
     const float* qw = Qs + warp * 4 * hd;
+#pragma unroll 4
     for (int d = 0; d < hd; d += 4) {
       const float4 x = *reinterpret_cast<const float4*>(k0 + d), y = *reinterpret_cast<const float4*>(k1 + d);
 #pragma unroll
@@ -195,16 +201,17 @@ __global__ void __launch_bounds__(256) attn_q8_simt_kernel(const AttnQ8Args a) {
       Ps[(warp * kSimtKeys + lane + 32) * 4 + i] = p1;
     }
     __syncwarp();
-    const int nk = min(kSimtKeys, k_hi - kb);
-    for (int j = 0; j < nk; ++j) {
+    // (keys past k_hi: P and V are zero)
+#pragma unroll 8
+    for (int j = 0; j < kSimtKeys; ++j) {
       const float4 p = *reinterpret_cast<const float4*>(Ps + (warp * kSimtKeys + j) * 4);
       // a key that no row of this warp sees adds nothing, whatever its value
-      if (p.x == 0.f && p.y == 0.f && p.z == 0.f && p.w == 0.f) continue;
+      const bool none = p.x == 0.f && p.y == 0.f && p.z == 0.f && p.w == 0.f;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int d = lane + 32 * u;
-        if (d < hd) {
-          const float v = Vs[j * pitch + d];
+        if (32 * u < hd) {  // uniform; lanes past hd read the pitch's padding or the next row and are not stored
+          const float v = none ? 0.f : Vs[j * pitch + d];
           acc[0][u] = fmaf(p.x, v, acc[0][u]);
           acc[1][u] = fmaf(p.y, v, acc[1][u]);
           acc[2][u] = fmaf(p.z, v, acc[2][u]);
@@ -254,23 +261,32 @@ __global__ void __launch_bounds__(256) attn_q8_simt_kernel(const AttnQ8Args a) {
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  const float* all = a.part + (int64_t)blockIdx.x * a.n_splits * kSimtRows * rec;
-  for (int i = 0; i < 4; ++i) {
-    const int r = warp * 4 + i;
-    if (r >= nq) continue;
+  // A warp joins a row: lane = slice for the weights, lane = dims for the sums.
+  const int64_t pitch_rec = (int64_t)kSimtRows * rec;
+  for (int r = warp; r < nq; r += kSimtWarps) {
+    const float* row = a.part + (int64_t)blockIdx.x * a.n_splits * pitch_rec + (int64_t)r * rec;
     float top = -INFINITY;
-    for (int sp = 0; sp < a.n_splits; ++sp) top = fmaxf(top, __ldcg(all + ((int64_t)sp * kSimtRows + r) * rec));
+    for (int sp = lane; sp < a.n_splits; sp += 32) top = fmaxf(top, __ldcg(row + sp * pitch_rec));
+    top = warp_max(top);
     float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int sp = 0; sp < a.n_splits; ++sp) {
-      const float* p = all + ((int64_t)sp * kSimtRows + r) * rec;
-      const float ls = __ldcg(p + 1), ms = __ldcg(p);
-      if (ls == 0.f) continue;
-      const float w = ms == -INFINITY ? 1.f : expf(ms - top);  // NaN scores: their sum is NaN, kept
-      sum = fmaf(ls, w, sum);
+    for (int s0 = 0; s0 < a.n_splits; s0 += 32) {
+      float ls = 0.f, w = 0.f;
+      if (s0 + lane < a.n_splits) {
+        const float ms = __ldcg(row + (s0 + lane) * pitch_rec);
+        ls = __ldcg(row + (s0 + lane) * pitch_rec + 1);
+        w = ls == 0.f ? 0.f : ms == -INFINITY ? 1.f : expf(ms - top);  // NaN scores: their sum is NaN, kept
+      }
+      sum += warp_sum(ls * w);
+      const uint32_t live = __ballot_sync(0xffffffffu, ls != 0.f);
+      const int n = min(32, a.n_splits - s0);
+#pragma unroll 4
+      for (int b = 0; b < n; ++b) {
+        const float ws = __shfl_sync(0xffffffffu, w, b);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int d = lane + 32 * u;
-        if (d < hd) o[u] = fmaf(__ldcg(p + 2 + d), w, o[u]);
+        for (int u = 0; u < 4; ++u) {
+          const int d = lane + 32 * u;
+          if (d < hd && ((live >> b) & 1u)) o[u] = fmaf(__ldcg(row + (s0 + b) * pitch_rec + 2 + d), ws, o[u]);
+        }
       }
     }
     store_row(r, o, sum);
@@ -282,9 +298,9 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
   a.tiles = (a.M + kSimtRows - 1) / kSimtRows;
   const int64_t blocks = (int64_t)a.n_kv * a.tiles;
   if (blocks > INT32_MAX) return fail(SSD_ERR_UNSUPPORTED, "ssd_tree_attention_q8: too many row tiles");
-  // Slices of at least 128 keys until the SMs hold two CTAs each.
+  // Slices of at least one key block until the SMs hold two CTAs each.
   int64_t splits = (2 * device_sms() + blocks - 1) / blocks;
-  const int64_t by_len = (a.kv_end + 127) / 128;
+  const int64_t by_len = (a.kv_end + kSimtKeys - 1) / kSimtKeys;
   if (splits > by_len) splits = by_len;
   if (splits < 1 || blocks > kAttnQ8MaxBlocks) splits = 1;
   a.n_splits = (int)splits;
