@@ -294,6 +294,16 @@ __global__ void __launch_bounds__(256) attn_q8_simt_kernel(const AttnQ8Args a) {
   if (threadIdx.x == 0) a.counters[kAttnQ8CounterBase + blockIdx.x] = 0u;
 }
 
+// Whether this is the current device's first call (a kernel's attributes are
+// set per device; setting them again is harmless). `seen`: a bit per device.
+static bool first_on_device(uint64_t& seen) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;
+  const bool first = !((seen >> dev) & 1u);
+  seen |= 1ull << dev;
+  return first;
+}
+
 static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
   a.tiles = (a.M + kSimtRows - 1) / kSimtRows;
   const int64_t blocks = (int64_t)a.n_kv * a.tiles;
@@ -311,17 +321,14 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
     a.counters = static_cast<uint32_t*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
   }
-  auto go = [&](auto kern, bool& set) {
-    if (!set) {
-      allow_max_dynamic_smem(kern);
-      set = true;
-    }
+  auto go = [&](auto kern, uint64_t& seen) {
+    if (first_on_device(seen)) allow_max_dynamic_smem(kern);
     return launch_kernel("attn_q8_simt_kernel", kern, dim3((unsigned)blocks, (unsigned)splits), dim3(256),
                          (size_t)simt_q8_smem(a.hd), stream, 1u, 1u, a);
   };
-  static bool set_f32 = false, set_bf16 = false;
-  if (dtype == SSD_F32) return go(attn_q8_simt_kernel<float>, set_f32);
-  return go(attn_q8_simt_kernel<bf16>, set_bf16);
+  static uint64_t seen_f32 = 0, seen_bf16 = 0;
+  if (dtype == SSD_F32) return go(attn_q8_simt_kernel<float>, seen_f32);
+  return go(attn_q8_simt_kernel<bf16>, seen_bf16);
 }
 
 // ------------------------------------------------------------ tensor cores
@@ -1487,11 +1494,9 @@ static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64
   typedef void (*Kern)(const AttnQ8Maps, const AttnQ8Args, int, int, int, int, int);
   const Kern kerns[5] = {attn_q8_tc_kernel<HD, 1, 4>, attn_q8_tc_kernel<HD, 2, 4>, attn_q8_tc_kernel<HD, 2, 2>,
                          attn_q8_tc_kernel<HD, 2, 1>, attn_q8_tc_kernel<HD, 3, 1>};
-  static bool set = false;
-  if (!set) {
+  static uint64_t seen = 0;
+  if (first_on_device(seen))
     for (Kern k : kerns) allow_max_dynamic_smem(k);
-    set = true;
-  }
   const Kern kern = kerns[f.ch == 3 ? 4 : f.sets == 4 ? f.ch - 1 : f.sets == 2 ? 2 : 3];
   int rc = launch_kernel("attn_q8_tc_kernel", kern, dim3((unsigned)blocks, (unsigned)splits),
                          dim3((unsigned)(kQ8Helpers + 128 * f.cg * f.sets)), smem, stream, 1u, 1u, maps, a, chunks, f.cg,

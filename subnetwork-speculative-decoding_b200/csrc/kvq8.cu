@@ -438,7 +438,7 @@ int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk,
   if (!k || !v || !slots) return fail(SSD_ERR_INVALID, "%s: NULL k, v or slots", who);
   if (q && (!q_out || n_heads <= 0)) return fail(SSD_ERR_INVALID, "%s: q needs q_out and n_heads", who);
   const int64_t hd = cache->head_dim;
-  if (n_heads * hd >= (1 << 30) || cache->n_kv_heads * hd >= (1 << 30))
+  if ((q && n_heads >= (1 << 30) / hd) || cache->n_kv_heads >= (1 << 30) / hd)
     return fail(SSD_ERR_UNSUPPORTED, "%s: rows too long", who);
   if (rot_dim < 0 || rot_dim > hd || (rot_dim & 1))
     return fail(SSD_ERR_INVALID, "%s: rot_dim must be even, 0 .. head_dim", who);

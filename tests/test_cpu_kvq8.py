@@ -65,7 +65,7 @@ BAD = [(write, dict(T=0), ValueError), (write, dict(k=None), ValueError), (write
        (write, dict(q_out=None), ValueError), (write, dict(H=0), ValueError), (write, dict(rot=-2), ValueError),
        (write, dict(rot=65), ValueError), (write, dict(rot=66), ValueError), (write, dict(cos=None), ValueError),
        (write, dict(pos=None), ValueError), (write, dict(max_pos=0), ValueError), (write, dict(dtype=7), L.SSDError),
-       (write, dict(ldq=511), ValueError), (write, dict(ldk=127), ValueError), (write, dict(ldqo=0), ValueError),
+       (write, dict(H=1 << 24, ldq=1 << 40, ldqo=1 << 40), L.SSDError), (write, dict(ldq=511), ValueError), (write, dict(ldk=127), ValueError), (write, dict(ldqo=0), ValueError),
        (read, dict(n=0), ValueError), (read, dict(k_out=None, v_out=None), ValueError), (read, dict(first=61), ValueError),
        (read, dict(first=-1), ValueError), (read, dict(ldk=64), ValueError), (read, dict(dtype=-1), L.SSDError),
        (attend, dict(T=0), ValueError), (attend, dict(H=7), ValueError), (attend, dict(H=0), ValueError),

@@ -134,6 +134,32 @@ def test_write_rotates_quantises_and_reads_back(ops, ws, dtype, T, H, Hkv, hd, r
         assert torch.equal(vo.double().view(T, Hkv, hd), value(layer.v[:, at], layer.v_scale[:, at]).transpose(0, 1))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,H,Hkv,hd,rot,inter", [(3, 8, 2, 128, 64, False), (600, 40, 40, 64, 24, False),
+                                                  (2, 70, 33, 64, 64, False), (400, 3, 20, 128, 128, True),
+                                                  (1, 1, 1, 16, 16, False), (150, 0, 37, 48, 32, False)])
+def test_write_partial_rotation_and_many_heads(ops, ws, dtype, T, H, Hkv, hd, rot, inter):
+    """Rotated parts that end inside a row, in vectors; more heads than a pass of
+    rows, over one block a token and over several; no query rows (H = 0)."""
+    layer = new_layer(ops, Hkv, T, hd)
+    q, k, v = (rand(T, max(n, 1) * hd, dtype=dtype, seed=s) for n, s in ((H, 20), (Hkv, 21), (Hkv, 22)))
+    cos, sin = tables(rot, 500)
+    pos = torch.randint(0, 500, (T,), device=DEV, dtype=torch.int32)
+    where = torch.randperm(T, device=DEV).to(torch.int32)
+    q_out = torch.empty_like(q) if H else None
+    ops.rope_kv_write_q8(q if H else None, k, v, H, Hkv, hd, cos, sin, pos, where, layer, q_out, ws, interleaved=inter)
+    ws.check_status()
+    if H:
+        want = rotate_ref(q.float().view(T, H, hd), cos, sin, pos, rot, inter)
+        assert torch.equal(q_out, want.reshape(T, -1).to(dtype))
+    at = where.long()
+    for x, codes, scale in ((rotate_ref(k.float().view(T, Hkv, hd), cos, sin, pos, rot, inter), layer.k, layer.k_scale),
+                            (v.float().view(T, Hkv, hd), layer.v, layer.v_scale)):
+        c, s = quantise_ref(x)
+        assert torch.equal(codes.view(torch.uint8)[:, at], c.view(torch.uint8).transpose(0, 1))
+        assert torch.equal(scale[:, at], s.transpose(0, 1))
+
+
 def test_write_borders_of_the_scale(ops, ws):
     """Zero rows, subnormals, the largest values, amax at and next to 448 * 2^e, Inf and NaN."""
     hd = 64
