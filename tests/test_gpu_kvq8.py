@@ -493,6 +493,38 @@ def test_attention_q_strides_streams_and_graphs(ops):
         w.check_status()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_two_graphs_share_a_workspace(ops, dtype):
+    """One token (joined by the last slice) and many, captured over one workspace
+    and replayed in turn; rows that start off alignment; the slices' counters end
+    at zero."""
+    H, Hkv, hd, slots = 32, 8, 128, 3000
+    layer = new_layer(ops, Hkv, slots, hd, seed=90)
+    ws = ops.Workspace(torch.device(DEV), max_rows=64, vocab=1)
+    calls, graphs = [], []
+    for T in (1, 33):
+        wide = rand(T, H * hd + 3, dtype=dtype, seed=91)
+        q, out = wide[:, 1:1 + H * hd], torch.zeros(T, H * hd + 1, dtype=dtype, device=DEV)[:, 1:]
+        plen = torch.randint(1, slots + 1, (T,), device=DEV, dtype=torch.int32)
+        calls.append((T, wide, q, plen, out))
+    side = torch.cuda.Stream()
+    for T, wide, q, plen, out in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            ops.tree_attention_q8(q, layer, H, Hkv, hd, plen, out, ws)
+        graphs.append(g)
+    for turn in range(3):
+        for (T, wide, q, plen, out), g in zip(calls, graphs):
+            wide.copy_(rand(*wide.shape, dtype=dtype, seed=92 + turn))
+            plen.copy_(torch.randint(0, slots + 1, (T,), device=DEV, dtype=torch.int32))
+            g.replay()
+        torch.cuda.synchronize()
+        for T, wide, q, plen, out in calls:
+            see = visible_ref(T, slots, plen)
+            check(out, attention_ref(q.contiguous(), layer, H, see), layer, see, dtype)
+    ws.check_status()
+
+
 def test_attention_is_deterministic(ops, ws):
     H, Hkv, hd, T, slots = 32, 8, 128, 33, 4000
     layer = new_layer(ops, Hkv, slots, hd, seed=90)
