@@ -379,7 +379,11 @@ constexpr float kQ8Unset = 1e30f;     // reference of a row that saw no key yet:
 constexpr int kQ8BarSoftmax = 8, kQ8BarHelpers = 9;  // named barriers (1 .. 5: the warpgroups')
 
 // Column chunks of 16 -> chunks per warpgroup, warpgroups that share a block,
-// sets of them that take blocks in turn.
+// sets of them that take blocks in turn: as many warpgroups as registers and
+// TMEM allow (up to four; three where l takes 48 registers), as sets where a
+// block's columns do not fill them. Measured over 32k keys of 8 heads, us: 32
+// rows a head {2, 1, 4} 31.6, {2, 1, 2} 32.2; 36 rows {2, 2, 2} 34, {2, 2, 1} 38, {3, 1, 1}
+// 45; 88 rows {2, 3, 1} 47, {3, 2, 1} 52; 120 rows {2, 4, 1} 57, {3, 3, 1} 61.
 struct Q8Shape {
   int ch, cg, sets;
 };
@@ -1434,7 +1438,10 @@ static int q8_tensor_map(const void* base, const SsdKvQ8& c, CUtensorMap* out) {
 
 // Query rows in groups of whole tokens, evenly, and key slices: one CTA per SM,
 // slices of at least two key blocks (one block each: 25 us against 19 for 33
-// tokens over 2k keys). Groups of up to 144 rows or of up to 128, whichever the
+// tokens over 2k keys), and no join at all for as many blocks as the warpgroup
+// sets, or one more, take side by side (one token over 350 slots 7.9 us in one
+// slice, 9.4 in two; 600 slots 9.2 and 10.0 in three; 1100 slots 11.5 and 10.2 in
+// five). Groups of up to 144 rows or of up to 128, whichever the
 // estimate takes for shorter: key blocks of a CTA, and two for the queries and
 // the results, x the measured time of one at that many columns, in 30 ns. (144
 // against 128 rows of 8 heads, us: 2048 tokens 125 and 114; 65 tokens over 2k
@@ -1457,7 +1464,9 @@ static Q8Plan q8_plan(int T, int G, int n_kv, int kv_end, int sms) {
     p.chunks = (p.tokens * G + 15) / 16;
     p.key_blocks = (kv_end + kQ8Keys - 1) / kQ8Keys;
     const int64_t blocks = (int64_t)n_kv * p.tiles;
-    p.splits = std::max<int64_t>(1, std::min<int64_t>(sms / blocks, (p.key_blocks + 1) / 2));
+    p.splits = p.key_blocks <= q8_shape(p.chunks).sets + 1
+                   ? 1
+                   : std::max<int64_t>(1, std::min<int64_t>(sms / blocks, (p.key_blocks + 1) / 2));
     const double waves = std::max(1., static_cast<double>(blocks) / sms);
     const double cost = waves * static_cast<double>((p.key_blocks + p.splits - 1) / p.splits + 2) * kCost[p.chunks];
     if (rows == kQ8MaxRows || cost < least) best = p, least = cost;
