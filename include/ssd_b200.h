@@ -256,7 +256,9 @@ int ssd_kv_read_q8(const SsdKvQ8* cache, const int32_t* slots, int64_t first, in
 
 /* ssd_tree_attention over the 8-bit cache: same rows, masks, slot ranges
  * (prefix_start and prefix_len per row, mask bits from spec_base, kv_bound)
- * and outputs (a row that sees nothing: zeros). dtype: of q and out. */
+ * and outputs (a row that sees nothing: zeros). dtype: of q and out. Slots
+ * that no row sees may hold anything. A NaN in a value row that some row sees
+ * makes that row NaN, and may make other rows of the call NaN (0 * NaN). */
 int ssd_tree_attention_q8(const void* q, int64_t ldq, int64_t T, int64_t n_heads, const SsdKvQ8* cache,
                           const int32_t* prefix_len, const int32_t* prefix_start, const int32_t* spec_base,
                           const uint64_t* spec_mask, int64_t mask_words, int64_t kv_bound, void* out, int64_t ldo,
