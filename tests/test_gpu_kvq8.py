@@ -404,6 +404,26 @@ def test_attention_extreme_values(ops, ws, dtype):
         check(out[t:t + 1], ref[t:t + 1], layer, see[t:t + 1], dtype)
 
 
+@pytest.mark.parametrize("T", [1, 9, 33, 300])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_weights_add_up_to_one(ops, ws, hd, T):
+    """Values of one everywhere give exactly one: with scores close together every
+    weight is held to 8 bits, and the sum that divides is that of the held ones
+    (fp32 sums of 1000 terms are off by less than 2^-14, half a bf16 step below one
+    is 2^-9)."""
+    H, Hkv, slots = 16, 4, 1000
+    k = rand(Hkv, slots, hd, seed=95, scale=0.25)
+    v = torch.ones_like(k)
+    (kc, ks), (vc, vs) = quantise_ref(k), quantise_ref(v)
+    layer = ops.KVLayerQ8(kc, vc, ks, vs)
+    q = rand(T, H * hd, dtype=BF, seed=96)
+    plen = torch.randint(1, slots + 1, (T,), device=DEV, dtype=torch.int32)
+    out = torch.zeros_like(q)
+    ops.tree_attention_q8(q, layer, H, Hkv, hd, plen, out, ws)
+    ws.check_status()
+    assert (out == 1).all()
+
+
 @pytest.mark.parametrize("slots,strong", [(4096, 10.0), (32768, 12.0)])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_attention_sink_beside_a_flat_tail(ops, ws, hd, slots, strong):
