@@ -1175,7 +1175,8 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       const bool part = m.part[buf];
       const uint32_t bytes = scales[buf * kQ8Keys + key];
       const float ck = q8_scale(max(bytes & 0xffu, 1u));  // (not 0: a masked score is -inf times this)
-      const int vb = max(static_cast<int>(bytes >> 8), kQ8MinScale);
+      // (inside the bytes ever written: an unseen slot's may be any, and 255 would make inv_v -Inf, 0 * Inf NaN)
+      const int vb = min(max(static_cast<int>(bytes >> 8), kQ8MinScale), kQ8MaxScale);
       const float ev = static_cast<float>(vb - 127), inv_v = q8_inv_scale(vb);
       tc_fence_after();
       const uint32_t ts = tmem + buf * N + lane_base + col_base;
