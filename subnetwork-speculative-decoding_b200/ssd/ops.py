@@ -406,8 +406,11 @@ def tree_attention_q8(q: torch.Tensor, layer: KVLayerQ8, n_heads: int, n_kv: int
 def kv_compact_q8(codes: torch.Tensor, scales: torch.Tensor, start, keep_slots, n_keep, max_keep: int,
                   ws: Optional[Workspace] = None) -> None:
     """kv_compact for an 8-bit cache: codes [L, 2, n_kv, max_slots, head_dim]
-    float8_e4m3fn, scales [L, 2, n_kv, max_slots] uint8 (ssd_kv_compact_q8)."""
+    float8_e4m3fn, scales [L, 2, n_kv, max_slots] uint8 (ssd_kv_compact_q8).
+    keep_slots holds max_keep entries at least; the first n_keep[0] count."""
     Ln, two, n_kv, slots, hd = codes.shape
+    if keep_slots.numel() < max_keep:  # n_keep is on the device: up to max_keep entries are read
+        raise ValueError(f"kv_compact_q8: keep_slots has {keep_slots.numel()} entries, max_keep is {max_keep}")
     dev, i32 = codes.get_device(), torch.int32
     if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8 or scales.shape != (Ln, two, n_kv, slots):
         raise ValueError("kv_compact_q8: codes float8_e4m3fn [L, 2, n_kv, max_slots, head_dim], scales uint8 "

@@ -1,0 +1,28 @@
+"""CPU tests of further refusals of the 8-bit key/value cache's entry points: calls
+that would have read or written out of place. Nothing is read or launched."""
+
+import pytest
+import torch
+
+from ssd import ops
+
+
+# ------------------------------------------------------------- compaction
+@pytest.mark.parametrize("entries,max_keep", [(1, 2), (0, 1), (3, 4), (31, 32)])
+def test_compact_refuses_a_keep_list_shorter_than_max_keep(entries, max_keep):
+    """How many entries count is on the device, so the list has to hold max_keep of them."""
+    codes = torch.zeros(1, 2, 1, 64, 16).to(torch.float8_e4m3fn)
+    scales = torch.zeros(1, 2, 1, 64, dtype=torch.uint8)
+    one = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="keep_slots has"):
+        ops.kv_compact_q8(codes, scales, one, torch.zeros(entries, dtype=torch.int32), one, max_keep)
+
+
+def test_compact_takes_keep_lists_of_max_keep_entries_and_more():
+    """As KVCache.keep_positions passes them (as many) and a round (one more)."""
+    codes = torch.zeros(1, 2, 1, 64, 16).to(torch.float8_e4m3fn)
+    scales = torch.zeros(1, 2, 1, 64, dtype=torch.uint8)
+    one = torch.zeros(1, dtype=torch.int32)
+    for entries, max_keep in ((4, 4), (6, 5)):
+        with pytest.raises(ValueError, match="CUDA"):  # past that check: these tensors are on the CPU
+            ops.kv_compact_q8(codes, scales, one, torch.zeros(entries, dtype=torch.int32), one, max_keep)
