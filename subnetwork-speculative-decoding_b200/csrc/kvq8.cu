@@ -1,6 +1,9 @@
 // The 8-bit key/value cache: rotary embedding + quantisation of new rows into
 // their slots, reading rows back, and moving an accepted path's rows.
 // (Row format: kvq8.cuh. The attention over it: attention_q8.cu.)
+#include <algorithm>
+#include <array>
+
 #include "host.cuh"
 #include "kvq8.cuh"
 
@@ -394,6 +397,19 @@ int check_kv_q8(const SsdKvQ8* c, const char* who) {
   return SSD_OK;
 }
 
+// Whether blocks of `extent` bytes at the given strides (of layers, K / V and
+// heads, in any order of size) overlap. A dimension of one has no stride.
+static bool blocks_overlap(int64_t extent, std::array<std::pair<int64_t, int64_t>, 3> dims) {
+  std::sort(dims.begin(), dims.end());
+  __int128 end = extent;  // bytes from the first block's start to the last one's end so far
+  for (const auto& [stride, n] : dims) {
+    if (n == 1) continue;
+    if (stride < end) return true;
+    end += static_cast<__int128>(stride) * (n - 1);
+  }
+  return false;
+}
+
 template <typename T, bool INTER, bool VEC>
 int launch_write_q8(WriteQ8Args& a, int64_t T_rows, cudaStream_t stream) {
   const int lanes = a.hd / 8;
@@ -540,6 +556,9 @@ int ssd_kv_compact_q8(void* codes, uint8_t* scales, int64_t n_layers, int64_t la
     return fail(SSD_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);
   if (!aligned16(codes, head_stride) || kv_stride % 16 || layer_stride % 16)
     return fail(SSD_ERR_INVALID, "%s: cache rows must be 16-byte aligned", who);
+  if (blocks_overlap(max_slots * head_dim, {{{layer_stride, n_layers}, {kv_stride, 2}, {head_stride, n_kv_heads}}}) ||
+      blocks_overlap(max_slots, {{{scale_layer_stride, n_layers}, {scale_kv_stride, 2}, {scale_head_stride, n_kv_heads}}}))
+    return fail(SSD_ERR_INVALID, "%s: cache layers, K and V or heads overlap", who);
   const int64_t total = n_layers * 2 * n_kv_heads * (head_dim / 16 + 1);
   return launch_kernel("kv_compact_q8_kernel", kv_compact_q8_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256),
                        0, static_cast<cudaStream_t>(stream), 1, 1, static_cast<uint8_t*>(codes), scales, n_layers,

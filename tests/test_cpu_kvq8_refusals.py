@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from ssd import ops
+from test_cpu_kvq8 import P, compact
 
 
 # ------------------------------------------------------------- compaction
@@ -26,3 +27,12 @@ def test_compact_takes_keep_lists_of_max_keep_entries_and_more():
     for entries, max_keep in ((4, 4), (6, 5)):
         with pytest.raises(ValueError, match="CUDA"):  # past that check: these tensors are on the CPU
             ops.kv_compact_q8(codes, scales, one, torch.zeros(entries, dtype=torch.int32), one, max_keep)
+
+
+@pytest.mark.parametrize("fields", [
+    dict(hs=4080), dict(hs=0), dict(hs=-4096), dict(kvs=4096), dict(kvs=8176), dict(kvs=0), dict(ls=8192), dict(ls=16368),
+    dict(shs=63), dict(shs=0), dict(skvs=64), dict(skvs=127), dict(sls=255), dict(sls=-256),
+    dict(hs=16384, kvs=4096, ls=8176)])
+def test_compact_refuses_layers_heads_or_keys_and_values_that_overlap(fields):
+    with pytest.raises(ValueError, match="overlap"):
+        compact(**fields)
