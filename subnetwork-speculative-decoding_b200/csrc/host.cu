@@ -47,17 +47,35 @@ bool pdl_enabled() {
   return on;
 }
 
+static TensorMapEncodeFn g_encode = nullptr;
+
+// The driver's encoder wants a context current on the calling thread, which a
+// thread that has made no runtime call yet does not have: it gets the current
+// device's then (a context the caller made current is left alone).
+static CUresult encode_in_context(CUtensorMap* map, CUtensorMapDataType type, cuuint32_t rank, void* base,
+                                  const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                                  const cuuint32_t* elem_strides, CUtensorMapInterleave interleave,
+                                  CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion,
+                                  CUtensorMapFloatOOBfill fill) {
+  const auto encode = [&] {
+    return g_encode(map, type, rank, base, dims, strides, box, elem_strides, interleave, swizzle, promotion, fill);
+  };
+  const CUresult r = encode();
+  int dev = 0;
+  if (r != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return r;
+  return encode();
+}
+
 TensorMapEncodeFn tensor_map_encoder() {
-  static TensorMapEncodeFn fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
         q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<TensorMapEncodeFn>(p);
+      g_encode = reinterpret_cast<TensorMapEncodeFn>(p);
   });
-  return fn;
+  return g_encode ? encode_in_context : nullptr;
 }
 
 }  // namespace ssd
