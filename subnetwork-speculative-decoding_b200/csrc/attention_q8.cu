@@ -5,6 +5,7 @@
 // set bit j of token t's mask; a row that sees nothing gives zeros.
 //   s = (q . k8) 2^ek / sqrt(hd),  o = sum p 2^ev v8 / sum p,  p = 2^(s log2 e - m)
 #include <algorithm>
+#include <atomic>
 
 #include "host.cuh"
 #include "kvq8.cuh"
@@ -294,14 +295,17 @@ __global__ void __launch_bounds__(256) attn_q8_simt_kernel(const AttnQ8Args a) {
   if (threadIdx.x == 0) a.counters[kAttnQ8CounterBase + blockIdx.x] = 0u;
 }
 
-// Whether this is the current device's first call (a kernel's attributes are
-// set per device; setting them again is harmless). `seen`: a bit per device.
-static bool first_on_device(uint64_t& seen) {
+// Lets the kernels use all shared memory, once per device (a kernel's attributes
+// are set per device). `done`: a bit per device, set only after the attributes
+// are: a call from another thread meanwhile sets them again, which is harmless,
+// and never launches without them.
+template <typename... Kerns>
+static void allow_smem_on_device(std::atomic<uint64_t>& done, Kerns... kerns) {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;
-  const bool first = !((seen >> dev) & 1u);
-  seen |= 1ull << dev;
-  return first;
+  const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+  if (known && (done.load(std::memory_order_acquire) >> dev & 1u)) return;
+  (allow_max_dynamic_smem(kerns), ...);
+  if (known) done.fetch_or(1ull << dev, std::memory_order_release);
 }
 
 static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
@@ -321,14 +325,14 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
     a.counters = static_cast<uint32_t*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
   }
-  auto go = [&](auto kern, uint64_t& seen) {
-    if (first_on_device(seen)) allow_max_dynamic_smem(kern);
+  auto go = [&](auto kern, std::atomic<uint64_t>& done) {
+    allow_smem_on_device(done, kern);
     return launch_kernel("attn_q8_simt_kernel", kern, dim3((unsigned)blocks, (unsigned)splits), dim3(256),
                          (size_t)simt_q8_smem(a.hd), stream, 1u, 1u, a);
   };
-  static uint64_t seen_f32 = 0, seen_bf16 = 0;
-  if (dtype == SSD_F32) return go(attn_q8_simt_kernel<float>, seen_f32);
-  return go(attn_q8_simt_kernel<bf16>, seen_bf16);
+  static std::atomic<uint64_t> done_f32{0}, done_bf16{0};
+  if (dtype == SSD_F32) return go(attn_q8_simt_kernel<float>, done_f32);
+  return go(attn_q8_simt_kernel<bf16>, done_bf16);
 }
 
 // ------------------------------------------------------------ tensor cores
@@ -1507,9 +1511,8 @@ static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64
   typedef void (*Kern)(const AttnQ8Maps, const AttnQ8Args, int, int, int, int, int);
   const Kern kerns[5] = {attn_q8_tc_kernel<HD, 1, 4>, attn_q8_tc_kernel<HD, 2, 4>, attn_q8_tc_kernel<HD, 2, 2>,
                          attn_q8_tc_kernel<HD, 2, 1>, attn_q8_tc_kernel<HD, 3, 1>};
-  static uint64_t seen = 0;
-  if (first_on_device(seen))
-    for (Kern k : kerns) allow_max_dynamic_smem(k);
+  static std::atomic<uint64_t> done{0};
+  allow_smem_on_device(done, kerns[0], kerns[1], kerns[2], kerns[3], kerns[4]);
   const Kern kern = kerns[f.ch == 3 ? 4 : f.sets == 4 ? f.ch - 1 : f.sets == 2 ? 2 : 3];
   int rc = launch_kernel("attn_q8_tc_kernel", kern, dim3((unsigned)blocks, (unsigned)splits),
                          dim3((unsigned)(kQ8Helpers + 128 * f.cg * f.sets)), smem, stream, 1u, 1u, maps, a, chunks, f.cg,
