@@ -343,24 +343,24 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 //   S^T [128 keys x N]  = K8 [128 x hd] Q^T          (K8: codes as stored)
 //   O^T [hd x N]       += V8^T [hd x 128] P'^T       (V8: codes as stored)
 // The cache's codes feed the tensor cores untouched (kind::f8f6f4); what they
-// multiply is split into two 8-bit terms: a bf16 query element has 8
-// significant bits, q = (hi + lo) 2^eq with hi its nearest e4m3 and lo the
-// exact rest; P' is cut to 8 bits and is hi + lo, hi its nearest e5m2 and lo the
-// rest in e4m3: exact from 2^-2 on, off by 2^-10 at most down to 2^-7, by 2^-3
-// of it down to 2^-14, by 2^-17 below. (Both in e4m3 flush all below 2^-10:
-// beside a key that holds 5/6 of the weight, 32768 others lost their share.)
+// multiply is split into 8-bit terms. A bf16 query element has 8 significant
+// bits: q = (hi + lo) 2^eq with hi its nearest e4m3 and lo the rest in e4m3:
+// exact down to 2^-10 of the row's largest, off by 2^-18 of that at most below.
+// P' is the sum of three e5m2 terms, 3 significant bits each, taken from its fp16
+// form (whose upper byte is an e5m2 code): off by 2^-10 of it at most, and by
+// 2^-16 below 2^-6. Two terms do not do: hi in e5m2 and the rest in e4m3 hold 8
+// bits down to 2^-2 only, and 3 where the rest vanishes, below 2^-7; the weights of
+// an even tail beside one strong key are then off by up to 1/8, all to the same side.
 // Scales never touch the operands: a softmax thread owns one key (= TMEM
 // lane), so 2^ek is a factor of its scores and 2^ev an addend in its exponent,
 //   t = s log2 e + ev,  P' = 2^(t - M + kBias),  l += P' 2^-ev,
 // with M a whole number per row that scales O and l. A block's column maxima
 // (one warp reduction instruction per column and warp, joined in shared memory)
 // move M only when some t exceeds it by kGrow; then O and l shift by whole
-// powers of two. P' <= 2^(kBias + kGrow) keeps lo <= P' / 8 below 448. The
-// weight at the reference is above 2^(kBias - 1): what is flushed lies below
-// 2^-21 of it. l sums the cut P' in fp32 per thread until the end: the weights
-// that reach O add up to one, and what the cut takes from all alike cancels (1.05
-// times the error of a bf16 result's rounding alone; 1.3 .. 1.7 with l of the uncut
-// P', in 98 % of the time).
+// powers of two. P' <= 2^(kBias + kGrow) = 2^15.75 stays below the largest e5m2.
+// The largest weight is above 2^(kBias - 1), so that what the last term cuts off
+// comes to at most n 2^-27 of it over n keys. l sums the uncut P' in fp32 per thread
+// until the end.
 //
 // A CTA = one KV head x up to 144 query rows (whole tokens) x one slice of the
 // key blocks that some row sees (a bitmap in shared memory: slot ranges of
@@ -380,8 +380,9 @@ constexpr int kQ8MaxRows = 144;       // query rows per CTA: three ring stages f
 constexpr int kQ8MaxStages = 6;
 constexpr int kQ8MapWords = 128;      // bitmap of key blocks (units of 2^unit_shift blocks)
 constexpr int kQ8Helpers = 128;       // threads of warps 0 .. 3
-constexpr float kQ8Bias = 5.f;
-constexpr float kQ8Grow = 6.75f;
+constexpr float kQ8Bias = 12.f;
+constexpr float kQ8Grow = 3.75f;
+constexpr int kQ8Terms = 3;           // e5m2 terms of a weight
 constexpr float kQ8Unset = 1e30f;     // reference of a row that saw no key yet: every t exceeds it
 constexpr int kQ8BarSoftmax = 8, kQ8BarHelpers = 9;  // named barriers (1 .. 5: the warpgroups')
 
@@ -391,14 +392,18 @@ constexpr int kQ8BarSoftmax = 8, kQ8BarHelpers = 9;  // named barriers (1 .. 5: 
 // block's columns do not fill them. Measured over 32k keys of 8 heads, us: 32
 // rows a head {2, 1, 4} 31.6, {2, 1, 2} 32.2; 36 rows {2, 2, 2} 34, {2, 2, 1} 38, {3, 1, 1}
 // 45; 88 rows {2, 3, 1} 47, {3, 2, 1} 52; 120 rows {2, 4, 1} 57, {3, 3, 1} 61.
+// P' has a buffer a set. A set alone of up to 96 columns has a second one: over few
+// key blocks the softmax would wait for the first values (33 rows over 2k keys,
+// 80 columns: 18.4 us with two, 20.0 with one). Of 128 columns one does: 2k prefill
+// 119.8 us with two, 117.6 with one, and with head_dim 64 40.0 and 39.2 for 1k.
 struct Q8Shape {
-  int ch, cg, sets;
+  int ch, cg, sets, p_buffers;
 };
 static Q8Shape q8_shape(int chunks) {
-  if (chunks <= 2) return {chunks, 1, 4};
-  if (chunks <= 4) return {2, 2, 2};
-  if (chunks <= 8) return {2, (chunks + 1) / 2, 1};
-  return {3, 3, 1};
+  if (chunks <= 2) return {chunks, 1, 4, 4};
+  if (chunks <= 4) return {2, 2, 2, 2};
+  if (chunks <= 8) return {2, (chunks + 1) / 2, 1, chunks <= 6 ? 2 : 1};
+  return {3, 3, 1, 1};
 }
 
 struct AttnQ8Maps {
@@ -420,9 +425,8 @@ struct AttnQ8Meta {
 };
 static_assert(sizeof(AttnQ8Meta) % 16 == 0, "the arrays behind it are read 16 bytes at a time");
 
-// S^T runs one block of each set ahead of the softmax; P' has a buffer a set.
+// S^T runs one block of each set ahead of the softmax.
 __host__ __device__ constexpr int q8_s_buffers(int sets) { return 2 * sets; }
-__host__ __device__ constexpr int q8_p_buffers(int sets) { return sets > 2 ? sets : 2; }
 __host__ __device__ constexpr int q8_p_bytes(int n) { return (n + 31) / 32 * 4096; }    // one term of one buffer
 // Behind AttnQ8Meta: per softmax warp and column {kBias - M, the last move as
 // a bf16 factor}, per warpgroup {column maxima of each warp's 32 keys}, and per
@@ -430,7 +434,7 @@ __host__ __device__ constexpr int q8_p_bytes(int n) { return (n + 31) / 32 * 409
 // per key, K's scale byte and V's in the high half}.
 static int q8_fixed_smem(int hd, int n, const Q8Shape& f) {
   const int state = 4 * f.cg * f.sets * 16 * f.ch;
-  return 1024 + 2 * n * hd + q8_p_buffers(f.sets) * 2 * q8_p_bytes(n) + (int)sizeof(AttnQ8Meta) + state * 10 +
+  return 1024 + 2 * n * hd + f.p_buffers * kQ8Terms * q8_p_bytes(n) + (int)sizeof(AttnQ8Meta) + state * 10 +
          q8_s_buffers(f.sets) * (n * 16 + kQ8Keys * 2);
 }
 
@@ -790,31 +794,31 @@ __device__ __forceinline__ void q8_scores(const float* rowc, float* x, float ck,
     x[j + 3] = fmaf(x[j + 3] * r.w, ck, ev);
   }
 }
-// Four weights as e5m2 codes (hi) plus e4m3 codes of the rest (lo). Through
-// fp16, whose upper byte is an e5m2 code: adding half a step and cutting the
-// lower byte off rounds to 3 significant bits. A NaN loses hi to the addition
-// and keeps lo.
-__device__ __forceinline__ void q8_split4(const float* p, uint32_t& hi, uint32_t& lo) {
-  const __half2 a = __floats2half2_rn(p[0], p[1]), b = __floats2half2_rn(p[2], p[3]);
-  uint32_t ab, bb;
-  memcpy(&ab, &a, 4);
-  memcpy(&bb, &b, 4);
-  ab = (ab + 0x00800080u) & 0xff00ff00u;
-  bb = (bb + 0x00800080u) & 0xff00ff00u;
-  __half2 ah, bh;
-  memcpy(&ah, &ab, 4);
-  memcpy(&bh, &bb, 4);
-  hi = __byte_perm(ab, bb, 0x7531);
-  const __half2 ar = __hsub2(a, ah), br = __hsub2(b, bh);
-  uint32_t x, y;
-  memcpy(&x, &ar, 4);
-  memcpy(&y, &br, 4);
-  asm("{\n\t.reg .b16 u, v;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 u, %1;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 v, %2;\n\t"
-      "mov.b32 %0, {u, v};\n\t}"
-      : "=r"(lo)
-      : "r"(x), "r"(y));
+// Four weights (>= 0) as three e5m2 codes each. Through fp16, whose upper byte
+// is an e5m2 code: hi is the weight cut to 3 significant bits, mid what is left
+// rounded to 3 (half a step added, the lower byte cut off), lo what is left then,
+// of either sign, cut to 3. Of the fp16's 11 bits that leaves a unit off at most.
+// A NaN stays in hi.
+__device__ __forceinline__ void q8_split4(const float* p, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const __half2 w[2] = {__floats2half2_rn(p[0], p[1]), __floats2half2_rn(p[2], p[3])};
+  uint32_t h[2], m[2], r[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t bits;
+    __half2 x;
+    memcpy(&bits, &w[i], 4);
+    h[i] = bits & 0xff00ff00u;
+    memcpy(&x, &h[i], 4);
+    const __half2 left = __hsub2(w[i], x);
+    memcpy(&bits, &left, 4);
+    m[i] = (bits + 0x00800080u) & 0xff00ff00u;
+    memcpy(&x, &m[i], 4);
+    const __half2 rest = __hsub2(left, x);
+    memcpy(&r[i], &rest, 4);
+  }
+  hi = __byte_perm(h[0], h[1], 0x7531);
+  mid = __byte_perm(m[0], m[1], 0x7531);
+  lo = __byte_perm(r[0], r[1], 0x7531);
 }
 __device__ __forceinline__ float q8_warp_max(float v) {  // NaN gives way to numbers, as in fmaxf
   float r;
@@ -885,15 +889,16 @@ __device__ __noinline__ void q8_join_row(const float* part, int n_splits, int bl
   for (int i = 0; i < DPL; ++i) dst[i] = f2bf(acc[i] * inv);
 }
 
-template <int HD, int CH, int A>
+template <int HD, int CH, int A, int PB>
 __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
     attn_q8_tc_kernel(const __grid_constant__ AttnQ8Maps maps, const AttnQ8Args a, const int n_chunks, const int cgs,
                       const int tok_per_group, const int stages, const int unit_shift) {
   constexpr int TILE = kQ8Keys * HD;              // bytes of a K or V block
   constexpr uint32_t SW = HD == 128 ? 2u : 4u;    // 128-byte or 64-byte swizzle: one atom row per cache row
   constexpr uint32_t SBO = 8 * HD;                // 8 rows of HD bytes
-  constexpr int SB = q8_s_buffers(A), PB = q8_p_buffers(A);  // powers of two
-  constexpr int SSH = SB == 8 ? 3 : SB == 4 ? 2 : 1, PSH = PB == 4 ? 2 : 1;
+  constexpr int SB = q8_s_buffers(A);             // S^T buffers; like PB, P' buffers, a power of two
+  constexpr int SSH = SB == 8 ? 3 : SB == 4 ? 2 : 1;
+  constexpr int PSH = PB == 4 ? 2 : PB == 2 ? 1 : 0;
   constexpr int WC = 16 * CH;                     // columns of a warpgroup
   constexpr bool KEEP = CH == 1;
   extern __shared__ uint8_t q8_smem_raw[];
@@ -904,8 +909,8 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
   const int wgs = cgs * A;
   uint8_t* k_ring = sm;
   uint8_t* v_ring = k_ring + stages * TILE;
-  uint8_t* p_buf = v_ring + stages * TILE;        // [PB][hi, lo][keys / 8][atoms][8 keys x 32 rows]
-  uint8_t* q_hi = p_buf + PB * 2 * p_bytes;       // [N][HD]
+  uint8_t* p_buf = v_ring + stages * TILE;        // [PB][terms][keys / 8][atoms][8 keys x 32 rows]
+  uint8_t* q_hi = p_buf + PB * kQ8Terms * p_bytes;       // [N][HD]
   uint8_t* q_lo = q_hi + N * HD;
   AttnQ8Meta& m = *reinterpret_cast<AttnQ8Meta*>(q_lo + N * HD);
   float* refs = reinterpret_cast<float*>(&m + 1);                            // [softmax warps][WC]
@@ -1011,11 +1016,13 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       // issues. The softmax frees S^T's buffer and fills P' at the same time, so
       // a fixed order loses nothing: S^T runs SB blocks ahead of O. (A loop
       // that polled for whichever is ready cost the softmax warps their
-      // instruction fetch: 20 % of the kernel.) Descriptors of later parts of an
-      // operand add to the low word.
+      // instruction fetch: 20 % of the kernel.) O(b) goes first: it frees the P'
+      // buffer, while S^T(b + SB) is wanted a whole softmax block later (the other
+      // way round: 65 rows over 32k keys 105 us against 101.5, 2k prefill 120.5
+      // against 117.6). Descriptors of later parts of an operand add to the low word.
       const bool leader = elect_one();
       if (nblocks > 0) {
-        const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true), id_o5 = idesc_f8(128, N, true, true);
+        const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true, true);
         const uint32_t rows_hi = q8_desc_hi(SBO, SW), p_hi = q8_desc_hi(atoms * 256, 6u);
         const uint32_t k_lo = q8_desc_lo(smem_u32(k_ring), 16), v_lo = q8_desc_lo(smem_u32(v_ring), 0);
         const uint32_t qh_lo = q8_desc_lo(smem_u32(q_hi), 16), ql_lo = q8_desc_lo(smem_u32(q_lo), 16);
@@ -1028,14 +1035,36 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
           const int nP = nS - SB, buf = nS & (SB - 1), pbuf = nP & (PB - 1);
           if (nP >= 0)
             ok = ok && mbar_wait(&m.s_free[buf], (nP >> SSH) & 1) && mbar_wait(&m.p_full[pbuf], (nP >> PSH) & 1);
-          if (nS < nblocks) ok = ok && mbar_wait(&m.k_full[sS], phS);
           if (__any_sync(0xffffffffu, !ok || *abort_flag)) {
             if (lane == 0) give_up();
             break;
           }
           tc_fence_after();
+          if (nP >= 0) {
+            ok = mbar_wait(&m.v_clean[sP], phP);
+            tc_fence_after();
+            if (leader && ok) {
+              // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
+              // M = 128 repeats the first (lanes 64 .. 127 are not read). P': MN-major, atoms of 32 rows x 8 keys.
+              const uint32_t d = tmem_o + (nP & (A - 1)) * N;
+              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + pbuf * (kQ8Terms * p_bytes >> 4);
+#pragma unroll
+              for (int term = 0; term < kQ8Terms; ++term)
+#pragma unroll
+                for (int kk = 0; kk < kQ8Keys / 32; ++kk)
+                  umma_f8(d, q8_desc(v + kk * 2 * HD, rows_hi),
+                          q8_desc(pl + term * (p_bytes >> 4) + kk * (atoms * 64), p_hi), id_o,
+                          (nP >= A || term > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&m.p_free[pbuf]);
+              umma_commit(&m.v_empty[sP]);
+            }
+            __syncwarp();
+            if (++sP == stages) sP = 0, phP ^= 1u;
+          }
           if (nS < nblocks) {
-            if (leader) {
+            ok = ok && mbar_wait(&m.k_full[sS], phS);
+            tc_fence_after();
+            if (leader && ok) {
               const uint32_t d = tmem + buf * N, k = k_lo + sS * (TILE >> 4);
 #pragma unroll
               for (int ks = 0; ks < HD / 32; ++ks)
@@ -1048,27 +1077,6 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
             }
             __syncwarp();
             if (++sS == stages) sS = 0, phS ^= 1u;
-          }
-          if (nP >= 0) {
-            ok = mbar_wait(&m.v_clean[sP], phP);
-            tc_fence_after();
-            if (leader) {
-              // V8^T: MN-major, one atom of HD head dims x 8 keys per 8 HD bytes; for HD = 64 the second half of
-              // M = 128 repeats the first (lanes 64 .. 127 are not read). P': MN-major, atoms of 32 rows x 8 keys.
-              const uint32_t d = tmem_o + (nP & (A - 1)) * N;
-              const uint32_t v = v_lo + sP * (TILE >> 4), pl = p_lo + pbuf * (2 * p_bytes >> 4);
-#pragma unroll
-              for (int term = 0; term < 2; ++term)
-#pragma unroll
-                for (int kk = 0; kk < kQ8Keys / 32; ++kk)
-                  umma_f8(d, q8_desc(v + kk * 2 * HD, rows_hi),
-                          q8_desc(pl + term * (p_bytes >> 4) + kk * (atoms * 64), p_hi), term == 0 ? id_o5 : id_o,
-                          (nP >= A || term > 0 || kk > 0) ? 1u : 0u);
-              umma_commit(&m.p_free[pbuf]);
-              umma_commit(&m.v_empty[sP]);
-            }
-            __syncwarp();
-            if (++sP == stages) sP = 0, phP ^= 1u;
           }
         }
       }
@@ -1258,7 +1266,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
         bad = true;
         give_up();
       }
-      const uint32_t pb = p_at + pbuf * 2 * p_bytes;
+      const uint32_t pb = p_at + pbuf * kQ8Terms * p_bytes;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (c < my_chunks) {
@@ -1269,25 +1277,24 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
             q8_tmem_wait16(p);
             q8_scores(m.rowc + col, p, ck, ev);
           }
-          uint32_t hi[4], lo[4];
+          uint32_t w[kQ8Terms][4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float4 ref = *reinterpret_cast<const float4*>(my_ref + c * 16 + 4 * j);
             const float r[4] = {ref.x, ref.y, ref.z, ref.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              p[4 * j + e] = __uint_as_float(__float_as_uint(q8_ex2(p[4 * j + e] + r[e])) & 0xffff0000u);
+              p[4 * j + e] = q8_ex2(p[4 * j + e] + r[e]);
               l[c * 16 + 4 * j + e] = fmaf(p[4 * j + e], inv_v, l[c * 16 + 4 * j + e]);
             }
-            q8_split4(p + 4 * j, hi[j], lo[j]);
+            q8_split4(p + 4 * j, w[0][j], w[1][j], w[2][j]);
           }
           const uint32_t at = pb + (col >> 5) * 256 + ((((col >> 4) & 1u) ^ p_flip) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]),
-                       "r"(hi[3])
-                       : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + p_bytes), "r"(lo[0]), "r"(lo[1]),
-                       "r"(lo[2]), "r"(lo[3])
-                       : "memory");
+#pragma unroll
+          for (int k = 0; k < kQ8Terms; ++k)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + k * p_bytes), "r"(w[k][0]), "r"(w[k][1]),
+                         "r"(w[k][2]), "r"(w[k][3])
+                         : "memory");
         }
       }
       fence_proxy_async_smem();
@@ -1509,11 +1516,11 @@ static int launch_tc(AttnQ8Args& a, const SsdKvQ8& cache, void* workspace, int64
   if (stages > kQ8MaxStages) stages = kQ8MaxStages;
   const size_t smem = (size_t)fixed + (size_t)stages * 2 * kQ8Keys * HD;
   typedef void (*Kern)(const AttnQ8Maps, const AttnQ8Args, int, int, int, int, int);
-  const Kern kerns[5] = {attn_q8_tc_kernel<HD, 1, 4>, attn_q8_tc_kernel<HD, 2, 4>, attn_q8_tc_kernel<HD, 2, 2>,
-                         attn_q8_tc_kernel<HD, 2, 1>, attn_q8_tc_kernel<HD, 3, 1>};
+  const Kern kerns[6] = {attn_q8_tc_kernel<HD, 1, 4, 4>, attn_q8_tc_kernel<HD, 2, 4, 4>, attn_q8_tc_kernel<HD, 2, 2, 2>,
+                         attn_q8_tc_kernel<HD, 2, 1, 2>, attn_q8_tc_kernel<HD, 2, 1, 1>, attn_q8_tc_kernel<HD, 3, 1, 1>};
   static std::atomic<uint64_t> done{0};
-  allow_smem_on_device(done, kerns[0], kerns[1], kerns[2], kerns[3], kerns[4]);
-  const Kern kern = kerns[f.ch == 3 ? 4 : f.sets == 4 ? f.ch - 1 : f.sets == 2 ? 2 : 3];
+  allow_smem_on_device(done, kerns[0], kerns[1], kerns[2], kerns[3], kerns[4], kerns[5]);
+  const Kern kern = kerns[f.ch == 3 ? 5 : f.sets == 4 ? f.ch - 1 : f.sets == 2 ? 2 : f.p_buffers == 2 ? 3 : 4];
   int rc = launch_kernel("attn_q8_tc_kernel", kern, dim3((unsigned)blocks, (unsigned)splits),
                          dim3((unsigned)(kQ8Helpers + 128 * f.cg * f.sets)), smem, stream, 1u, 1u, maps, a, chunks, f.cg,
                          tpg, stages, shift);
