@@ -344,8 +344,8 @@ static int launch_simt(AttnQ8Args& a, int dtype, void* workspace, int64_t worksp
 //   O^T [hd x N]       += V8^T [hd x 128] P'^T       (V8: codes as stored)
 // The cache's codes feed the tensor cores untouched (kind::f8f6f4); what they
 // multiply is split into 8-bit terms. A bf16 query element has 8 significant
-// bits: q = (hi + lo) 2^eq with hi its nearest e4m3 and lo the rest in e4m3:
-// exact down to 2^-10 of the row's largest, off by 2^-18 of that at most below.
+// bits: q = (hi + lo) 2^eq with hi its nearest e4m3 (4 bits) and lo the rest in
+// e5m2: exact down to 2^-13 of the row's largest, off by 2^-21 of that at most below.
 // P' is the sum of three e5m2 terms, 3 significant bits each, taken from its fp16
 // form (whose upper byte is an e5m2 code): off by 2^-10 of it at most, and by
 // 2^-16 below 2^-6. Two terms do not do: hi in e5m2 and the rest in e4m3 hold 8
@@ -607,7 +607,7 @@ __device__ __forceinline__ void q8_slice(const AttnQ8Meta& m, int split, int n_s
 // Rows per token G: r / G for r < 2^20 / G as a product (0 <= r < 144, G <= 144).
 __device__ __forceinline__ int q8_token(int r, uint32_t inv_g) { return static_cast<int>((r * inv_g) >> 20); }
 
-// The CTA's query rows as two e4m3 terms per element, K-major rows of HD bytes
+// The CTA's query rows as an e4m3 and an e5m2 term per element, K-major rows of HD bytes
 // (by the softmax warps). A row is LPR lanes x 8 elements; a lane loads a batch
 // of rows (all it has, in every shape) before it converts the first.
 template <int HD>
@@ -665,7 +665,8 @@ __device__ __forceinline__ void q8_queries(const AttnQ8Args& a, AttnQ8Meta& m, u
         const uint32_t c = q8_pack2(y0, y1);
         const float2 back = q8_unpack2(c);
         hi[e >> 2] |= c << (8 * (e & 3));
-        lo[e >> 2] |= q8_pack2(y0 - back.x, y1 - back.y) << (8 * (e & 3));
+        const float2 rest = make_float2(y0 - back.x, y1 - back.y);
+        lo[e >> 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(rest, __NV_SATFINITE, __NV_E5M2)) << (8 * (e & 3));
       }
       if (r < N) {
         const int sw = HD == 128 ? (r & 7) : ((r >> 1) & 3);  // swizzled place of the lane's 8 bytes
@@ -1022,7 +1023,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
       // against 117.6). Descriptors of later parts of an operand add to the low word.
       const bool leader = elect_one();
       if (nblocks > 0) {
-        const uint32_t id_s = idesc_f8(128, N, false), id_o = idesc_f8(128, N, true, true);
+        const uint32_t id_s = idesc_f8(128, N, false), id_s5 = idesc_f8(128, N, false, true), id_o = idesc_f8(128, N, true, true);
         const uint32_t rows_hi = q8_desc_hi(SBO, SW), p_hi = q8_desc_hi(atoms * 256, 6u);
         const uint32_t k_lo = q8_desc_lo(smem_u32(k_ring), 16), v_lo = q8_desc_lo(smem_u32(v_ring), 0);
         const uint32_t qh_lo = q8_desc_lo(smem_u32(q_hi), 16), ql_lo = q8_desc_lo(smem_u32(q_lo), 16);
@@ -1071,7 +1072,7 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
                 umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(qh_lo + ks * 2, rows_hi), id_s, ks > 0);
 #pragma unroll
               for (int ks = 0; ks < HD / 32; ++ks)
-                umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(ql_lo + ks * 2, rows_hi), id_s, 1u);
+                umma_f8(d, q8_desc(k + ks * 2, rows_hi), q8_desc(ql_lo + ks * 2, rows_hi), id_s5, 1u);
               umma_commit(&m.s_full[buf]);
               umma_commit(&m.k_empty[sS]);
             }

@@ -6,7 +6,8 @@ Tolerance of the latter (bf16, tensor cores). A weight is off by 2^-10 of itself
 at most plus 2^-12 for its fp16 form, and by 2^-27 of the largest where it is
 smaller than 2^-18 of that; with n keys the mean of the values is then off by
 (1.25 2^-10 + n 2^-27) max |v|, the bf16 result by 2^-9 of max |v| more. For
-n = 32768 that is 0.0034, below the 2^-8 = 0.0039 that is asked for.
+n = 32768 that is 0.0034, below the 2^-8 = 0.0039 that is asked for. Query elements
+down to 2^-13 of their row's largest are exact.
 """
 
 import math
@@ -112,3 +113,31 @@ def test_a_flat_tail_beside_a_sink_keeps_its_share(ops, ws, T, H, hd, slots, dee
             continue
         err = (out.double() - attention_ref(q, layer, H, see)).abs().max().item()
         assert err <= 2.0**-8, err
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("depth", [9, 11, 13])
+def test_small_query_elements_are_exact(ops, ws, hd, depth):
+    """Scores of about 20 from query elements 2^-depth of the row's largest, which
+    meets zeros in the keys: of two keys one adds up many such elements with all of
+    their 8 bits in use, the other a single one that is a power of two."""
+    T, S, root = 64, 20.0, math.sqrt(hd)
+    c = 2.0**-depth * (1 + (2 * torch.arange(T, device=DEV) + 1) / 128)  # the last of 8 bits is set
+    q = c[:, None].repeat(1, hd)
+    q[:, 0], q[:, 1] = 1.0, 2.0**-depth
+    k, v = torch.zeros(1, 2, hd, device=DEV), torch.ones(1, 2, hd, device=DEV)
+    k[0, 0, 2:] = S * root / ((hd - 2) * 1.4 * 2.0**-depth)
+    k[0, 1, 1] = S * root * 2.0**depth
+    v[0, 1] = -1
+    (kc, ks), (vc, vs) = quantise_ref(k), quantise_ref(v)
+    layer = ops.KVLayerQ8(kc, vc, ks, vs)
+    q = q.to(BF)
+    assert torch.equal(q[:, 2].float(), c)
+    plen = torch.full((T,), 2, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q)
+    ops.tree_attention_q8(q, layer, 1, 1, hd, plen, out, ws)
+    ws.check_status()
+    ref = attention_ref(q, layer, 1, visible_ref(T, 2, plen))
+    assert (ref.abs().amin() < 0.9)  # the keys compete in some rows
+    err = (out.double() - ref).abs().max().item()
+    assert err <= 2.0**-8, err
