@@ -220,7 +220,7 @@ int ssd_tree_attention(const void* q, int64_t ldq, int64_t T, int64_t n_heads, i
  * k, v: [n_kv_heads, max_slots, head_dim] codes, head stride `head_stride`
  * bytes (a multiple of 16, base 16-byte aligned); k_scale, v_scale:
  * [n_kv_heads, max_slots] bytes, head stride `scale_head_stride`. head_dim: a
- * multiple of 16 up to 128. */
+ * multiple of 16 up to 128; max_slots: up to 2^31 - 2^21. */
 typedef struct SsdKvQ8 {
   void* k;
   void* v;

@@ -389,7 +389,7 @@ int check_kv_q8(const SsdKvQ8* c, const char* who) {
     return fail(SSD_ERR_INVALID, "%s: bad cache shape", who);
   if (c->head_dim % 16 || c->head_dim > 128)
     return fail(SSD_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);
-  if (c->max_slots > (int64_t)INT32_MAX - 1024) return fail(SSD_ERR_UNSUPPORTED, "%s: too many slots", who);
+  if (c->max_slots > kQ8MaxSlots) return fail(SSD_ERR_UNSUPPORTED, "%s: too many slots", who);
   if (c->head_stride < c->max_slots * c->head_dim || c->scale_head_stride < c->max_slots)
     return fail(SSD_ERR_INVALID, "%s: cache heads overlap", who);
   if (!aligned16(c->k, c->head_stride) || !aligned16(c->v, c->head_stride))
@@ -550,7 +550,7 @@ int ssd_kv_compact_q8(void* codes, uint8_t* scales, int64_t n_layers, int64_t la
   const char* who = "ssd_kv_compact_q8";
   if (max_keep <= 0 || max_keep > 32) return fail(SSD_ERR_UNSUPPORTED, "%s: max_keep must be 1..32", who);
   if (!codes || !scales || !start || !keep_slots || !n_keep) return fail(SSD_ERR_INVALID, "%s: NULL argument", who);
-  if (n_layers <= 0 || n_kv_heads <= 0 || max_slots <= 0 || max_slots > INT32_MAX - 1024)
+  if (n_layers <= 0 || n_kv_heads <= 0 || max_slots <= 0 || max_slots > kQ8MaxSlots)
     return fail(SSD_ERR_INVALID, "%s: bad cache shape", who);
   if (head_dim <= 0 || head_dim % 16 || head_dim > 128)
     return fail(SSD_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);

@@ -18,6 +18,9 @@ namespace ssd {
 
 constexpr int kQ8MinScale = 127 - 40;   // smallest scale byte written
 constexpr int kQ8MaxScale = 127 + 119;  // largest
+// Slots of a cache: attention rounds its slot range up to whole units of key
+// blocks (2^19 slots at this length), which have to stay below 2^31 too.
+constexpr int64_t kQ8MaxSlots = (1ll << 31) - (1 << 21);
 
 // Scale byte of a row with the given amax (finite, >= 0). 448 = 1.75 * 2^8:
 // with amax = 1.m * 2^x, e = x - 8 up to m = 0.75 and x - 7 above; adding

@@ -4,8 +4,9 @@ that would have read or written out of place. Nothing is read or launched."""
 import pytest
 import torch
 
+from ssd import _lib as L
 from ssd import ops
-from test_cpu_kvq8 import P, compact
+from test_cpu_kvq8 import attend, cache, compact, read, write
 
 
 # ------------------------------------------------------------- compaction
@@ -36,3 +37,31 @@ def test_compact_takes_keep_lists_of_max_keep_entries_and_more():
 def test_compact_refuses_layers_heads_or_keys_and_values_that_overlap(fields):
     with pytest.raises(ValueError, match="overlap"):
         compact(**fields)
+
+
+# ----------------------------------------------------------- longest cache
+LONGEST = 2**31 - 2**21
+
+
+@pytest.mark.parametrize("call", [write, read, attend])
+@pytest.mark.parametrize("slots", [LONGEST + 1, 2**31 - 2**20, 2**31 - 1024 - 1])
+def test_caches_whose_rounded_slots_pass_32_bits_are_refused(call, slots):
+    with pytest.raises(L.SSDError, match="too many slots"):
+        call(cache(max_slots=slots, head_stride=slots * 64, scale_head_stride=slots))
+
+
+def test_compaction_of_such_a_cache_is_refused():
+    n = LONGEST + 1
+    with pytest.raises(ValueError, match="cache shape"):
+        compact(slots=n, hs=64 * n, kvs=2 * 64 * n, ls=4 * 64 * n, shs=n, skvs=2 * n, sls=4 * n)
+
+
+def test_the_longest_cache_fits_32_bits_rounded_up():
+    """The attention kernel's units, restated: as many key blocks of 128 slots as
+    leave at most 4096 units; its last block's end is a 32-bit number."""
+    for slots, fits in ((LONGEST, True), (2**31 - 1024 - 1, False)):
+        blocks, shift = (slots + 127) // 128, 0
+        while (blocks >> shift) >= 4096:
+            shift += 1
+        units = (blocks + (1 << shift) - 1) >> shift
+        assert ((units << shift) * 128 <= 2**31 - 1) == fits
