@@ -505,7 +505,7 @@ int ssd_kv_read_q8(const SsdKvQ8* cache, const int32_t* slots, int64_t first, in
   if (const int rc = check_kv_q8(cache, who)) return rc;
   if (n <= 0) return fail(SSD_ERR_INVALID, "%s: n must be positive", who);
   if (!k_out && !v_out) return fail(SSD_ERR_INVALID, "%s: NULL k_out and v_out", who);
-  if (!slots && (first < 0 || first + n > cache->max_slots))
+  if (!slots && (first < 0 || first > cache->max_slots || n > cache->max_slots - first))
     return fail(SSD_ERR_INVALID, "%s: slots outside the cache", who);
   if (dtype != SSD_F32 && dtype != SSD_BF16) return fail(SSD_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   const int64_t width = cache->n_kv_heads * cache->head_dim;

@@ -65,3 +65,10 @@ def test_the_longest_cache_fits_32_bits_rounded_up():
             shift += 1
         units = (blocks + (1 << shift) - 1) >> shift
         assert ((units << shift) * 128 <= 2**31 - 1) == fits
+
+
+# ---------------------------------------------------------------- reading
+@pytest.mark.parametrize("first,n", [(2**63 - 1, 4), (2**63 - 4, 64), (1, 2**63 - 1), (65, 1), (64, 1), (0, 65)])
+def test_a_read_range_that_wraps_around_is_refused(first, n):
+    with pytest.raises(ValueError, match="outside the cache"):
+        read(first=first, n=n)
