@@ -15,6 +15,7 @@ import math
 import pytest
 import torch
 
+import kvq8_cases
 from test_gpu_kvq8 import BF, DEV, F32, attention_ref, check, new_layer, quantise_ref, rand, visible_ref
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +142,23 @@ def test_small_query_elements_are_exact(ops, ws, hd, depth):
     assert (ref.abs().amin() < 0.9)  # the keys compete in some rows
     err = (out.double() - ref).abs().max().item()
     assert err <= 2.0**-8, err
+
+
+# -------------------------------------------------------------- visibility
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("args", kvq8_cases.CASES, ids=lambda a: "-".join(map(str, a)))
+def test_every_slot_counts(ops, ws, dtype, args):
+    """Inputs in which one slot too many or too few shows (test_cpu_kvq8_visibility.py),
+    against the 64-bit result, channel by channel."""
+    c = kvq8_cases.case(*args, DEV)
+    H, Hkv, hd, T = c["H"], c["Hkv"], c["hd"], c["T"]
+    layer = ops.KVLayerQ8(c["k"], c["v"], c["ks"], c["vs"])
+    q = c["q"].to(dtype)
+    out = torch.full((T, H * hd), math.nan, dtype=dtype, device=DEV)
+    ops.tree_attention_q8(q, layer, H, Hkv, hd, c["len"], out, ws, prefix_start=c["start"], spec_mask=c["mask"],
+                          spec_base=None if c["base"] is None else torch.tensor([c["base"]], dtype=torch.int32, device=DEV),
+                          kv_bound=c["bound"])
+    ws.check_status()
+    ref = kvq8_cases.attention(c, q, kvq8_cases.visible(c))
+    err = ((out.double().view(T, H, hd) - ref).abs() / ref.abs().clamp(min=2.0**-40)).amax().item()
+    assert err <= kvq8_cases.TOL, err
