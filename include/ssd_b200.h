@@ -241,7 +241,10 @@ typedef struct SsdKvQ8 {
  * which carry any frequency scaling: pairs (i, i + rot_dim/2), or (2i, 2i+1)
  * if `interleaved`. q / k / v: row strides in elements, heads contiguous. The
  * slots of one call are distinct. A slot outside the cache is not written and
- * a position outside the tables is taken as 0; either sets status bit 2. */
+ * a position outside the tables is taken as 0; either sets status bit 2.
+ * dtype: of q, k, v and q_out; SSD_BF16 | SSD_ROWS_F32: fp32 rows q, k, v (a
+ * projection's accumulators, rounded once) and a bf16 q_out (not q itself). */
+enum { SSD_ROWS_F32 = 16 };
 int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t T,
                          int64_t n_heads, const float* rope_cos, const float* rope_sin, int64_t max_pos,
                          int64_t rot_dim, int interleaved, const int32_t* positions, const int32_t* slots,

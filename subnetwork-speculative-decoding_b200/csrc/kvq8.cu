@@ -116,7 +116,9 @@ __device__ __forceinline__ void store8(T* p, const float* x) {
 // the copy rate: 32 us; lanes of 8 neighbouring elements that also read their
 // partners issued 1.6 times as many and took 47). Five CTAs per SM want 48
 // registers: U = 1 with six 34 us, U = 2 with four 34, U = 4 with two 48.
-template <typename T, int LPR, bool INTER, bool VEC>
+// T: of the rows. TO: of q_out, T or bf16 of fp32 rows (a projection's accumulators:
+// the rotated query is rounded once).
+template <typename T, typename TO, int LPR, bool INTER, bool VEC>
 __global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 5 : 3) rope_kv_write_q8_kernel(const WriteQ8Args a) {
   constexpr int RPC = 256 / LPR;  // rows per pass of the CTA
   constexpr int U = 2;
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 5 : 3) rope_kv_wr
   int rkv = ((int)blockIdx.y - a.kv_shift + ((int)blockIdx.y < a.kv_shift ? (int)gridDim.y : 0)) * RPC + sub;
   // (a token's own offsets are 32-bit: the entry point checks)
   const T* q_src = static_cast<const T*>(a.q) + (int64_t)t * a.ldq;
-  T* q_dst = static_cast<T*>(a.q_out) + (int64_t)t * a.ldqo;
+  TO* q_dst = static_cast<TO*>(a.q_out) + (int64_t)t * a.ldqo;
   auto load_kv = [&](int r) {
     const T* src = r < a.n_kv ? static_cast<const T*>(a.k) + (int64_t)t * a.ldk : static_cast<const T*>(a.v) + (int64_t)t * a.ldv;
     return load(src, (r < a.n_kv ? r : r - a.n_kv) * a.hd);
@@ -253,12 +255,12 @@ __global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 5 : 3) rope_kv_wr
       if constexpr (!VEC) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          q_dst[at + first_of(4 * l + j)] = from_f32<T>(x[j]);
-          q_dst[at + second_of(4 * l + j)] = from_f32<T>(x[4 + j]);
+          q_dst[at + first_of(4 * l + j)] = from_f32<TO>(x[j]);
+          q_dst[at + second_of(4 * l + j)] = from_f32<TO>(x[4 + j]);
         }
       } else {
-        const Quad<T> y0 = quad_of<T>(x), y1 = quad_of<T>(x + 4);
-        if constexpr (INTER && sizeof(T) == 2) {
+        const Quad<TO> y0 = quad_of<TO>(x), y1 = quad_of<TO>(x + 4);
+        if constexpr (INTER && sizeof(TO) == 2) {
           *reinterpret_cast<uint4*>(q_dst + (at + lo)) = make_uint4(y0.w[0], y0.w[1], y1.w[0], y1.w[1]);
         } else {
           store_quad(q_dst + (at + lo), y0);
@@ -410,7 +412,7 @@ static bool blocks_overlap(int64_t extent, std::array<std::pair<int64_t, int64_t
   return false;
 }
 
-template <typename T, bool INTER, bool VEC>
+template <typename T, typename TO, bool INTER, bool VEC>
 int launch_write_q8(WriteQ8Args& a, int64_t T_rows, cudaStream_t stream) {
   const int lanes = a.hd / 8;
   auto go = [&](auto kern, int lpr) {
@@ -426,16 +428,18 @@ int launch_write_q8(WriteQ8Args& a, int64_t T_rows, cudaStream_t stream) {
     return launch_kernel("rope_kv_write_q8_kernel", kern, dim3((unsigned)T_rows, (unsigned)gy), dim3(256), 0, stream,
                          1, 1, a);
   };
-  if (lanes <= 2) return go(rope_kv_write_q8_kernel<T, 2, INTER, VEC>, 2);
-  if (lanes <= 4) return go(rope_kv_write_q8_kernel<T, 4, INTER, VEC>, 4);
-  if (lanes <= 8) return go(rope_kv_write_q8_kernel<T, 8, INTER, VEC>, 8);
-  return go(rope_kv_write_q8_kernel<T, 16, INTER, VEC>, 16);
+  if (lanes <= 2) return go(rope_kv_write_q8_kernel<T, TO, 2, INTER, VEC>, 2);
+  if (lanes <= 4) return go(rope_kv_write_q8_kernel<T, TO, 4, INTER, VEC>, 4);
+  if (lanes <= 8) return go(rope_kv_write_q8_kernel<T, TO, 8, INTER, VEC>, 8);
+  return go(rope_kv_write_q8_kernel<T, TO, 16, INTER, VEC>, 16);
 }
-template <typename T>
+template <typename T, typename TO>
 int launch_write_q8(WriteQ8Args& a, bool vec, int64_t T_rows, cudaStream_t stream) {
   if (a.interleaved)
-    return vec ? launch_write_q8<T, true, true>(a, T_rows, stream) : launch_write_q8<T, true, false>(a, T_rows, stream);
-  return vec ? launch_write_q8<T, false, true>(a, T_rows, stream) : launch_write_q8<T, false, false>(a, T_rows, stream);
+    return vec ? launch_write_q8<T, TO, true, true>(a, T_rows, stream)
+               : launch_write_q8<T, TO, true, false>(a, T_rows, stream);
+  return vec ? launch_write_q8<T, TO, false, true>(a, T_rows, stream)
+             : launch_write_q8<T, TO, false, false>(a, T_rows, stream);
 }
 
 }  // namespace ssd
@@ -460,7 +464,11 @@ int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk,
     return fail(SSD_ERR_INVALID, "%s: rot_dim must be even, 0 .. head_dim", who);
   if (rot_dim && (!rope_cos || !rope_sin || !positions || max_pos <= 0))
     return fail(SSD_ERR_INVALID, "%s: rotation needs tables and positions", who);
-  if (dtype != SSD_F32 && dtype != SSD_BF16) return fail(SSD_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+  const int out_dtype = dtype & ~SSD_ROWS_F32;
+  if (out_dtype != SSD_F32 && out_dtype != SSD_BF16) return fail(SSD_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+  const bool rows_f32 = out_dtype == SSD_F32 || (dtype & SSD_ROWS_F32);
+  if (q && q == q_out && rows_f32 && out_dtype == SSD_BF16)
+    return fail(SSD_ERR_INVALID, "%s: fp32 rows cannot be rotated in place into bf16", who);
   if (T > 1 && ((q && (ldq < n_heads * hd || ldqo < n_heads * hd)) || ldk < cache->n_kv_heads * hd ||
                 ldv < cache->n_kv_heads * hd))
     return fail(SSD_ERR_INVALID, "%s: rows overlap", who);
@@ -491,12 +499,13 @@ int ssd_rope_kv_write_q8(const void* q, int64_t ldq, const void* k, int64_t ldk,
   a.q_out = q_out;
   a.ldqo = ldqo;
   a.status = status;
-  const int64_t es = dtype == SSD_F32 ? 4 : 2;
+  const int64_t es = rows_f32 ? 4 : 2, es_out = out_dtype == SSD_F32 ? 4 : 2;
   const bool vec = rot_dim % 8 == 0 && aligned16(rope_cos, 0) && aligned16(rope_sin, 0) && aligned16(k, ldk * es) &&
                    aligned16(v, ldv * es) &&
-                   (!q || (aligned16(q, ldq * es) && aligned16(q_out, ldqo * es)));
+                   (!q || (aligned16(q, ldq * es) && aligned16(q_out, ldqo * es_out)));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == SSD_F32 ? launch_write_q8<float>(a, vec, T, s) : launch_write_q8<bf16>(a, vec, T, s);
+  if (out_dtype == SSD_F32) return launch_write_q8<float, float>(a, vec, T, s);
+  return rows_f32 ? launch_write_q8<float, bf16>(a, vec, T, s) : launch_write_q8<bf16, bf16>(a, vec, T, s);
 }
 
 int ssd_kv_read_q8(const SsdKvQ8* cache, const int32_t* slots, int64_t first, int64_t n, void* k_out, int64_t ldk,

@@ -51,6 +51,7 @@ class SsdKvQ8(C.Structure):
 
 
 EPI_QKV = 16
+ROWS_F32 = 16  # or'ed into ssd_rope_kv_write_q8's dtype: fp32 rows, bf16 q_out
 CHAIN_MAX = 6
 
 TP_MAX_RANKS = 8

@@ -6,8 +6,9 @@ Per layer (all launches on the current stream, no host syncs):
   rmsnorm -> QKV GEMM (+RoPE, K/V written into the cache) -> tree attention
   -> o_proj GEMM (+residual) -> rmsnorm -> gate/up GEMM (+SwiGLU)
   -> down GEMM (+residual)
-Over an 8-bit cache the q/k/v GEMM writes plain rows, which one kernel then
-rotates and quantises into the cache, and attention reads the 8-bit rows.
+Over an 8-bit cache the q/k/v GEMM writes its fp32 sums, which one kernel then
+rotates (q, rounded once, as in the fused epilogue) and quantises into the
+cache, and attention reads the 8-bit rows.
 The residual stream is fp32; GEMM operands use the weights' dtype (bf16:
 tcgen05 tensor cores, fp32: CUDA cores). Every buffer is allocated once and
 reused, so a forward can be captured in a CUDA graph.
@@ -227,10 +228,10 @@ class Scratch:
         return t
 
     def qkv(self, rows: int) -> torch.Tensor:
-        """q | k | v rows of a forward over an 8-bit cache (before the rotation)."""
+        """q | k | v rows (fp32) of a forward over an 8-bit cache, before the rotation."""
         if self._qkv is None:
             w = self.w
-            self._qkv = torch.zeros(self.rows, (w.H + 2 * w.Hkv) * w.hd, dtype=w.dtype, device=w.device)
+            self._qkv = torch.zeros(self.rows, (w.H + 2 * w.Hkv) * w.hd, dtype=torch.float32, device=w.device)
         return self._qkv[:rows]
 
     def reserve_bridges(self, bridges) -> None:
@@ -298,7 +299,7 @@ def run_layer(w: ModelWeights, li: int, fwd: ForwardInputs, T: int, cache, scrat
     ops.rmsnorm(resid, lw.ln1, lw.eps1, xn)
     if cache.quantized:
         qkv = scratch.qkv(T)
-        ops.linear(xn, [lw.q, lw.k, lw.v], ws, out=qkv)
+        ops.linear(xn, [lw.q, lw.k, lw.v], ws, epilogue=L.EPI_STORE_F32, out=qkv)
         write_kv_q8(w, qkv, fwd, T, cache.layer_q8(li), scratch, ws)
     else:
         kc, vc = cache.layer(li)
@@ -383,7 +384,7 @@ def run_stack_folded(w: ModelWeights, layer_indices, pre_layer_bridges, pre_norm
         lw = w.layers[li]
         if cache.quantized:
             qkv = scratch.qkv(T)
-            chain.linear(xg, [lw.q, lw.k, lw.v], out=qkv, in_norm=in_for(k))
+            chain.linear(xg, [lw.q, lw.k, lw.v], epilogue=L.EPI_STORE_F32, out=qkv, in_norm=in_for(k))
             chain.flush()
             write_kv_q8(w, qkv, fwd, T, cache.layer_q8(li), scratch, ws)
         else:

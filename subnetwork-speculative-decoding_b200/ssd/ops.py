@@ -337,8 +337,9 @@ def rope_kv_write_q8(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor
     [max_pos, rot_dim / 2] fp32 (None: no rotation). rot_dim: how many elements
     of a head turn (default: twice the tables' width); interleaved: pairs
     (2i, 2i + 1) instead of (i, i + rot_dim / 2). q None: cache write only;
-    q_out may be q. The slots of one call must be distinct. Bad slots and
-    positions are reported by ws.check_status()."""
+    q_out may be q, or bf16 of fp32 rows (a projection's accumulators, which
+    are then rounded once). The slots of one call must be distinct. Bad slots
+    and positions are reported by ws.check_status()."""
     T = k.shape[0] if T is None else T
     dev, dt = layer.index, k.dtype
     if n_kv != layer.n_kv or head_dim != layer.head_dim:
@@ -355,13 +356,20 @@ def rope_kv_write_q8(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor
     pq, ldq = _q8_rows("q", q, dt, dev, T, n_heads * head_dim)
     pk, ldk = _q8_rows("k", k, dt, dev, T, n_kv * head_dim)
     pv, ldv = _q8_rows("v", v, dt, dev, T, n_kv * head_dim)
-    po, ldo = _q8_rows("q_out", q_out if q is not None else None, dt, dev, T, n_heads * head_dim)
     f32, i32 = torch.float32, torch.int32
+    code = dtype_code(dt)
+    if q is None:
+        po, ldo = None, 0
+    elif dt is f32 and q_out.dtype is torch.bfloat16:
+        code = L.SSD_BF16 | L.ROWS_F32
+        po, ldo = _q8_rows("q_out", q_out, torch.bfloat16, dev, T, n_heads * head_dim)
+    else:
+        po, ldo = _q8_rows("q_out", q_out, dt, dev, T, n_heads * head_dim)
     _q8_call("ssd_rope_kv_write_q8", dev, pq, ldq, pk, ldk, pv, ldv, T, n_heads,
              _q8_ptr("cos", cos, f32, dev, 0) if rot_dim else None, _q8_ptr("sin", sin, f32, dev, 0) if rot_dim else None,
              max_pos, rot_dim, 1 if interleaved else 0,
              _q8_ptr("positions", positions, i32, dev, T) if rot_dim else None, _q8_ptr("slots", slots, i32, dev, T),
-             layer._ref, po, ldo, dtype_code(dt), _q8_status(ws, dev))
+             layer._ref, po, ldo, code, _q8_status(ws, dev))
 
 
 def kv_read_q8(layer: KVLayerQ8, slots: Optional[torch.Tensor], k_out: Optional[torch.Tensor],

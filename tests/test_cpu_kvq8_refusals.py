@@ -72,3 +72,11 @@ def test_the_longest_cache_fits_32_bits_rounded_up():
 def test_a_read_range_that_wraps_around_is_refused(first, n):
     with pytest.raises(ValueError, match="outside the cache"):
         read(first=first, n=n)
+
+
+# ----------------------------------------------------------------- writing
+@pytest.mark.parametrize("fields,exc", [(dict(dtype=16 | 2), L.SSDError), (dict(dtype=32 | 1), L.SSDError),
+                                        (dict(dtype=-1), L.SSDError), (dict(dtype=16 | 1), ValueError)])
+def test_write_refuses_unknown_types_and_fp32_rows_turned_in_place_into_bf16(fields, exc):
+    with pytest.raises(exc):
+        write(**fields)  # (q and q_out are one address here)
