@@ -389,9 +389,11 @@ constexpr int kQ8BarSoftmax = 8, kQ8BarHelpers = 9;  // named barriers (1 .. 5: 
 // Column chunks of 16 -> chunks per warpgroup, warpgroups that share a block,
 // sets of them that take blocks in turn: as many warpgroups as registers and
 // TMEM allow (up to four; three where l takes 48 registers), as sets where a
-// block's columns do not fill them. Measured over 32k keys of 8 heads, us: 32
-// rows a head {2, 1, 4} 31.6, {2, 1, 2} 32.2; 36 rows {2, 2, 2} 34, {2, 2, 1} 38, {3, 1, 1}
-// 45; 88 rows {2, 3, 1} 47, {3, 2, 1} 52; 120 rows {2, 4, 1} 57, {3, 3, 1} 61.
+// block's columns do not fill them. Measured over 32k keys of 8 heads, us: 36 rows a
+// head {2, 2, 2} 35.4, {2, 2, 1} 41.4, {3, 1, 1} 48.2; 88 rows {2, 3, 1} 50.6, {3, 2, 1}
+// 54.8; 120 rows {2, 4, 1} 61.5, {3, 3, 1} 65.1. Up to 32 rows {2, 1, 4} and {2, 1, 2}
+// come out even: 20 rows 31.0 and 31.7, 32 rows 33.4 and 31.9, heads of 64 27.7
+// and 28.7, 340 slots 10.0 and 10.7, but 8k keys 20.0 and 17.8.
 // P' has a buffer a set. A set alone of up to 96 columns has a second one: over few
 // key blocks the softmax would wait for the first values (33 rows over 2k keys,
 // 80 columns: 18.4 us with two, 20.0 with one). Of 128 columns one does: 2k prefill
@@ -1420,10 +1422,10 @@ __global__ void __launch_bounds__(CH == 3 ? 512 : 640, 1)
 
 // The join as a launch of its own, one warp a row. With up to 16 query rows
 // the last CTA of a column joins its records itself, which the device hardly
-// notices (one token over 2k keys: 12.0 us against 12.1 replayed from a graph)
-// but the host does: 13.6 -> 11.9 us launched call by call, where the second
-// launch was the bound. With 48 rows over 32k keys, 18 slices, the one CTA
-// takes 1.8 us longer than the launch (39.7 us against 37.9).
+// notices (one token over 2k keys: 11.2 us against 11.6 replayed from a graph)
+// but the host does: 13.6 -> 12.1 us launched call by call, where the second
+// launch was the bound. With 36 rows over 32k keys, 18 slices, the one CTA
+// takes 2.4 us longer than the launch (37.8 us against 35.4).
 template <int HD>
 __global__ void __launch_bounds__(256) attn_q8_join_kernel(const AttnQ8Args a, const int tok_per_group) {
   pdl_wait();
@@ -1453,16 +1455,16 @@ static int q8_tensor_map(const void* base, const SsdKvQ8& c, CUtensorMap* out) {
 }
 
 // Query rows in groups of whole tokens, evenly, and key slices: one CTA per SM,
-// slices of at least two key blocks (one block each: 25 us against 19 for 33
-// tokens over 2k keys), and no join at all for as many blocks as the warpgroup
-// sets, or one more, take side by side (one token over 350 slots 7.9 us in one
-// slice, 9.4 in two; 600 slots 9.2 and 10.0 in three; 1100 slots 11.5 and 10.2 in
+// slices of at least two key blocks (one block each: 12.4 us against 11.2 for one
+// token over 2k keys), and no join at all for as many blocks as the warpgroup
+// sets, or one more, take side by side (one token over 340 slots 8.8 us in one
+// slice, 10.2 in two; 600 slots 10.2 and 10.3 in three; 1100 slots 13.8 and 10.5 in
 // five). Groups of up to 144 rows or of up to 128, whichever the
 // estimate takes for shorter: key blocks of a CTA, and two for the queries and
 // the results, x the measured time of one at that many columns, in 30 ns. (144
-// against 128 rows of 8 heads, us: 2048 tokens 125 and 114; 65 tokens over 2k
-// keys 23.7 and 20.4, 33 tokens 19.1 and 18.0, as SMs are left; 65 tokens over
-// 32k keys 100 and 102, as they fill two groups but not three; 33 tokens 64 and 68.)
+// against 128 rows of 8 heads, us: 2048 tokens 128 and 118; 65 tokens over 2k
+// keys 23.7 and 20.3, 33 tokens 19.4 and 17.7, as SMs are left; 65 tokens over
+// 32k keys 101 and 108, as they fill two groups but not three; 33 tokens 67 and 74.)
 struct Q8Plan {
   int tiles, tokens, chunks, key_blocks;
   int64_t splits;
